@@ -1,0 +1,920 @@
+// decay_attn.hip - linear attention with a decay for each head (include/humanoid_env.h hum_decay_attn*): the memory of
+// a recurrent policy beside policy.hip's network.  Per lane and head, with S [dv, dk] in float32:
+//
+//     S_t = a_t S_{t-1} + v_t k_t^T,   o_t = scale S_t q_t,   a_t = 0 at an episode's first step, else lambda_h
+//
+// Unrolled, o_t = scale (sum_{s <= t} D[t, s] (q_t . k_s) v_s + lambda^{t+1} S_0 q_t) with D[t, s] = lambda^{t-s} inside
+// one episode and 0 across two.  The gradients have the same form with the operands' roles changed:
+//
+//     dq_t = scale sum_{s <= t} D[t, s] (do_t . v_s) k_s + ...     forwards,  state sum v k^T
+//     dk_s = scale sum_{t >= s} D[t, s] (v_s . do_t) q_t + ...     backwards, state sum do q^T
+//     dv_s = scale sum_{t >= s} D[t, s] (k_s . q_t) do_t + ...     backwards, the same state transposed
+//
+// so one kernel, the walk out = walk(x, y, z) with the state sum y z^T, computes all four (struct Role).
+//
+// The walk goes over chunks of 32 steps.  Inside a chunk it is products of small matrices on the matrix cores:
+// P = (Y X^T) masked and weighted by D, O^T = Z^T P + S^T X^T, S = lambda^32 S + (w Y)^T Z.  One wave owns one (lane,
+// head, slice of z's channels) and keeps that slice of S in its accumulators for the whole walk; P and S never leave
+// registers, because the rows of every A operand are taken in the order
+//     matrix row m of tile a  <->  index 8 (m >> 2) + 4 a + (m & 3)   (of 32)
+// under which the accumulators of a pair of tiles (lane group g holds rows 4 g .. 4 g + 3 of each) are exactly the 8
+// consecutive contraction indexes 8 g .. 8 g + 7 that lane group needs as an operand of the next product.  Only Y^T and
+// Z^T (contraction over the steps) go through LDS, read back transposed.
+//
+// Rounding.  Products of bf16 inputs are exact in the float32 accumulators.  Computed operands are split into bf16
+// parts that sum to them: P and the state read by O into two (2^-18 of the value, under the output's own 2^-9), the
+// weighted Y that enters the state into three (2^-26, below float32's 2^-24: the state is held in 32 bits).  float32 and
+// float16 inputs use the float32 matrix instruction (16 times slower, 153 TFLOP/s on this card) and are not split.
+//
+// Non-finite values.  A row of Z multiplies zeros of P for the steps that must not see it (earlier steps, other
+// episodes), and 0 x inf is NaN: a chunk whose z rows hold one is walked step by step with the unseen rows zeroed, so
+// an episode that diverged leaves the next one, and its own earlier steps, untouched.
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+#include <cstdint>
+#include <cstdio>
+
+#include "../../include/humanoid_env.h"
+
+void hum_internal_set_error(const char* msg);
+
+namespace {
+
+constexpr int CH = 32;             // steps per chunk: the contraction length of one bf16 matrix instruction
+constexpr int MAX_D = 128;         // channels per head
+constexpr int XCDS = 8;            // consecutive workgroups go to different XCDs
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+
+struct Rows {               // [lane, step, head, channel] with unit channel stride
+    void* p;
+    long lane, step, head;  // strides in elements
+    int shared;             // heads that read one of its heads
+    int vec;                // 16-byte loads of 8 channels are aligned
+};
+
+struct Role {
+    Rows x, y, z, out;
+    int dy, dz;             // channels of x, y and of z, out
+    int rev;                // walks from the last step to the first
+    int out_f32;            // float32 partial results (shared heads' gradients), summed by a second launch
+    float s_pair, s_in, s_add;   // the scale's place: on the pairs, on what the entering state gives, on what joins it
+    const float* state_in;  // element (y channel i, z channel j) at i sy + j sz; NULL = zeros
+    float* state_out;       // NULL = not wanted
+    long sy, sz, s_lane;    // s_lane: from one (lane, head) to the next
+    int s_vec;              // sy == 1 and 16-byte aligned rows
+    int slice0;             // first workgroup part of this role
+};
+
+struct WalkArgs {
+    Role r[3];
+    int nroles, parts;
+    int lanes, steps, heads;
+    const float* log_decay;
+    const unsigned char* reset;
+    long reset_lane, reset_step;
+    const int* lengths;
+};
+
+// ---- the element types: ST storage, operands of 8 consecutive contraction indexes per lane
+template <int ST> struct Num;   // HUM_F32 / HUM_F16: float32 matrix instructions
+
+template <> struct Num<HUM_BF16> {
+    typedef bf16x8 Op;
+    typedef __bf16 Elem;
+    static constexpr int PAD = 8, PARTS = 3;
+    static __device__ __forceinline__ Op zero() { return Op{}; }
+    static __device__ __forceinline__ Op load(const void* p, long off, int n, bool vec) {
+        const __bf16* e = (const __bf16*)p + off;
+        if (vec) return *(const Op*)e;
+        Op v = {};
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if (j < n) v[j] = e[j];
+        return v;
+    }
+    static __device__ __forceinline__ void store(void* p, long off, int n, bool vec, f32x8 v) {
+        __bf16* e = (__bf16*)p + off;
+        const Op o = __builtin_convertvector(v, Op);   // to nearest, ties to even
+        if (vec) { *(Op*)e = o; return; }
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if (j < n) e[j] = o[j];
+    }
+    static __device__ __forceinline__ bool finite(Op v) {
+        const u32x4 u = __builtin_bit_cast(u32x4, v);
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < 4; i++) bad |= (u[i] & 0x7f80u) == 0x7f80u || (u[i] & 0x7f800000u) == 0x7f800000u;
+        return !bad;
+    }
+    static __device__ __forceinline__ void mma(f32x4& c, Op a, Op b) {
+        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    }
+    // v as N bf16 parts: each the rounding of what the ones before leave
+    template <int N>
+    static __device__ __forceinline__ void split(f32x8 v, Op (&o)[N]) {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            o[i] = __builtin_convertvector(v, Op);
+            if (i + 1 < N) v -= __builtin_convertvector(o[i], f32x8);
+        }
+    }
+    static __device__ __forceinline__ f32x8 wide(Op a) { return __builtin_convertvector(a, f32x8); }
+    // rows s0 .. s0 + 7 of column c (4 columns per quarter of 16 lanes: the transposing LDS load)
+    static __device__ __forceinline__ void put(Elem* m, Op v) { *(Op*)m = v; }
+    static __device__ __forceinline__ Op column(const Elem* m, int pitch, int s0, int c0, int r) {
+        typedef __attribute__((address_space(3))) bf16x4 L4;
+        const Elem* p = m + (s0 + (r >> 2)) * pitch + c0 + 8 * (r & 3);
+        const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((L4*)p);
+        const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((L4*)(p + 4 * pitch));
+        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+};
+
+template <int ST> struct Num {
+    typedef f32x8 Op;
+    typedef float Elem;
+    static constexpr int PAD = 4, PARTS = 1;
+    static __device__ __forceinline__ Op zero() { return Op{}; }
+    static __device__ __forceinline__ Op load(const void* p, long off, int n, bool vec) {
+        if constexpr (ST == HUM_F16) {
+            const _Float16* e = (const _Float16*)p + off;
+            if (vec) return __builtin_convertvector(*(const f16x8*)e, Op);
+            Op v = {};
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (j < n) v[j] = (float)e[j];
+            return v;
+        } else {
+            const float* e = (const float*)p + off;
+            if (vec) {
+                const f32x4 a = *(const f32x4*)e, b = *(const f32x4*)(e + 4);
+                return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+            }
+            Op v = {};
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (j < n) v[j] = e[j];
+            return v;
+        }
+    }
+    static __device__ __forceinline__ void store(void* p, long off, int n, bool vec, f32x8 v) {
+        if constexpr (ST == HUM_F16) {
+            _Float16* e = (_Float16*)p + off;
+            const f16x8 o = __builtin_convertvector(v, f16x8);
+            if (vec) { *(f16x8*)e = o; return; }
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (j < n) e[j] = o[j];
+        } else {
+            float* e = (float*)p + off;
+            if (vec) {
+                *(f32x4*)e = __builtin_shufflevector(v, v, 0, 1, 2, 3);
+                *(f32x4*)(e + 4) = __builtin_shufflevector(v, v, 4, 5, 6, 7);
+                return;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (j < n) e[j] = v[j];
+        }
+    }
+    static __device__ __forceinline__ bool finite(Op v) {
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < 8; i++) bad |= (__builtin_bit_cast(unsigned, (float)v[i]) & 0x7f800000u) == 0x7f800000u;
+        return !bad;
+    }
+    static __device__ __forceinline__ void mma(f32x4& c, Op a, Op b) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
+    }
+    template <int N>
+    static __device__ __forceinline__ void split(f32x8 v, Op (&o)[N]) { o[0] = v; }
+    static __device__ __forceinline__ f32x8 wide(Op a) { return a; }
+    static __device__ __forceinline__ void put(Elem* m, Op v) {
+        *(f32x4*)m = __builtin_shufflevector(v, v, 0, 1, 2, 3);
+        *(f32x4*)(m + 4) = __builtin_shufflevector(v, v, 4, 5, 6, 7);
+    }
+    static __device__ __forceinline__ Op column(const Elem* m, int pitch, int s0, int c0, int r) {
+        const Elem* p = m + s0 * pitch + c0 + 8 * (r >> 2) + (r & 3);
+        Op v;
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = p[j * pitch];
+        return v;
+    }
+};
+
+__device__ __forceinline__ f32x8 pair(f32x4 a, f32x4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
+
+// LDS operations of one wave execute in order; this keeps the compiler from moving them past each other
+__device__ __forceinline__ void lds_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// One wave per workgroup.  DY, DZ: channels of y and of the z slice rounded up to 32.
+template <int ST, int DY, int DZ>
+__global__ void __launch_bounds__(64) walk_kernel(WalkArgs a) {
+    typedef Num<ST> M;
+    typedef typename M::Op Op;
+    constexpr int KY = DY / 32, KZ = DZ / 32;
+    constexpr int PO = M::PARTS > 1 ? 2 : 1;   // parts of P and of the state's reading
+    constexpr int PS = M::PARTS;               // parts of what joins the state
+    constexpr int PY = DY + M::PAD, PZ = DZ + M::PAD;
+    __shared__ __attribute__((aligned(16))) typename M::Elem ly[CH * PY];
+    __shared__ __attribute__((aligned(16))) typename M::Elem lz[CH * PZ];
+
+    const int l = threadIdx.x, g = l >> 4, r = l & 15;
+    // the parts (roles, slices) of one (lane, head) read the same rows: they go to one XCD, one after the other
+    const int block = blockIdx.x, part = block / XCDS % a.parts;
+    const int unit = block / (XCDS * a.parts) * XCDS + block % XCDS;
+    if (unit >= a.lanes * a.heads) return;
+    const int ri = (a.nroles > 1 && part >= a.r[1].slice0) + (a.nroles > 2 && part >= a.r[2].slice0);
+    const Role& R = a.r[ri];
+    const int dz0 = (part - R.slice0) * DZ;
+    const int b = unit / a.heads, h = unit - b * a.heads;
+    const int steps = a.steps;
+    int len = steps;
+    if (a.lengths) {
+        len = a.lengths[b];
+        len = len < 0 ? 0 : len > steps ? steps : len;
+    }
+    const int rev = R.rev;
+    const float lg = a.log_decay[h] * 1.44269504088896340736f;
+    auto power = [&](int n) { return n == 0 ? 1.f : __builtin_amdgcn_exp2f(lg * (float)n); };
+
+    // ---- the entering state: tile (i, j) holds y channels 32 (i / 2) + 8 g + 4 (i & 1) + 0..3 of z channel zc(j)
+    f32x4 S[2 * KY][2 * KZ];
+    auto zc = [&](int j) { return dz0 + 32 * (j >> 1) + 8 * (r >> 2) + 4 * (j & 1) + (r & 3); };
+    {
+        const float* s = R.state_in ? R.state_in + (long)unit * R.s_lane : nullptr;
+#pragma unroll
+        for (int j = 0; j < 2 * KZ; j++)
+#pragma unroll
+            for (int i = 0; i < 2 * KY; i++) {
+                const int y0 = 32 * (i >> 1) + 8 * g + 4 * (i & 1), z = zc(j);
+                f32x4 v = {0.f, 0.f, 0.f, 0.f};
+                if (s && z < R.dz) {
+                    if (R.s_vec) {
+                        if (y0 < R.dy) v = *(const f32x4*)(s + (long)z * R.sz + y0);
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < 4; q++)
+                            if (y0 + q < R.dy) v[q] = s[(long)z * R.sz + (long)(y0 + q) * R.sy];
+                    }
+                }
+                S[i][j] = v;
+            }
+    }
+
+    // ---- what a chunk's weights depend on besides its marks
+    float w_pair[2][8];   // step t = 16 c + r of the walk, step s = 8 g + j: lambda^(t - s) for s <= t
+#pragma unroll
+    for (int c = 0; c < 2; c++)
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const int d = 16 * c + r - (8 * g + j);
+            w_pair[c][j] = d < 0 ? 0.f : R.s_pair * power(d);
+        }
+    float w_in[2];
+#pragma unroll
+    for (int c = 0; c < 2; c++) w_in[c] = R.s_in * power(16 * c + r + 1 - rev);
+
+    const long xo = (long)b * R.x.lane + (long)(h / R.x.shared) * R.x.head;
+    const long yo = (long)b * R.y.lane + (long)(h / R.y.shared) * R.y.head;
+    const long zo = (long)b * R.z.lane + (long)(h / R.z.shared) * R.z.head;
+    const long oo = (long)b * R.out.lane + (long)(h / R.out.shared) * R.out.head;
+    const unsigned char* marks = a.reset ? a.reset + (long)b * a.reset_lane : nullptr;
+    auto row_of = [&](int tile) { return 8 * (r >> 2) + 4 * tile + (r & 3); };
+
+    for (int n0 = 0; n0 < len; n0 += CH) {
+        const int L = len - n0 < CH ? len - n0 : CH;
+        auto time = [&](int n) { return rev ? len - 1 - (n0 + n) : n0 + n; };
+        // ---- rows: x by walk step 16 c + r, y and z by step row_of(a)
+        Op X[2][KY], Y[2][KY], Z[2][KZ];
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+            const int n = 16 * c + r;
+            const long at = xo + (long)time(n) * R.x.step;
+#pragma unroll
+            for (int k = 0; k < KY; k++) {
+                const int d = 32 * k + 8 * g;
+                X[c][k] = n < L && d < R.dy ? M::load(R.x.p, at + d, R.dy - d, R.x.vec) : M::zero();
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            const int n = row_of(t);
+            const long aty = yo + (long)time(n) * R.y.step, atz = zo + (long)time(n) * R.z.step;
+#pragma unroll
+            for (int k = 0; k < KY; k++) {
+                const int d = 32 * k + 8 * g;
+                Y[t][k] = n < L && d < R.dy ? M::load(R.y.p, aty + d, R.dy - d, R.y.vec) : M::zero();
+            }
+#pragma unroll
+            for (int k = 0; k < KZ; k++) {
+                const int d = dz0 + 32 * k + 8 * g;
+                Z[t][k] = n < L && d < R.dz ? M::load(R.z.p, atz + d, R.dz - d, R.z.vec) : M::zero();
+            }
+        }
+        // ---- marks: bit j separates walk steps j - 1 and j (bit 0 the entering state, bit L the leaving one).  An
+        // episode's first step is cut off from what time puts before it, so the backward walk has it one later.
+        unsigned long long cut = 0;
+        if (marks) {
+            const int n = l - rev;
+            const bool m = n >= 0 && n < L && marks[(long)time(n) * a.reset_step] != 0;
+            cut = __ballot(m);
+        }
+        bool sane = true;
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int k = 0; k < KZ; k++) sane = sane && M::finite(Z[t][k]);
+        const bool slow = __any(!sane);
+
+        auto upto = [&](int j) { return __builtin_popcountll(cut & ((2ull << j) - 1)); };   // cuts at or before step j
+        float wi[2], wo[8];
+        int ct[2], cs[8];
+        const int cl = __builtin_popcountll(cut);
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+            ct[c] = upto(16 * c + r);
+            wi[c] = ct[c] == 0 ? w_in[c] : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const int s = 8 * g + j;
+            cs[j] = upto(s);
+            wo[j] = s < L && cs[j] == cl ? R.s_add * power(L - 1 - s + rev) : 0.f;
+        }
+
+        // ---- P^T: rows s, columns t; masked entries are chosen away, not multiplied
+        Op P[2][PO];
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+            f32x4 p[2];
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                p[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < KY; k++) M::mma(p[t], Y[t][k], X[c][k]);
+            }
+            f32x8 v = pair(p[0], p[1]);
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[j] = w_pair[c][j] != 0.f && cs[j] == ct[c] ? v[j] * w_pair[c][j] : 0.f;
+            M::template split<PO>(v, P[c]);
+        }
+
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int k = 0; k < KY; k++) M::put(ly + row_of(t) * PY + 32 * k + 8 * g, Y[t][k]);
+
+        // ---- one pass over the chunk's steps, or one per step where a z row is not finite
+        for (int lo = 0; lo < L;) {
+            int hi = L, from = 0;
+            if (slow) {
+                hi = lo + 1;
+                const unsigned long long seen = cut & ((2ull << lo) - 1) & ~1ull;   // the last cut at or before lo
+                from = seen ? 63 - __builtin_clzll(seen) : 0;
+            }
+            lds_order();
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                const int n = row_of(t);
+#pragma unroll
+                for (int k = 0; k < KZ; k++)
+                    M::put(lz + n * PZ + 32 * k + 8 * g, n >= from && n < hi ? Z[t][k] : M::zero());
+            }
+            lds_order();
+            Op T[2 * KZ];   // Z^T
+#pragma unroll
+            for (int j = 0; j < 2 * KZ; j++) T[j] = M::column(lz, PZ, 8 * g, 32 * (j >> 1) + 4 * (j & 1), r);
+            // ---- O^T: rows z channels, columns t
+            if (R.out.p) {
+#pragma unroll
+                for (int k = 0; k < KZ; k++) {
+                    f32x4 o[2][2];
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const int j = 2 * k + e;
+#pragma unroll
+                        for (int c = 0; c < 2; c++) o[c][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int q = 0; q < KY; q++) {
+                            Op sp[PO];
+                            M::template split<PO>(pair(S[2 * q][j], S[2 * q + 1][j]), sp);
+#pragma unroll
+                            for (int u = 0; u < PO; u++)
+#pragma unroll
+                                for (int c = 0; c < 2; c++) M::mma(o[c][e], sp[u], X[c][q]);
+                        }
+#pragma unroll
+                        for (int c = 0; c < 2; c++) {
+#pragma unroll
+                            for (int q = 0; q < 4; q++) o[c][e][q] = ct[c] == 0 ? o[c][e][q] * wi[c] : 0.f;
+#pragma unroll
+                            for (int u = 0; u < PO; u++) M::mma(o[c][e], T[j], P[c][u]);
+                        }
+                    }
+                    const int d = dz0 + 32 * k + 8 * g;
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {
+                        const int n = 16 * c + r;
+                        if (n >= lo && n < hi && d < R.dz) {
+                            const long at = oo + (long)time(n) * R.out.step + d;
+                            if (R.out_f32) Num<HUM_F32>::store(R.out.p, at, R.dz - d, R.out.vec, pair(o[c][0], o[c][1]));
+                            else M::store(R.out.p, at, R.dz - d, R.out.vec, pair(o[c][0], o[c][1]));
+                        }
+                    }
+                }
+            }
+            // ---- the state behind the chunk
+            if (hi == L && (cut >> L & 1)) {   // an episode starts right behind (before, in time): nothing is left
+#pragma unroll
+                for (int i = 0; i < 2 * KY; i++)
+#pragma unroll
+                    for (int j = 0; j < 2 * KZ; j++) S[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            } else if (hi == L) {
+                const float through = power(L);
+#pragma unroll
+                for (int i = 0; i < 2 * KY; i++)
+#pragma unroll
+                    for (int j = 0; j < 2 * KZ; j++)
+#pragma unroll
+                        for (int q = 0; q < 4; q++) S[i][j][q] = cl == 0 ? S[i][j][q] * through : 0.f;
+#pragma unroll
+                for (int i = 0; i < 2 * KY; i++) {
+                    f32x8 v = M::wide(M::column(ly, PY, 8 * g, 32 * (i >> 1) + 4 * (i & 1), r));
+#pragma unroll
+                    for (int j = 0; j < 8; j++) v[j] = wo[j] != 0.f ? v[j] * wo[j] : 0.f;
+                    Op yp[PS];
+                    M::template split<PS>(v, yp);
+#pragma unroll
+                    for (int u = 0; u < PS; u++)
+#pragma unroll
+                        for (int j = 0; j < 2 * KZ; j++) M::mma(S[i][j], yp[u], T[j]);
+                }
+            }
+            lo = hi;
+        }
+        lds_order();
+    }
+
+    // ---- the steps behind the lane's length
+    if (R.out.p)
+        for (int n = len + r; n < steps; n += 16)
+#pragma unroll
+            for (int k = 0; k < KZ; k++) {
+                const int d = dz0 + 32 * k + 8 * g;
+                if (d < R.dz) {
+                    const long at = oo + (long)n * R.out.step + d;
+                    if (R.out_f32) Num<HUM_F32>::store(R.out.p, at, R.dz - d, R.out.vec, f32x8{});
+                    else M::store(R.out.p, at, R.dz - d, R.out.vec, f32x8{});
+                }
+            }
+    if (R.state_out) {
+        float* s = R.state_out + (long)unit * R.s_lane;
+#pragma unroll
+        for (int j = 0; j < 2 * KZ; j++)
+#pragma unroll
+            for (int i = 0; i < 2 * KY; i++) {
+                const int y0 = 32 * (i >> 1) + 8 * g + 4 * (i & 1), z = zc(j);
+                if (z >= R.dz) continue;
+                if (R.s_vec) {
+                    if (y0 < R.dy) *(f32x4*)(s + (long)z * R.sz + y0) = S[i][j];
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 4; q++)
+                        if (y0 + q < R.dy) s[(long)z * R.sz + (long)(y0 + q) * R.sy] = S[i][j][q];
+                }
+            }
+    }
+}
+
+// gradients of keys and values that `group` heads share: the sum of the heads' float32 partial results
+// part [lanes, steps, heads, d] -> out [lanes, steps, heads / group, d]; one thread per output channel
+template <int ST>
+__global__ void __launch_bounds__(256) share_kernel(const float* part, Rows out, long rows, int steps, int kv, int group, int d) {
+    for (long e = (long)blockIdx.x * 256 + threadIdx.x; e < rows * kv * d; e += (long)gridDim.x * 256) {
+        const int c = (int)(e % d);
+        const long row = e / d;          // (lane, step, kv head)
+        const int g = (int)(row % kv);
+        const long bt = row / kv;
+        float s = 0.f;
+        for (int i = 0; i < group; i++) s += part[((bt * kv + g) * group + i) * d + c];
+        const long at = bt / steps * out.lane + bt % steps * out.step + (long)g * out.head + c;
+        if constexpr (ST == HUM_F32) ((float*)out.p)[at] = s;
+        else if constexpr (ST == HUM_BF16) ((__bf16*)out.p)[at] = (__bf16)s;
+        else ((_Float16*)out.p)[at] = (_Float16)s;
+    }
+}
+
+// ---- single step: S = a S + v k^T, o = scale S q, all in float32 on the vector units - the state is read and written
+// once (8 bytes for 4 operations), so HBM bounds it.  LPR lanes of 4 key channels hold one row of S; a wave has
+// 64 / LPR rows in one load and U loads in flight.
+struct StepArgs {
+    Rows q, k, v, out;
+    const float* log_decay;
+    const float* state_in;
+    float* state_out;
+    const unsigned char* reset;
+    long reset_lane;
+    const unsigned char* active;
+    int heads, dk, dv, blocks;   // blocks: workgroups per (lane, head)
+    int s_vec;
+    float scale;
+    long units;
+};
+
+template <int ST>
+__device__ __forceinline__ float elem(const void* p, long at) {
+    if constexpr (ST == HUM_F32) return ((const float*)p)[at];
+    else if constexpr (ST == HUM_BF16) return (float)((const __bf16*)p)[at];
+    else return (float)((const _Float16*)p)[at];
+}
+
+template <int LPR>
+__device__ __forceinline__ float row_sum(float v) {   // over LPR neighbouring lanes, every one of them gets it
+    if constexpr (LPR > 1) v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0xB1, 0xf, 0xf, false));   // quad [1,0,3,2]
+    if constexpr (LPR > 2) v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x4E, 0xf, 0xf, false));   // quad [2,3,0,1]
+    if constexpr (LPR > 4) v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x141, 0xf, 0xf, false));  // mirror in 8
+    if constexpr (LPR > 8) v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x140, 0xf, 0xf, false));  // mirror in 16
+    if constexpr (LPR > 16) v += __shfl_xor(v, 16);
+    return v;
+}
+
+template <int ST, int LPR>
+__global__ void __launch_bounds__(256) step_kernel(StepArgs a) {
+    constexpr int U = 4, ROWS = 64 / LPR;
+    const long unit = blockIdx.x / a.blocks;
+    const int blk = (int)(blockIdx.x - unit * a.blocks);
+    const long b = unit / a.heads;
+    const int h = (int)(unit - b * a.heads);
+    const int wave = threadIdx.x >> 6, l = threadIdx.x & 63;
+    const int c0 = 4 * (l % LPR), row0 = (blk * 4 + wave) * U * ROWS + l / LPR;
+    const bool on = !a.active || a.active[b];
+    const bool fresh = a.reset && a.reset[b * a.reset_lane];
+    const float* si = a.state_in ? a.state_in + unit * a.dv * a.dk : nullptr;
+    float* so = a.state_out + unit * a.dv * a.dk;
+    const float lambda = __builtin_amdgcn_exp2f(a.log_decay[h] * 1.44269504088896340736f);
+    if (!on && si == so) si = nullptr;   // an idle lane's state in place stays as it is
+    f32x4 s[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int row = row0 + u * ROWS;
+        s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (row < a.dv && si && (!fresh || !on)) {
+            if (a.s_vec) {
+                if (c0 < a.dk) s[u] = *(const f32x4*)(si + (long)row * a.dk + c0);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (c0 + j < a.dk) s[u][j] = si[(long)row * a.dk + c0 + j];
+            }
+        }
+    }
+    const long qo = b * a.q.lane + (long)(h / a.q.shared) * a.q.head, ko = b * a.k.lane + (long)(h / a.k.shared) * a.k.head;
+    const long vo = b * a.v.lane + (long)(h / a.v.shared) * a.v.head, oo = b * a.out.lane + (long)h * a.out.head;
+    float q[4], k[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        q[j] = c0 + j < a.dk ? elem<ST>(a.q.p, qo + c0 + j) : 0.f;
+        k[j] = c0 + j < a.dk ? elem<ST>(a.k.p, ko + c0 + j) : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int row = row0 + u * ROWS;
+        float o = 0.f;
+        if (on) {
+            const float v = row < a.dv ? elem<ST>(a.v.p, vo + row) : 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                s[u][j] = c0 + j < a.dk ? s[u][j] * lambda + v * k[j] : 0.f;
+                o += s[u][j] * q[j];
+            }
+            o = row_sum<LPR>(o) * a.scale;
+        }
+        if (row < a.dv) {
+            if (on || si) {
+                if (a.s_vec) {
+                    if (c0 < a.dk) *(f32x4*)(so + (long)row * a.dk + c0) = s[u];
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        if (c0 + j < a.dk) so[(long)row * a.dk + c0 + j] = s[u][j];
+                }
+            } else if (a.state_in == nullptr) {   // idle and no state yet: an empty one
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (c0 + j < a.dk) so[(long)row * a.dk + c0 + j] = 0.f;
+            }
+            if (l % LPR == 0) {
+                if constexpr (ST == HUM_F32) ((float*)a.out.p)[oo + row] = o;
+                else if constexpr (ST == HUM_BF16) ((__bf16*)a.out.p)[oo + row] = (__bf16)o;
+                else ((_Float16*)a.out.p)[oo + row] = (_Float16)o;
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ host side
+int derr(int code, const char* fn, const char* m) {
+    char t[256];
+    std::snprintf(t, sizeof t, "%s: %s", fn, m);
+    hum_internal_set_error(t);
+    return code;
+}
+
+struct OnDevice {   // the caller's current device stays what it was
+    int old = -1;
+    bool ok;
+    explicit OnDevice(int d) { ok = hipGetDevice(&old) == hipSuccess && (old == d || hipSetDevice(d) == hipSuccess); }
+    ~OnDevice() {
+        int now = -1;
+        if (old >= 0 && hipGetDevice(&now) == hipSuccess && now != old) (void)hipSetDevice(old);
+    }
+};
+
+int elem_size(int type) { return type == HUM_F32 ? 4 : 2; }
+
+Rows rows_of(const hum_rows& r, int shared, int size, int d) {
+    const bool vec = ((uintptr_t)r.ptr | (uintptr_t)(r.lane * size) | (uintptr_t)(r.step * size) | (uintptr_t)(r.head * size)) % 16 == 0 && d % 8 == 0;
+    return Rows{r.ptr, (long)r.lane, (long)r.step, (long)r.head, shared, vec};
+}
+
+int check_args(const char* fn, const hum_decay_attn_args* p) {
+    if (!p) return derr(HUM_ERR_ARG, fn, "null argument");
+    if (p->type != HUM_F32 && p->type != HUM_BF16 && p->type != HUM_F16) return derr(HUM_ERR_ARG, fn, "unknown element type");
+    if (p->lanes < 0 || p->steps < 0 || p->heads < 1 || p->kv_heads < 1 || p->heads % p->kv_heads)
+        return derr(HUM_ERR_ARG, fn, "lanes and steps must be >= 0 and kv_heads must divide heads");
+    if (p->dk < 1 || p->dk > MAX_D || p->dv < 1 || p->dv > MAX_D)
+        return derr(HUM_ERR_ARG, fn, "dk and dv must be in [1, 128]");
+    if ((long)p->lanes * p->heads > (1l << 21)) return derr(HUM_ERR_ARG, fn, "lanes x heads must not pass 2^21");
+    if (!std::isfinite(p->scale)) return derr(HUM_ERR_ARG, fn, "scale must be finite");
+    if (p->lanes && (!p->log_decay)) return derr(HUM_ERR_ARG, fn, "log_decay is required");
+    if (p->lanes && p->steps && (!p->q.ptr || !p->k.ptr || !p->v.ptr)) return derr(HUM_ERR_ARG, fn, "q, k and v are required");
+    const hum_rows* all[3] = {&p->q, &p->k, &p->v};
+    for (const hum_rows* r : all)
+        if (((uintptr_t)r->ptr) % elem_size(p->type)) return derr(HUM_ERR_ARG, fn, "q, k and v must be aligned to their elements");
+    if (((uintptr_t)p->state_in | (uintptr_t)p->state_out | (uintptr_t)p->log_decay | (uintptr_t)p->lengths) % 4)
+        return derr(HUM_ERR_ARG, fn, "states, log_decay and lengths must be aligned to 4 bytes");
+    return HUM_OK;
+}
+
+int y_width(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
+// channels of z per workgroup: 64 (half as many waves form P twice), but 32 where float32 operands of 128 channels would
+// leave too few registers (a 128 x 64 state spills there)
+int z_slice(int type, int dy, int d) { return d <= 32 || (type != HUM_BF16 && y_width(dy) == 128) ? 32 : 64; }
+
+template <int ST, int DY>
+void launch_walk_z(const WalkArgs& a, int dzs, hipStream_t s) {
+    const long units = (long)a.lanes * a.heads;
+    const dim3 grid((unsigned)((units + XCDS - 1) / XCDS * XCDS * a.parts));
+    if constexpr (ST == HUM_BF16 || DY < 128)
+        if (dzs == 64) {
+            hipLaunchKernelGGL((walk_kernel<ST, DY, 64>), grid, dim3(64), 0, s, a);
+            return;
+        }
+    hipLaunchKernelGGL((walk_kernel<ST, DY, 32>), grid, dim3(64), 0, s, a);
+}
+template <int ST>
+void launch_walk_y(const WalkArgs& a, int dyw, int dzs, hipStream_t s) {
+    if (dyw == 32) launch_walk_z<ST, 32>(a, dzs, s);
+    else if (dyw == 64) launch_walk_z<ST, 64>(a, dzs, s);
+    else launch_walk_z<ST, 128>(a, dzs, s);
+}
+void launch_walk(int type, const WalkArgs& a, int dyw, int dzs, hipStream_t s) {
+    if (type == HUM_BF16) launch_walk_y<HUM_BF16>(a, dyw, dzs, s);
+    else if (type == HUM_F16) launch_walk_y<HUM_F16>(a, dyw, dzs, s);
+    else launch_walk_y<HUM_F32>(a, dyw, dzs, s);
+}
+
+// the roles of equal widths share a launch (their workgroups read the same rows at about the same time)
+void launch_roles(const hum_decay_attn_args* p, Role* r, int n, hipStream_t s) {
+    bool done[3] = {};
+    for (int i = 0; i < n; i++) {
+        if (done[i]) continue;
+        const int dyw = y_width(r[i].dy), dzs = z_slice(p->type, r[i].dy, r[i].dz);
+        WalkArgs a = {};
+        for (int j = i; j < n; j++) {
+            if (done[j] || y_width(r[j].dy) != dyw || z_slice(p->type, r[j].dy, r[j].dz) != dzs) continue;
+            done[j] = true;
+            r[j].slice0 = a.parts;
+            a.parts += (r[j].dz + dzs - 1) / dzs;
+            a.r[a.nroles++] = r[j];
+        }
+        a.lanes = p->lanes;
+        a.steps = p->steps;
+        a.heads = p->heads;
+        a.log_decay = p->log_decay;
+        a.reset = p->reset;
+        a.reset_lane = p->reset_lane;
+        a.reset_step = p->reset_step;
+        a.lengths = p->lengths;
+        launch_walk(p->type, a, dyw, dzs, s);
+    }
+}
+
+// a state [dv, dk] as the walk's sum over (y channel, z channel): y = keys' side or y = values' side
+void role_state(Role& r, const float* in, float* out, const hum_decay_attn_args* p, bool y_is_k) {
+    r.state_in = in;
+    r.state_out = out;
+    r.sy = y_is_k ? 1 : p->dk;
+    r.sz = y_is_k ? p->dk : 1;
+    r.s_lane = (long)p->dk * p->dv;
+    r.s_vec = y_is_k && p->dk % 4 == 0 && ((uintptr_t)in | (uintptr_t)out) % 16 == 0;
+}
+
+int launched(const char* fn) {
+    const hipError_t st = hipGetLastError();
+    return st == hipSuccess ? HUM_OK : derr(HUM_ERR_HIP, fn, hipGetErrorString(st));
+}
+
+}  // namespace
+
+extern "C" {
+
+int hum_decay_attn_workspace(const hum_decay_attn_args* p, int32_t backward, uint64_t* bytes) {
+    const char* fn = "hum_decay_attn_workspace";
+    if (const int rc = check_args(fn, p)) return rc;
+    if (!bytes) return derr(HUM_ERR_ARG, fn, "null argument");
+    *bytes = 0;
+    if (backward && p->kv_heads != p->heads)
+        *bytes = 4ull * p->lanes * p->steps * p->heads * (uint64_t)(p->dk + p->dv);
+    return HUM_OK;
+}
+
+int hum_decay_attn(const hum_decay_attn_args* p, const hum_rows* out, void* workspace, uint64_t workspace_bytes, void* stream) {
+    const char* fn = "hum_decay_attn";
+    if (const int rc = check_args(fn, p)) return rc;
+    if (!out || (p->lanes && p->steps && !out->ptr) || ((uintptr_t)out->ptr) % elem_size(p->type))
+        return derr(HUM_ERR_ARG, fn, "out is required, aligned to its elements");
+    uint64_t need = 0;
+    if (const int rc = hum_decay_attn_workspace(p, 0, &need)) return rc;
+    if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
+        return derr(HUM_ERR_ARG, fn, "the workspace is too small (hum_decay_attn_workspace) or not aligned to 16 bytes");
+    if (!p->lanes) return HUM_OK;
+    const OnDevice dev(p->device);
+    if (!dev.ok) return derr(HUM_ERR_HIP, fn, "hipSetDevice");
+    const int size = elem_size(p->type), group = p->heads / p->kv_heads;
+    Role r = {};
+    r.x = rows_of(p->q, 1, size, p->dk);
+    r.y = rows_of(p->k, group, size, p->dk);
+    r.z = rows_of(p->v, group, size, p->dv);
+    r.out = rows_of(*out, 1, size, p->dv);
+    r.dy = p->dk;
+    r.dz = p->dv;
+    r.s_pair = r.s_in = p->scale;
+    r.s_add = 1.f;
+    role_state(r, p->state_in, p->state_out, p, true);
+    launch_roles(p, &r, 1, (hipStream_t)stream);
+    return launched(fn);
+}
+
+int hum_decay_attn_backward(const hum_decay_attn_args* p, const hum_rows* d_out, const float* d_state_out,
+                            const hum_rows* dq, const hum_rows* dk, const hum_rows* dv, float* d_state_in, void* workspace,
+                            uint64_t workspace_bytes, void* stream) {
+    const char* fn = "hum_decay_attn_backward";
+    if (const int rc = check_args(fn, p)) return rc;
+    const hum_rows none = {};
+    const hum_rows& gq = dq ? *dq : none;
+    const hum_rows& gk = dk ? *dk : none;
+    const hum_rows& gv = dv ? *dv : none;
+    const int size = elem_size(p->type), group = p->heads / p->kv_heads;
+    if (!d_out || (p->lanes && p->steps && !d_out->ptr) || ((uintptr_t)d_out->ptr) % size)
+        return derr(HUM_ERR_ARG, fn, "d_out is required, aligned to its elements");
+    if (((uintptr_t)gq.ptr | (uintptr_t)gk.ptr | (uintptr_t)gv.ptr) % size || ((uintptr_t)d_state_out | (uintptr_t)d_state_in) % 4)
+        return derr(HUM_ERR_ARG, fn, "gradients must be aligned to their elements");
+    uint64_t need = 0;
+    if (const int rc = hum_decay_attn_workspace(p, 1, &need)) return rc;
+    if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
+        return derr(HUM_ERR_ARG, fn, "the workspace is too small (hum_decay_attn_workspace) or not aligned to 16 bytes");
+    const uint64_t state = 4ull * p->lanes * p->heads * p->dk * p->dv;
+    auto meets = [&](const float* a, const float* b) {
+        return a && b && (uintptr_t)a < (uintptr_t)b + state && (uintptr_t)b < (uintptr_t)a + state;
+    };
+    if (meets(d_state_in, d_state_out) || meets(d_state_in, p->state_in))
+        return derr(HUM_ERR_ARG, fn, "d_state_in must not overlap state_in or d_state_out");
+    if (!p->lanes) return HUM_OK;
+    const OnDevice dev(p->device);
+    if (!dev.ok) return derr(HUM_ERR_HIP, fn, "hipSetDevice");
+    const Rows q = rows_of(p->q, 1, size, p->dk), k = rows_of(p->k, group, size, p->dk);
+    const Rows v = rows_of(p->v, group, size, p->dv), g = rows_of(*d_out, 1, size, p->dv);
+    float* part_k = (float*)workspace;
+    float* part_v = part_k + (group > 1 ? (size_t)p->lanes * p->steps * p->heads * p->dk : 0);
+    const hum_rows pk = {part_k, (int64_t)p->steps * p->heads * p->dk, (int64_t)p->heads * p->dk, p->dk};
+    const hum_rows pv = {part_v, (int64_t)p->steps * p->heads * p->dv, (int64_t)p->heads * p->dv, p->dv};
+    Role r[3];
+    int n = 0;
+    if (gq.ptr) {
+        Role& w = r[n++] = Role{};
+        w.x = g; w.y = v; w.z = k;
+        w.out = rows_of(gq, 1, size, p->dk);
+        w.dy = p->dv; w.dz = p->dk;
+        w.s_pair = w.s_in = p->scale;
+        w.s_add = 1.f;
+        role_state(w, p->state_in, nullptr, p, false);
+    }
+    if (gk.ptr) {
+        Role& w = r[n++] = Role{};
+        w.x = v; w.y = g; w.z = q;
+        w.out = group > 1 ? rows_of(pk, 1, 4, p->dk) : rows_of(gk, 1, size, p->dk);
+        w.out_f32 = group > 1;
+        w.dy = p->dv; w.dz = p->dk;
+        w.rev = 1;
+        w.s_pair = w.s_add = p->scale;
+        w.s_in = 1.f;
+        role_state(w, d_state_out, nullptr, p, false);
+    }
+    if (gv.ptr || d_state_in) {
+        Role& w = r[n++] = Role{};
+        w.x = k; w.y = q; w.z = g;
+        w.out = gv.ptr ? (group > 1 ? rows_of(pv, 1, 4, p->dv) : rows_of(gv, 1, size, p->dv)) : Rows{};
+        w.out.shared = 1;
+        w.out_f32 = group > 1;
+        w.dy = p->dk; w.dz = p->dv;
+        w.rev = 1;
+        w.s_pair = w.s_add = p->scale;
+        w.s_in = 1.f;
+        role_state(w, d_state_out, d_state_in, p, true);
+    }
+    hipStream_t s = (hipStream_t)stream;
+    launch_roles(p, r, n, s);
+    if (group > 1 && p->steps) {
+        const long rows = (long)p->lanes * p->steps;
+        struct { const hum_rows* o; const float* part; int d; } sums[2] = {{&gk, part_k, p->dk}, {&gv, part_v, p->dv}};
+        for (auto& x : sums) {
+            if (!x.o->ptr) continue;
+            const Rows o = rows_of(*x.o, 1, size, x.d);
+            const long blocks = (rows * p->kv_heads * x.d + 255) / 256;
+            const dim3 grid((unsigned)(blocks < (1 << 16) ? blocks : (1 << 16)));
+            if (p->type == HUM_F32) hipLaunchKernelGGL(share_kernel<HUM_F32>, grid, dim3(256), 0, s, x.part, o, rows, p->steps, p->kv_heads, group, x.d);
+            else if (p->type == HUM_BF16) hipLaunchKernelGGL(share_kernel<HUM_BF16>, grid, dim3(256), 0, s, x.part, o, rows, p->steps, p->kv_heads, group, x.d);
+            else hipLaunchKernelGGL(share_kernel<HUM_F16>, grid, dim3(256), 0, s, x.part, o, rows, p->steps, p->kv_heads, group, x.d);
+        }
+    }
+    return launched(fn);
+}
+
+}  // extern "C"
+
+namespace {
+template <int ST>
+void launch_step(const StepArgs& a, int lpr, long grid, hipStream_t s) {
+    const dim3 g((unsigned)grid), b(256);
+    switch (lpr) {
+        case 1: hipLaunchKernelGGL((step_kernel<ST, 1>), g, b, 0, s, a); break;
+        case 2: hipLaunchKernelGGL((step_kernel<ST, 2>), g, b, 0, s, a); break;
+        case 4: hipLaunchKernelGGL((step_kernel<ST, 4>), g, b, 0, s, a); break;
+        case 8: hipLaunchKernelGGL((step_kernel<ST, 8>), g, b, 0, s, a); break;
+        case 16: hipLaunchKernelGGL((step_kernel<ST, 16>), g, b, 0, s, a); break;
+        default: hipLaunchKernelGGL((step_kernel<ST, 32>), g, b, 0, s, a); break;
+    }
+}
+}  // namespace
+
+extern "C" int hum_decay_attn_step(const hum_decay_attn_args* p, const uint8_t* active, const hum_rows* out, void* stream) {
+    const char* fn = "hum_decay_attn_step";
+    if (const int rc = check_args(fn, p)) return rc;
+    if (p->steps != 1 || p->lengths) return derr(HUM_ERR_ARG, fn, "steps must be 1 and lengths NULL (active says which lanes step)");
+    if (!out || (p->lanes && (!out->ptr || !p->state_out)) || ((uintptr_t)out->ptr) % elem_size(p->type))
+        return derr(HUM_ERR_ARG, fn, "out (aligned to its elements) and state_out are required");
+    if (!p->lanes) return HUM_OK;
+    const OnDevice dev(p->device);
+    if (!dev.ok) return derr(HUM_ERR_HIP, fn, "hipSetDevice");
+    const int size = elem_size(p->type), group = p->heads / p->kv_heads;
+    StepArgs a = {};
+    a.q = rows_of(p->q, 1, size, p->dk);
+    a.k = rows_of(p->k, group, size, p->dk);
+    a.v = rows_of(p->v, group, size, p->dv);
+    a.out = rows_of(*out, 1, size, p->dv);
+    a.log_decay = p->log_decay;
+    a.state_in = p->state_in;
+    a.state_out = p->state_out;
+    a.reset = p->reset;
+    a.reset_lane = p->reset_lane;
+    a.active = active;
+    a.heads = p->heads;
+    a.dk = p->dk;
+    a.dv = p->dv;
+    a.scale = p->scale;
+    a.units = (long)p->lanes * p->heads;
+    a.s_vec = p->dk % 4 == 0 && ((uintptr_t)p->state_in | (uintptr_t)p->state_out) % 16 == 0;
+    int lpr = 1;
+    while (4 * lpr < p->dk) lpr *= 2;
+    const int rows = 4 * 4 * (64 / lpr);
+    a.blocks = (p->dv + rows - 1) / rows;
+    const long grid = a.units * a.blocks;
+    if (p->type == HUM_BF16) launch_step<HUM_BF16>(a, lpr, grid, (hipStream_t)stream);
+    else if (p->type == HUM_F16) launch_step<HUM_F16>(a, lpr, grid, (hipStream_t)stream);
+    else launch_step<HUM_F32>(a, lpr, grid, (hipStream_t)stream);
+    return launched(fn);
+}

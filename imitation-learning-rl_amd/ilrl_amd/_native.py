@@ -13,11 +13,11 @@ LIB_PATH = os.environ.get("ILRL_AMD_LIB", DEFAULT_LIB_PATH)
 # signatures are unchanged - later ones only added entry points).  Without it every library, override or not,
 # must match HUM_ABI_VERSION and export every symbol.
 AB_MODE = os.environ.get("ILRL_AMD_AB") == "1"
-AB_COMPATIBLE_ABIS = (8, 9, 10, 11, 12, 13)   # ABI 10 added hum_policy_create_ex, hum_hier_rollout; 11 hum_pack_rows;
+AB_COMPATIBLE_ABIS = (8, 9, 10, 11, 12, 13, 14)   # ABI 10 added hum_policy_create_ex, hum_hier_rollout; 11 hum_pack_rows;
 # 12 hum_hier_rollout_fused; 13 hum_rollout_fused_ex, hum_hier_rollout_fused_ex (the policy mean traces); 14 the
-# heightfield ridge contacts (HUM_MAX_CONTACTS 95 -> 119) and the IPC fragment transport
+# heightfield ridge contacts (HUM_MAX_CONTACTS 95 -> 119) and the IPC fragment transport; 15 the policy memory's operators
 
-HUM_ABI_VERSION = 14   # include/humanoid_env.h
+HUM_ABI_VERSION = 15   # include/humanoid_env.h
 HUM_NSTATE, HUM_NOBS, HUM_NACT, HUM_NBOOK, HUM_NAUX = 47, 70, 17, 48, 17
 HUM_NOBS_HIGH, HUM_NACT_HIGH = 44, 2
 HUM_AGENT_HIGH, HUM_AGENT_LOW, HUM_AGENT_SEL_SKIP = 1, 2, 255
@@ -55,7 +55,8 @@ EXPORTS = ["hum_abi_version", "hum_last_error", "hum_default_config", "hum_creat
            "hum_step_k", "hum_hier_step_k", "hum_set_terrain_ex", "hum_policy_act_ex", "hum_policy_create_ex",
            "hum_hier_rollout", "hum_pack_rows", "hum_hier_rollout_fused", "hum_rollout_fused_ex",
            "hum_hier_rollout_fused_ex", "hum_ipc_export", "hum_ipc_open", "hum_ipc_close", "hum_dma_copy",
-           "hum_dma_wait"]
+           "hum_dma_wait", "hum_decay_attn_workspace", "hum_decay_attn", "hum_decay_attn_backward", "hum_decay_attn_step",
+           "hum_layer_norm", "hum_layer_norm_workspace", "hum_layer_norm_backward"]
 
 
 class HumConfig(ctypes.Structure):
@@ -96,6 +97,25 @@ class HumPackField(ctypes.Structure):   # hum_pack_field
     _fields_ = [("src", ctypes.c_void_p), ("dst", ctypes.c_void_p), ("src_step", ctypes.c_int64),
                 ("src_lane", ctypes.c_int64), ("dst_step", ctypes.c_int64), ("dst_lane", ctypes.c_int64),
                 ("row_bytes", ctypes.c_int32)]
+
+
+HUM_F32, HUM_BF16, HUM_F16 = 0, 1, 2
+
+
+class HumRows(ctypes.Structure):   # hum_rows
+    _fields_ = [("ptr", ctypes.c_void_p), ("lane", ctypes.c_int64), ("step", ctypes.c_int64), ("head", ctypes.c_int64)]
+
+
+class HumDecayAttnArgs(ctypes.Structure):   # hum_decay_attn_args
+    _fields_ = [(k, ctypes.c_int32) for k in ("device", "type", "lanes", "steps", "heads", "kv_heads", "dk", "dv")] + \
+               [("scale", ctypes.c_float), ("log_decay", ctypes.c_void_p), ("q", HumRows), ("k", HumRows), ("v", HumRows),
+                ("state_in", ctypes.c_void_p), ("state_out", ctypes.c_void_p), ("reset", ctypes.c_void_p),
+                ("reset_lane", ctypes.c_int64), ("reset_step", ctypes.c_int64), ("lengths", ctypes.c_void_p)]
+
+
+class HumNormArgs(ctypes.Structure):   # hum_norm_args
+    _fields_ = [(k, ctypes.c_int32) for k in ("device", "type", "param_type", "channels")] + \
+               [("rows", ctypes.c_int64), ("x_row", ctypes.c_int64), ("x", ctypes.c_void_p), ("weight", ctypes.c_void_p)]
 
 
 class NativeError(RuntimeError):
@@ -156,6 +176,15 @@ def lib():
     L.hum_ipc_close.argtypes = [vp]
     L.hum_dma_copy.argtypes = [vp, vp, u64, i32, ctypes.POINTER(HumDmaTicket)]
     L.hum_dma_wait.argtypes = [ctypes.POINTER(HumDmaTicket)]
+    rows, attn, norm = ctypes.POINTER(HumRows), ctypes.POINTER(HumDecayAttnArgs), ctypes.POINTER(HumNormArgs)
+    i64, f32 = ctypes.c_int64, ctypes.c_float
+    L.hum_decay_attn_workspace.argtypes = [attn, i32, ctypes.POINTER(u64)]
+    L.hum_decay_attn.argtypes = [attn, rows, vp, u64, vp]
+    L.hum_decay_attn_backward.argtypes = [attn, rows, vp, rows, rows, rows, vp, vp, u64, vp]
+    L.hum_decay_attn_step.argtypes = [attn, vp, rows, vp]
+    L.hum_layer_norm.argtypes = [norm, vp, f32, vp, i64, vp, vp, vp]
+    L.hum_layer_norm_workspace.argtypes = [norm, ctypes.POINTER(u64)]
+    L.hum_layer_norm_backward.argtypes = [norm, vp, i64, vp, vp, vp, i64, vp, vp, vp, u64, vp]
     L.hum_policy_act.argtypes = [vp, vp, vp, vp, i32, vp, vp, vp, i32, u64, vp]
     L.hum_policy_act_ex.argtypes = [vp, vp, vp, vp, i32, vp, vp, vp, vp, i32, u64, vp]
     L.hum_rollout.argtypes = [vp, vp, i32, i32, u64, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp]

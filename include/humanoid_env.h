@@ -35,7 +35,7 @@
 extern "C" {
 #endif
 
-#define HUM_ABI_VERSION 14
+#define HUM_ABI_VERSION 15
 #define HUM_NSTATE 47   /* physics state per lane */
 #define HUM_NOBS 70     /* observation_space shape, low_level_env.py:53-55 */
 #define HUM_NACT 17     /* action_space shape, low_level_env.py:56 */
@@ -448,6 +448,76 @@ int hum_hier_rollout_fused(hum_env* env, hum_policy* high, hum_policy* low, int3
 int hum_hier_rollout_fused_ex(hum_env* env, hum_policy* high, hum_policy* low, int32_t k, int32_t explore,
                               uint64_t step0, const hum_hier_io* io, const hum_hier_traj* traj, float* mean_high,
                               float* mean_low, void* stream);
+
+/* ---- The policy's memory (ABI 15): linear attention with a decay for each head and layer norm, the operators of a
+ * recurrent core between the observations and the policy network, so that a policy can act on what it saw earlier in the
+ * episode (the heightfield scene, for one, is not in the 70-dim observation).  The single-step form serves the sampler
+ * loop, the form over whole fragments and its gradient the learner (ilrl_amd/memory.py).
+ * These calls need no handle: `device` names the GPU that every pointer belongs to, `stream` one of its streams; the
+ * caller's current device is left as it was; scratch memory is the caller's, so calls on different streams and
+ * captured graphs with scratch of their own do not meet.  Errors: HUM_ERR_ARG / HUM_ERR_HIP. */
+#define HUM_F32 0
+#define HUM_BF16 1
+#define HUM_F16 2
+/* rows [lane, step, head, channel]: strides in elements, channels adjacent */
+typedef struct {
+    void* ptr;
+    int64_t lane, step, head;
+} hum_rows;
+/* Per lane and head, S [dv, dk] float32, steps t = 0 .. length - 1:
+ *     S_t = a_t S_{t-1} + v_t k_t^T,  o_t = scale S_t q_t,  a_t = 0 where reset[lane, t] != 0 (an episode starts at step
+ *     t: nothing before it is seen), else exp(log_decay[head]).
+ * q [lanes, steps, heads, dk], k [lanes, steps, kv_heads, dk], v [lanes, steps, kv_heads, dv] of element type `type`;
+ * query head h reads key / value head h / (heads / kv_heads).  Products of bf16 rows are summed in float32; the state is
+ * float32.  Steps behind a lane's length are not read; their outputs and gradients are zeros.  log_decay is a constant
+ * schedule (<= 0; -inf: no memory), not a trained parameter: it has no gradient. */
+typedef struct {
+    int32_t device, type;
+    int32_t lanes, steps, heads, kv_heads, dk, dv;   /* dk, dv in [1, 128]; lanes x heads <= 2^21 */
+    float scale;
+    const float* log_decay;      /* [heads] */
+    hum_rows q, k, v;
+    const float* state_in;       /* [lanes, heads, dv, dk], contiguous; NULL = zeros */
+    float* state_out;            /* the same, may be state_in; NULL = not wanted */
+    const uint8_t* reset;        /* element [lane, step] at lane * reset_lane + step * reset_step; NULL = none */
+    int64_t reset_lane, reset_step;
+    const int32_t* lengths;      /* [lanes], clamped to [0, steps]; NULL = all steps */
+} hum_decay_attn_args;
+/* bytes of scratch that hum_decay_attn (backward = 0) or hum_decay_attn_backward (1) needs for these sizes (0: none) */
+int hum_decay_attn_workspace(const hum_decay_attn_args* args, int32_t backward, uint64_t* bytes);
+/* out [lanes, steps, heads, dv] must not overlap an input. */
+int hum_decay_attn(const hum_decay_attn_args* args, const hum_rows* out, void* workspace, uint64_t workspace_bytes,
+                   void* stream);
+/* Gradients for d_out [lanes, steps, heads, dv] and d_state_out (gradient of state_out; NULL = zeros), from the forward
+ * call's inputs (args->state_out is not used): dq, dk, dv shaped like q, k, v (dk, dv summed over the heads that share
+ * one) and d_state_in; each may be NULL.  Outputs must not overlap inputs or each other. */
+int hum_decay_attn_backward(const hum_decay_attn_args* args, const hum_rows* d_out, const float* d_state_out,
+                            const hum_rows* dq, const hum_rows* dk, const hum_rows* dv, float* d_state_in,
+                            void* workspace, uint64_t workspace_bytes, void* stream);
+/* One step (args->steps = 1, lengths NULL) of every lane with active[lane] != 0 (NULL = all): the sampler's form.  An
+ * idle lane keeps its state and gives zeros.  state_out is required and may be state_in.  The step strides are unused. */
+int hum_decay_attn_step(const hum_decay_attn_args* args, const uint8_t* active, const hum_rows* out, void* stream);
+
+/* Layer norm over the channels of each row: y = (x - mean) rstd weight + bias, rstd = 1 / sqrt(var + eps), sums in
+ * float32.  x [rows, channels] of element type `type`, x_row elements from one row to the next, channels adjacent (the
+ * same holds for y, dy and dx with their own); weight, bias [channels] of param_type (HUM_F32 or `type`); NULL weight =
+ * ones, NULL bias = zeros.  y may be x. */
+typedef struct {
+    int32_t device, type, param_type, channels;   /* channels in [1, 16384] */
+    int64_t rows, x_row;
+    const void* x;
+    const void* weight;
+} hum_norm_args;
+/* mean, rstd [rows] (together or NULL): what the backward call needs of this one */
+int hum_layer_norm(const hum_norm_args* args, const void* bias, float eps, void* y, int64_t y_row, float* mean,
+                   float* rstd, void* stream);
+/* bytes of scratch hum_layer_norm_backward needs when d_weight or d_bias is wanted */
+int hum_layer_norm_workspace(const hum_norm_args* args, uint64_t* bytes);
+/* dx [rows, channels], d_weight and d_bias [channels] of param_type, each may be NULL; dx may be dy or x.  The
+ * parameter gradients are summed in a fixed order: the same inputs give the same bits. */
+int hum_layer_norm_backward(const hum_norm_args* args, const void* dy, int64_t dy_row, const float* mean,
+                            const float* rstd, void* dx, int64_t dx_row, void* d_weight, void* d_bias, void* workspace,
+                            uint64_t workspace_bytes, void* stream);
 
 /* RewardLogCallback terms (custom_callback.py:43-80) per lane: device float32 [n, HUM_NAUX]. */
 int hum_get_aux(hum_env* env, float* aux_out, void* stream);
