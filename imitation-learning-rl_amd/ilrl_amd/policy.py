@@ -112,7 +112,8 @@ class DevicePolicy:
              "w3": _normc(rng, (H, 1), 0.01), "b3": np.zeros(1)}
         return cls(w, device=device, seed=seed, n_in=n_in, n_out=1)
 
-    def sample_batch_columns(self, obs, actions, value=None, out=None, mean=None, valid=None):
+    def sample_batch_columns(self, obs, actions, value=None, out=None, mean=None, valid=None, memory=None, state=None,
+                             resets=None):
         """The policy-side SampleBatch columns RLlib's sampler records per step, for recorded policy inputs obs
         [..., n_in] and raw samples actions [..., n_out] (device; e.g. a rollout's trajectory, any leading shape):
         action_dist_inputs [..., 2 n_out] (the DiagGaussian's mean and log_std), action_logp [...] (log-density of
@@ -124,8 +125,20 @@ class DevicePolicy:
         valid: a bool mask of the leading shape marking the rows that hold a real transition.  A fused hierarchical
         rollout (hier_rollout(fused=True)) leaves the non-acting agent's obs / act / mean rows unwritten, so their
         columns would be computed from stale or uninitialised memory: pass valid = (acted & HUM_AGENT_x) != 0 there;
-        the invalid rows' columns are written as zeros."""
+        the invalid rows' columns are written as zeros.
+        memory: the PolicyMemory a rollout(memory=) acted through; obs [k,n,n_in], `resets` [k,n] and `state` (the lanes'
+        memory before the first row; None = empty) are that rollout's, and both networks read the features it gives the
+        fragment (one pass over all k steps instead of k single ones: equal up to fp32 rounding)."""
         t = self.torch
+        if memory is not None:
+            if obs.dim() != 3 or resets is None:
+                raise ValueError("sample_batch_columns: memory needs obs [k, n, n_in] and the rollout's resets [k, n]")
+            if mean is not None or valid is not None:
+                raise ValueError("sample_batch_columns: memory goes with neither mean nor valid")
+            with t.no_grad():
+                obs, _ = memory.forward(obs, state=state, reset=resets)
+        elif state is not None or resets is not None:
+            raise ValueError("sample_batch_columns: state and resets need memory")
         lead = tuple(obs.shape[:-1])
         R = int(np.prod(lead)) if lead else 1
         o2 = obs.reshape(R, self.n_in)
@@ -197,7 +210,8 @@ class DevicePolicy:
                 "hum_policy_act")
         return act
 
-    def rollout(self, venv, k, explore=True, step0=0, trajectories=True, fused=False, out=None, means=False):
+    def rollout(self, venv, k, explore=True, step0=0, trajectories=True, fused=False, out=None, means=False, memory=None,
+                state=None):
         """k sampler steps (policy -> env step with auto-reset) on venv's lanes, all on the device with no host
         round trip.  venv.obs must hold the current observation (after venv.reset()).  Returns the trajectory
         tensors {obs [k,n,70] (policy inputs), actions [k,n,17] (the samples before clip_actions, as RLlib records
@@ -205,9 +219,18 @@ class DevicePolicy:
         (hum_rollout_fused; cooperative fp32 handles with 4 envs per block on the plane).  out: a dict of the same
         tensors to write into (reused across calls, e.g. by a timed loop) instead of fresh ones.  means (fused only):
         also means [k,n,17], the policy's mean per step as the in-kernel network forms it (hum_rollout_fused_ex), for
-        sample_batch_columns(..., mean=...)."""
+        sample_batch_columns(..., mean=...).
+        memory: a PolicyMemory (ilrl_amd/memory.py) between the observations and the network; per step it advances the
+        lanes' memory `state` (memory.begin(n), moved on in place from call to call) and the network reads its features.
+        An episode that ended at the previous step is forgotten.  The trajectory then also holds resets [k,n] (the rows
+        at which an episode started), what sample_batch_columns(..., memory=) and memory.forward need with a copy of
+        `state` from before the call.  Not with fused."""
         t = self.torch
         n = venv.n
+        if memory is not None:
+            return self._rollout_memory(venv, k, explore, step0, trajectories, fused or means, out, memory, state)
+        if state is not None:
+            raise ValueError("rollout: state needs memory")
         if means and not (fused and trajectories):
             raise ValueError("rollout: means=True needs fused=True and trajectories=True")
         if not hasattr(venv, "_act_buf"):
@@ -235,6 +258,42 @@ class DevicePolicy:
         else:
             fn = N.lib().hum_rollout_fused if fused else N.lib().hum_rollout
             N.check(fn(*args, venv._stream()), "hum_rollout_fused" if fused else "hum_rollout")
+        return tr
+
+
+    def _rollout_memory(self, venv, k, explore, step0, trajectories, fused, out, memory, state):
+        t, n = self.torch, venv.n
+        if fused:
+            raise ValueError("rollout: memory goes with neither fused nor means")
+        if memory.n_in != self.n_in or memory.device != self.device or venv.device != self.device:
+            raise ValueError("rollout: the memory must have the policy's input width and all three one device")
+        if state is None:
+            raise ValueError("rollout: memory needs its lanes' state (memory.begin(venv.n))")
+        tr = {}
+        if trajectories:
+            shapes = {"obs": ((N.HUM_NOBS,), t.float32), "actions": ((N.HUM_NACT,), t.float32), "rewards": ((), t.float32),
+                      "dones": ((), t.uint8), "resets": ((), t.uint8)}
+            for f, (sh, dt) in shapes.items():
+                x = out.get(f) if out else None
+                if x is None:
+                    x = t.empty((k, n) + sh, dtype=dt, device=venv.device)
+                elif tuple(x.shape) != (k, n) + sh or x.dtype != dt or x.device != venv.device or not x.is_contiguous():
+                    raise ValueError("rollout: out[%r] must be a contiguous %s tensor of shape %s on %s"
+                                     % (f, dt, (k, n) + sh, venv.device))
+                tr[f] = x
+        act = t.empty(n, N.HUM_NACT, dtype=t.float32, device=venv.device)
+        for i in range(k):
+            # lanes that finished an episode in the previous step act on their reset observation, with nothing remembered
+            obs = t.where(venv.done.bool()[:, None], venv.obs_reset, venv.obs)
+            feat = memory.step(obs, state, reset=venv.done)
+            if tr:
+                tr["obs"][i].copy_(obs)
+                tr["resets"][i].copy_(venv.done)
+            self.act(feat, explore=explore, step=step0 + i, out=act, raw_out=tr["actions"][i] if tr else None)
+            venv.step(act, autoreset=True)
+            if tr:
+                tr["rewards"][i].copy_(venv.reward)
+                tr["dones"][i].copy_(venv.done)
         return tr
 
 
