@@ -34,14 +34,14 @@ def _attn(**kw):
     rows = N.HumRows(0x1000, 64, 64, 8)
     d = dict(device=0, type=N.HUM_F32, lanes=2, steps=3, heads=4, kv_heads=2, dk=8, dv=8, scale=1.0, log_decay=0x1000, q=rows,
              k=rows, v=rows)
-    d.update(kw)
+    d.update({k: N.HumRows(*v) if isinstance(v, tuple) else v for k, v in kw.items()})
     return N.HumDecayAttnArgs(**d)
 
 
 BAD = [(dict(type=3), b"element type"), (dict(lanes=-1), b">= 0"), (dict(steps=-1), b">= 0"), (dict(heads=0), b"divide"),
        (dict(kv_heads=3), b"divide"), (dict(dk=0), b"\\[1, 128\\]"), (dict(dv=129), b"\\[1, 128\\]"),
        (dict(lanes=1 << 20, heads=4), b"2\\^21"), (dict(scale=float("nan")), b"finite"), (dict(log_decay=None), b"log_decay"),
-       (dict(q=N.HumRows(None, 0, 0, 0)), b"required"), (dict(k=N.HumRows(0x1002, 0, 0, 0)), b"aligned"),
+       (dict(q=(None, 0, 0, 0)), b"required"), (dict(k=(0x1002, 0, 0, 0)), b"aligned"),
        (dict(state_in=0x1002), b"aligned"), (dict(lengths=0x1001), b"aligned")]
 
 
