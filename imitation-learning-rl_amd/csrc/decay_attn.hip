@@ -67,8 +67,10 @@ struct Role {
     float s_pair, s_in, s_add;   // the scale's place: on the pairs, on what the entering state gives, on what joins it
     const float* state_in;  // element (y channel i, z channel j) at i sy + j sz; NULL = zeros
     float* state_out;       // NULL = not wanted
-    long sy, sz, s_lane;    // s_lane: from one (lane, head) to the next
-    int s_vec;              // sy == 1 and 16-byte aligned rows
+    float* through;         // [(lane, head), segment]: what the segment leaves of an entering state; NULL = not wanted
+    long sy, sz;            // one of them is 1
+    long in_unit, in_seg, out_unit, out_seg;   // from one (lane, head) / segment to the next
+    int s_vec;              // 16-byte aligned rows of the unit stride
     int slice0;             // first workgroup part of this role
 };
 
@@ -76,6 +78,8 @@ struct WalkArgs {
     Role r[3];
     int nroles, parts;
     int lanes, steps, heads;
+    int segs, seg_steps;    // the walk of a (lane, head) is cut into segs pieces of seg_steps (a multiple of 32) steps
+    int last_only;          // state_out is the last segment's
     const float* log_decay;
     const unsigned char* reset;
     long reset_lane, reset_step;
@@ -219,23 +223,54 @@ __device__ __forceinline__ void lds_order() {
     __builtin_amdgcn_wave_barrier();
 }
 
+// 4 x 4 transposes inside quads of lanes: v[q] of quad lane i <-> v[i] of quad lane q
+__device__ __forceinline__ f32x4 quad_transpose(f32x4 v) {
+    const int l = threadIdx.x;
+    auto from = [](float x, auto ctrl) {
+        return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), decltype(ctrl)::value, 0xf, 0xf, false));
+    };
+    struct X1 { enum { value = 0xB1 }; };   // quad lane ^ 1
+    struct X2 { enum { value = 0x4E }; };   // quad lane ^ 2
+    const bool odd = l & 1, upper = l & 2;
+#pragma unroll
+    for (int p = 0; p < 4; p += 2) {
+        const float got = from(odd ? v[p] : v[p + 1], X1{});
+        if (odd) v[p] = got; else v[p + 1] = got;
+    }
+#pragma unroll
+    for (int p = 0; p < 2; p++) {
+        const float got = from(upper ? v[p] : v[p + 2], X2{});
+        if (upper) v[p] = got; else v[p + 2] = got;
+    }
+    return v;
+}
+
+// waves per SIMD that the registers are limited for: two hide each other's loads, where the state and operands fit into
+// 256 registers
+constexpr int walk_waves(int st, int dy, int dz) { return dy * dz * (st == HUM_BF16 ? 1 : 2) <= 4096 ? 2 : 1; }
+
 // One wave per workgroup.  DY, DZ: channels of y and of the z slice rounded up to 32.
 template <int ST, int DY, int DZ>
-__global__ void __launch_bounds__(64) walk_kernel(WalkArgs a) {
+__global__ void __launch_bounds__(64, walk_waves(ST, DY, DZ)) walk_kernel(WalkArgs a) {
     typedef Num<ST> M;
     typedef typename M::Op Op;
     constexpr int KY = DY / 32, KZ = DZ / 32;
     constexpr int PO = M::PARTS > 1 ? 2 : 1;   // parts of P and of the state's reading
     constexpr int PS = M::PARTS;               // parts of what joins the state
     constexpr int PY = DY + M::PAD, PZ = DZ + M::PAD;
+    constexpr bool WEIGH_Y = KY <= KZ;         // the side with fewer tiles carries the weights into the state
     __shared__ __attribute__((aligned(16))) typename M::Elem ly[CH * PY];
     __shared__ __attribute__((aligned(16))) typename M::Elem lz[CH * PZ];
+    // lambda^d times the scale's part for d = -31 .. 32 steps, zeros for d < 0: between two steps of a chunk, and from a
+    // step to the chunk's end
+    __shared__ float pow_pair[2 * CH], pow_add[2 * CH];
 
     const int l = threadIdx.x, g = l >> 4, r = l & 15;
-    // the parts (roles, slices) of one (lane, head) read the same rows: they go to one XCD, one after the other
+    // the parts (roles, slices) of one segment read the same rows: they go to one XCD, one after the other
     const int block = blockIdx.x, part = block / XCDS % a.parts;
-    const int unit = block / (XCDS * a.parts) * XCDS + block % XCDS;
-    if (unit >= a.lanes * a.heads) return;
+    const int item = block / (XCDS * a.parts) * XCDS + block % XCDS;
+    if (item >= a.lanes * a.heads * a.segs) return;
+    const int unit = item / a.segs, seg = item - unit * a.segs;
     const int ri = (a.nroles > 1 && part >= a.r[1].slice0) + (a.nroles > 2 && part >= a.r[2].slice0);
     const Role& R = a.r[ri];
     const int dz0 = (part - R.slice0) * DZ;
@@ -249,89 +284,112 @@ __global__ void __launch_bounds__(64) walk_kernel(WalkArgs a) {
     const int rev = R.rev;
     const float lg = a.log_decay[h] * 1.44269504088896340736f;
     auto power = [&](int n) { return n == 0 ? 1.f : __builtin_amdgcn_exp2f(lg * (float)n); };
+    pow_pair[l] = l < CH - 1 ? 0.f : R.s_pair * power(l - (CH - 1));
+    pow_add[l] = l < CH - 1 ? 0.f : R.s_add * power(l - (CH - 1));
+    const int seg0 = seg * a.seg_steps, seg1 = seg + 1 < a.segs ? seg0 + a.seg_steps : steps;
+    const int end = len < seg1 ? len : seg1;
+    auto row_of = [&](int tile) { return 8 * (r >> 2) + 4 * tile + (r & 3); };
+
+    // ---- rows of a chunk: x by walk step 16 c + r, y and z by step row_of(t)
+    // (64-bit positions of the lane's first rows; its other rows and the next chunk's are uniform distances away)
+    const long dir = rev ? -1 : 1, first = rev ? len - 1 - seg0 : seg0;
+    auto start = [&](const Rows& m, int row) {
+        return (long)b * m.lane + (long)(h / m.shared) * m.head + (first + dir * row) * m.step;
+    };
+    long px = start(R.x, r), py = start(R.y, row_of(0)), pz = start(R.z, row_of(0)), po = start(R.out, r);
+    const long sx = dir * R.x.step, sy = dir * R.y.step, sz = dir * R.z.step, so = dir * R.out.step;
+    const unsigned char* marks = a.reset ? a.reset + (long)b * a.reset_lane : nullptr;
+    auto time = [&](int n) { return rev ? len - 1 - n : n; };   // of walk step n
+    Op X[2][KY], Y[2][KY], Z[2][KZ];
+    bool mark = false;
+    auto load_x = [&](int n0) {
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+            const int n = n0 + 16 * c + r;
+            const long at = px + 16 * c * sx;
+#pragma unroll
+            for (int k = 0; k < KY; k++) {
+                const int d = 32 * k + 8 * g;
+                X[c][k] = n < end && d < R.dy ? M::load(R.x.p, at + d, R.dy - d, R.x.vec) : M::zero();
+            }
+        }
+        px += CH * sx;
+    };
+    auto load_yz = [&](int n0) {
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            const int n = n0 + row_of(t);
+            const long aty = py + 4 * t * sy, atz = pz + 4 * t * sz;
+#pragma unroll
+            for (int k = 0; k < KY; k++) {
+                const int d = 32 * k + 8 * g;
+                Y[t][k] = n < end && d < R.dy ? M::load(R.y.p, aty + d, R.dy - d, R.y.vec) : M::zero();
+            }
+#pragma unroll
+            for (int k = 0; k < KZ; k++) {
+                const int d = dz0 + 32 * k + 8 * g;
+                Z[t][k] = n < end && d < R.dz ? M::load(R.z.p, atz + d, R.dz - d, R.z.vec) : M::zero();
+            }
+        }
+        py += CH * sy;
+        pz += CH * sz;
+        // bit j separates the chunk's walk steps j - 1 and j (bit 0 the entering state, bit L the leaving one).  An
+        // episode's first step is cut off from what time puts before it, so the backward walk has it one later.
+        if (marks) {
+            const int n = n0 + l - rev;
+            mark = l <= CH && l >= rev && l - rev < CH && n < end && marks[(long)time(n) * a.reset_step] != 0;
+        }
+    };
+    if (seg0 < end) {
+        if (R.out.p) load_x(seg0);
+        load_yz(seg0);
+    }
 
     // ---- the entering state: tile (i, j) holds y channels 32 (i / 2) + 8 g + 4 (i & 1) + 0..3 of z channel zc(j)
     f32x4 S[2 * KY][2 * KZ];
     auto zc = [&](int j) { return dz0 + 32 * (j >> 1) + 8 * (r >> 2) + 4 * (j & 1) + (r & 3); };
+    // rows of unit stride are read 16 bytes at a time: along y directly, along z by one row a quad lane and a transpose
+    const bool along_y = R.sy == 1;
     {
-        const float* s = R.state_in ? R.state_in + (long)unit * R.s_lane : nullptr;
+        const float* s = R.state_in ? R.state_in + (long)unit * R.in_unit + (long)seg * R.in_seg : nullptr;
 #pragma unroll
         for (int j = 0; j < 2 * KZ; j++)
 #pragma unroll
             for (int i = 0; i < 2 * KY; i++) {
                 const int y0 = 32 * (i >> 1) + 8 * g + 4 * (i & 1), z = zc(j);
                 f32x4 v = {0.f, 0.f, 0.f, 0.f};
-                if (s && z < R.dz) {
-                    if (R.s_vec) {
-                        if (y0 < R.dy) v = *(const f32x4*)(s + (long)z * R.sz + y0);
-                    } else {
+                if (s) {
+                    if (!R.s_vec) {
 #pragma unroll
                         for (int q = 0; q < 4; q++)
-                            if (y0 + q < R.dy) v[q] = s[(long)z * R.sz + (long)(y0 + q) * R.sy];
+                            if (z < R.dz && y0 + q < R.dy) v[q] = s[(long)z * R.sz + (long)(y0 + q) * R.sy];
+                    } else if (along_y) {
+                        if (z < R.dz && y0 < R.dy) v = *(const f32x4*)(s + (long)z * R.sz + y0);
+                    } else {
+                        const int y = y0 + (r & 3), z4 = z - (r & 3);
+                        if (z4 < R.dz && y < R.dy) v = *(const f32x4*)(s + (long)y * R.sy + z4);
                     }
                 }
                 S[i][j] = v;
             }
+        if (s && R.s_vec && !along_y)
+#pragma unroll
+            for (int j = 0; j < 2 * KZ; j++)
+#pragma unroll
+                for (int i = 0; i < 2 * KY; i++) S[i][j] = quad_transpose(S[i][j]);
     }
 
-    // ---- what a chunk's weights depend on besides its marks
-    float w_pair[2][8];   // step t = 16 c + r of the walk, step s = 8 g + j: lambda^(t - s) for s <= t
-#pragma unroll
-    for (int c = 0; c < 2; c++)
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const int d = 16 * c + r - (8 * g + j);
-            w_pair[c][j] = d < 0 ? 0.f : R.s_pair * power(d);
-        }
     float w_in[2];
 #pragma unroll
     for (int c = 0; c < 2; c++) w_in[c] = R.s_in * power(16 * c + r + 1 - rev);
+    float passed = 1.f;   // what is left of the entering state
 
-    const long xo = (long)b * R.x.lane + (long)(h / R.x.shared) * R.x.head;
-    const long yo = (long)b * R.y.lane + (long)(h / R.y.shared) * R.y.head;
-    const long zo = (long)b * R.z.lane + (long)(h / R.z.shared) * R.z.head;
-    const long oo = (long)b * R.out.lane + (long)(h / R.out.shared) * R.out.head;
-    const unsigned char* marks = a.reset ? a.reset + (long)b * a.reset_lane : nullptr;
-    auto row_of = [&](int tile) { return 8 * (r >> 2) + 4 * tile + (r & 3); };
-
-    for (int n0 = 0; n0 < len; n0 += CH) {
-        const int L = len - n0 < CH ? len - n0 : CH;
-        auto time = [&](int n) { return rev ? len - 1 - (n0 + n) : n0 + n; };
-        // ---- rows: x by walk step 16 c + r, y and z by step row_of(a)
-        Op X[2][KY], Y[2][KY], Z[2][KZ];
-#pragma unroll
-        for (int c = 0; c < 2; c++) {
-            const int n = 16 * c + r;
-            const long at = xo + (long)time(n) * R.x.step;
-#pragma unroll
-            for (int k = 0; k < KY; k++) {
-                const int d = 32 * k + 8 * g;
-                X[c][k] = n < L && d < R.dy ? M::load(R.x.p, at + d, R.dy - d, R.x.vec) : M::zero();
-            }
-        }
-#pragma unroll
-        for (int t = 0; t < 2; t++) {
-            const int n = row_of(t);
-            const long aty = yo + (long)time(n) * R.y.step, atz = zo + (long)time(n) * R.z.step;
-#pragma unroll
-            for (int k = 0; k < KY; k++) {
-                const int d = 32 * k + 8 * g;
-                Y[t][k] = n < L && d < R.dy ? M::load(R.y.p, aty + d, R.dy - d, R.y.vec) : M::zero();
-            }
-#pragma unroll
-            for (int k = 0; k < KZ; k++) {
-                const int d = dz0 + 32 * k + 8 * g;
-                Z[t][k] = n < L && d < R.dz ? M::load(R.z.p, atz + d, R.dz - d, R.z.vec) : M::zero();
-            }
-        }
-        // ---- marks: bit j separates walk steps j - 1 and j (bit 0 the entering state, bit L the leaving one).  An
-        // episode's first step is cut off from what time puts before it, so the backward walk has it one later.
-        unsigned long long cut = 0;
-        if (marks) {
-            const int n = l - rev;
-            const bool m = n >= 0 && n < L && marks[(long)time(n) * a.reset_step] != 0;
-            cut = __ballot(m);
-        }
+    for (int n0 = seg0; n0 < end; n0 += CH) {
+        const int L = end - n0 < CH ? end - n0 : CH;
+        const bool more = n0 + CH < end;
+        // a mark beyond the chunk's last step (its bit L when walking backwards) is this chunk's as well as the first
+        // of the next
+        const unsigned long long cut = marks ? __ballot(mark) & ((2ull << (L - 1 + rev)) - 1) : 0;
         bool sane = true;
 #pragma unroll
         for (int t = 0; t < 2; t++)
@@ -339,64 +397,67 @@ __global__ void __launch_bounds__(64) walk_kernel(WalkArgs a) {
             for (int k = 0; k < KZ; k++) sane = sane && M::finite(Z[t][k]);
         const bool slow = __any(!sane);
 
-        auto upto = [&](int j) { return __builtin_popcountll(cut & ((2ull << j) - 1)); };   // cuts at or before step j
-        float wi[2], wo[8];
-        int ct[2], cs[8];
+        float wi[2];
+        int ct[2] = {0, 0}, cs[8] = {0, 0, 0, 0, 0, 0, 0, 0};   // cuts at or before a step
         const int cl = __builtin_popcountll(cut);
+        if (cut) {
+            auto upto = [&](int j) { return __builtin_popcountll(cut & ((2ull << j) - 1)); };
 #pragma unroll
-        for (int c = 0; c < 2; c++) {
-            ct[c] = upto(16 * c + r);
-            wi[c] = ct[c] == 0 ? w_in[c] : 0.f;
+            for (int c = 0; c < 2; c++) ct[c] = upto(16 * c + r);
+#pragma unroll
+            for (int j = 0; j < 8; j++) cs[j] = upto(8 * g + j);
         }
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const int s = 8 * g + j;
-            cs[j] = upto(s);
-            wo[j] = s < L && cs[j] == cl ? R.s_add * power(L - 1 - s + rev) : 0.f;
+        for (int c = 0; c < 2; c++) wi[c] = ct[c] == 0 ? w_in[c] : 0.f;
+
+        lds_order();
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+#pragma unroll
+            for (int k = 0; k < KY; k++) M::put(ly + row_of(t) * PY + 32 * k + 8 * g, Y[t][k]);
+#pragma unroll
+            for (int k = 0; k < KZ; k++) M::put(lz + row_of(t) * PZ + 32 * k + 8 * g, Z[t][k]);
         }
+        lds_order();
 
         // ---- P^T: rows s, columns t; masked entries are chosen away, not multiplied
         Op P[2][PO];
+        if (R.out.p) {
 #pragma unroll
-        for (int c = 0; c < 2; c++) {
-            f32x4 p[2];
+            for (int c = 0; c < 2; c++) {
+                f32x4 p[2];
 #pragma unroll
-            for (int t = 0; t < 2; t++) {
-                p[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+                for (int t = 0; t < 2; t++) {
+                    p[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int k = 0; k < KY; k++) M::mma(p[t], Y[t][k], X[c][k]);
+                    for (int k = 0; k < KY; k++) M::mma(p[t], Y[t][k], X[c][k]);
+                }
+                f32x8 v = pair(p[0], p[1]);
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const float w = pow_pair[CH - 1 + 16 * c + r - 8 * g - j];
+                    v[j] = w != 0.f && cs[j] == ct[c] ? v[j] * w : 0.f;
+                }
+                M::template split<PO>(v, P[c]);
             }
-            f32x8 v = pair(p[0], p[1]);
-#pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = w_pair[c][j] != 0.f && cs[j] == ct[c] ? v[j] * w_pair[c][j] : 0.f;
-            M::template split<PO>(v, P[c]);
         }
-
-#pragma unroll
-        for (int t = 0; t < 2; t++)
-#pragma unroll
-            for (int k = 0; k < KY; k++) M::put(ly + row_of(t) * PY + 32 * k + 8 * g, Y[t][k]);
+        __builtin_amdgcn_sched_barrier(0);
+        if (more) load_yz(n0 + CH);   // y and z are in LDS: their registers take the next chunk's rows
 
         // ---- one pass over the chunk's steps, or one per step where a z row is not finite
         for (int lo = 0; lo < L;) {
-            int hi = L, from = 0;
-            if (slow) {
-                hi = lo + 1;
-                const unsigned long long seen = cut & ((2ull << lo) - 1) & ~1ull;   // the last cut at or before lo
-                from = seen ? 63 - __builtin_clzll(seen) : 0;
-            }
-            lds_order();
-#pragma unroll
-            for (int t = 0; t < 2; t++) {
-                const int n = row_of(t);
-#pragma unroll
-                for (int k = 0; k < KZ; k++)
-                    M::put(lz + n * PZ + 32 * k + 8 * g, n >= from && n < hi ? Z[t][k] : M::zero());
-            }
-            lds_order();
+            const int hi = slow ? lo + 1 : L;
             Op T[2 * KZ];   // Z^T
 #pragma unroll
             for (int j = 0; j < 2 * KZ; j++) T[j] = M::column(lz, PZ, 8 * g, 32 * (j >> 1) + 4 * (j & 1), r);
+            if (slow) {     // of which step lo sees its episode's, up to itself
+                const unsigned long long seen = cut & ((2ull << lo) - 1) & ~1ull;
+                const int from = seen ? 63 - __builtin_clzll(seen) : 0;
+#pragma unroll
+                for (int j = 0; j < 2 * KZ; j++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) T[j][e] = 8 * g + e >= from && 8 * g + e < hi ? T[j][e] : (typename M::Elem)0.f;
+            }
             // ---- O^T: rows z channels, columns t
             if (R.out.p) {
 #pragma unroll
@@ -429,71 +490,134 @@ __global__ void __launch_bounds__(64) walk_kernel(WalkArgs a) {
                     for (int c = 0; c < 2; c++) {
                         const int n = 16 * c + r;
                         if (n >= lo && n < hi && d < R.dz) {
-                            const long at = oo + (long)time(n) * R.out.step + d;
+                            const long at = po + 16 * c * so + d;
                             if (R.out_f32) Num<HUM_F32>::store(R.out.p, at, R.dz - d, R.out.vec, pair(o[c][0], o[c][1]));
                             else M::store(R.out.p, at, R.dz - d, R.out.vec, pair(o[c][0], o[c][1]));
                         }
                     }
                 }
+                if (hi == L && more) load_x(n0 + CH);
             }
+            __builtin_amdgcn_sched_barrier(0);
             // ---- the state behind the chunk
-            if (hi == L && (cut >> L & 1)) {   // an episode starts right behind (before, in time): nothing is left
+            if (hi == L && (more || R.state_out)) {
+                const float through = cl == 0 ? power(L) : 0.f;
+                passed *= through;
+                if (cl == 0) {
 #pragma unroll
-                for (int i = 0; i < 2 * KY; i++)
+                    for (int i = 0; i < 2 * KY; i++)
 #pragma unroll
-                    for (int j = 0; j < 2 * KZ; j++) S[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-            } else if (hi == L) {
-                const float through = power(L);
+                        for (int j = 0; j < 2 * KZ; j++) S[i][j] *= through;
+                } else {
 #pragma unroll
-                for (int i = 0; i < 2 * KY; i++)
+                    for (int i = 0; i < 2 * KY; i++)
 #pragma unroll
-                    for (int j = 0; j < 2 * KZ; j++)
+                        for (int j = 0; j < 2 * KZ; j++) S[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+                }
+                float wo[8];   // (rows behind the chunk's last step are zeros)
 #pragma unroll
-                        for (int q = 0; q < 4; q++) S[i][j][q] = cl == 0 ? S[i][j][q] * through : 0.f;
-#pragma unroll
-                for (int i = 0; i < 2 * KY; i++) {
-                    f32x8 v = M::wide(M::column(ly, PY, 8 * g, 32 * (i >> 1) + 4 * (i & 1), r));
+                for (int j = 0; j < 8; j++) {
+                    const float w = pow_add[CH - 1 + L - 1 + rev - 8 * g - j];
+                    wo[j] = cs[j] == cl ? w : 0.f;
+                }
+                // nothing joins it where an episode starts right behind (before, in time)
+                auto weigh = [&](Op x) {
+                    f32x8 v = M::wide(x);
 #pragma unroll
                     for (int j = 0; j < 8; j++) v[j] = wo[j] != 0.f ? v[j] * wo[j] : 0.f;
-                    Op yp[PS];
-                    M::template split<PS>(v, yp);
+                    return v;
+                };
+                if (!(cut >> L & 1)) {
+                    if constexpr (WEIGH_Y) {
 #pragma unroll
-                    for (int u = 0; u < PS; u++)
+                        for (int i = 0; i < 2 * KY; i++) {
+                            __builtin_amdgcn_sched_barrier(0);
+                            Op yp[PS];
+                            M::template split<PS>(weigh(M::column(ly, PY, 8 * g, 32 * (i >> 1) + 4 * (i & 1), r)), yp);
 #pragma unroll
-                        for (int j = 0; j < 2 * KZ; j++) M::mma(S[i][j], yp[u], T[j]);
+                            for (int u = 0; u < PS; u++)
+#pragma unroll
+                                for (int j = 0; j < 2 * KZ; j++) M::mma(S[i][j], yp[u], T[j]);
+                        }
+                    } else {
+                        Op yt[2 * KY];
+#pragma unroll
+                        for (int i = 0; i < 2 * KY; i++) yt[i] = M::column(ly, PY, 8 * g, 32 * (i >> 1) + 4 * (i & 1), r);
+#pragma unroll
+                        for (int j = 0; j < 2 * KZ; j++) {
+                            __builtin_amdgcn_sched_barrier(0);
+                            Op zp[PS];
+                            M::template split<PS>(weigh(T[j]), zp);
+#pragma unroll
+                            for (int u = 0; u < PS; u++)
+#pragma unroll
+                                for (int i = 0; i < 2 * KY; i++) M::mma(S[i][j], yt[i], zp[u]);
+                        }
+                    }
                 }
             }
             lo = hi;
         }
-        lds_order();
+        po += CH * so;
     }
 
     // ---- the steps behind the lane's length
     if (R.out.p)
-        for (int n = len + r; n < steps; n += 16)
+        for (int n = (len > seg0 ? len : seg0) + r; n < seg1; n += 16)
 #pragma unroll
             for (int k = 0; k < KZ; k++) {
                 const int d = dz0 + 32 * k + 8 * g;
                 if (d < R.dz) {
-                    const long at = oo + (long)n * R.out.step + d;
+                    const long at = (long)b * R.out.lane + (long)(h / R.out.shared) * R.out.head + (long)n * R.out.step + d;
                     if (R.out_f32) Num<HUM_F32>::store(R.out.p, at, R.dz - d, R.out.vec, f32x8{});
                     else M::store(R.out.p, at, R.dz - d, R.out.vec, f32x8{});
                 }
             }
-    if (R.state_out) {
-        float* s = R.state_out + (long)unit * R.s_lane;
+    if (R.through && l == 0 && dz0 == 0) R.through[item] = passed;
+    if (R.state_out && (!a.last_only || seg + 1 == a.segs)) {
+        float* s = R.state_out + (long)unit * R.out_unit + (long)seg * R.out_seg;
 #pragma unroll
         for (int j = 0; j < 2 * KZ; j++)
 #pragma unroll
             for (int i = 0; i < 2 * KY; i++) {
                 const int y0 = 32 * (i >> 1) + 8 * g + 4 * (i & 1), z = zc(j);
                 if (z >= R.dz) continue;
-                if (R.s_vec) {
+                if (R.s_vec && along_y) {
                     if (y0 < R.dy) *(f32x4*)(s + (long)z * R.sz + y0) = S[i][j];
                 } else {
 #pragma unroll
                     for (int q = 0; q < 4; q++)
                         if (y0 + q < R.dy) s[(long)z * R.sz + (long)(y0 + q) * R.sy] = S[i][j][q];
+                }
+            }
+    }
+}
+
+// the segments' entering states from what each of them adds: seg[g] <- state before segment g, one thread per N elements
+template <int N>
+__global__ void __launch_bounds__(256) scan_kernel(const float* in, float* seg, const float* through, int segs, long units, int size) {
+    typedef float V __attribute__((ext_vector_type(N)));
+    const long e = ((long)blockIdx.x * 256 + threadIdx.x) * N;
+    if (e >= units * size) return;
+    const long unit = e / size;
+    const int at = (int)(e - unit * size);
+    V cur = {};
+    if (in) cur = *(const V*)(in + e);
+    float* s = seg + unit * segs * size + at;
+    const float* th = through + unit * segs;
+    constexpr int AHEAD = 8;   // loads in flight
+    for (int g0 = 0; g0 < segs; g0 += AHEAD) {
+        V add[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++)
+            if (g0 + i + 1 < segs) add[i] = *(const V*)(s + (long)(g0 + i) * size);
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++)
+            if (g0 + i < segs) {
+                *(V*)(s + (long)(g0 + i) * size) = cur;
+                if (g0 + i + 1 < segs) {
+                    const float t = th[g0 + i];
+                    cur = t != 0.f ? cur * t + add[i] : add[i];   // behind a cut nothing of the old state is left
                 }
             }
     }
@@ -676,7 +800,7 @@ int z_slice(int type, int dy, int d) { return d <= 32 || (type != HUM_BF16 && y_
 
 template <int ST, int DY>
 void launch_walk_z(const WalkArgs& a, int dzs, hipStream_t s) {
-    const long units = (long)a.lanes * a.heads;
+    const long units = (long)a.lanes * a.heads * a.segs;
     const dim3 grid((unsigned)((units + XCDS - 1) / XCDS * XCDS * a.parts));
     if constexpr (ST == HUM_BF16 || DY < 128)
         if (dzs == 64) {
@@ -697,8 +821,22 @@ void launch_walk(int type, const WalkArgs& a, int dyw, int dzs, hipStream_t s) {
     else launch_walk_y<HUM_F32>(a, dyw, dzs, s);
 }
 
+// Few lanes and many steps: the walks are cut into segments that run side by side, each from the state that a first pass
+// over the segments before it and a scan have left for it (segments without outputs: half the work of a walk).
+struct Cut { int segs, steps; };
+constexpr int WAVES = 1024, MIN_CHUNKS = 4;   // one wave per SIMD; segments of 4 chunks at least
+Cut cut_of(const hum_decay_attn_args* p, int parts) {
+    const long waves = (long)p->lanes * p->heads * parts;
+    const int chunks = (p->steps + CH - 1) / CH;
+    if (waves == 0 || 2 * waves > WAVES || chunks < 2 * MIN_CHUNKS) return {1, p->steps};
+    long segs = WAVES / waves;
+    if (segs > chunks / MIN_CHUNKS) segs = chunks / MIN_CHUNKS;
+    const int per = (int)((chunks + segs - 1) / segs);
+    return {(chunks + per - 1) / per, per * CH};
+}
+
 // the roles of equal widths share a launch (their workgroups read the same rows at about the same time)
-void launch_roles(const hum_decay_attn_args* p, Role* r, int n, hipStream_t s) {
+void launch_roles(const hum_decay_attn_args* p, Role* r, int n, Cut c, bool last_only, hipStream_t s) {
     bool done[3] = {};
     for (int i = 0; i < n; i++) {
         if (done[i]) continue;
@@ -714,6 +852,9 @@ void launch_roles(const hum_decay_attn_args* p, Role* r, int n, hipStream_t s) {
         a.lanes = p->lanes;
         a.steps = p->steps;
         a.heads = p->heads;
+        a.segs = c.segs;
+        a.seg_steps = c.steps;
+        a.last_only = last_only;
         a.log_decay = p->log_decay;
         a.reset = p->reset;
         a.reset_lane = p->reset_lane;
@@ -729,9 +870,47 @@ void role_state(Role& r, const float* in, float* out, const hum_decay_attn_args*
     r.state_out = out;
     r.sy = y_is_k ? 1 : p->dk;
     r.sz = y_is_k ? p->dk : 1;
-    r.s_lane = (long)p->dk * p->dv;
-    r.s_vec = y_is_k && p->dk % 4 == 0 && ((uintptr_t)in | (uintptr_t)out) % 16 == 0;
+    r.in_unit = r.out_unit = (long)p->dk * p->dv;
+    r.s_vec = p->dk % 4 == 0 && ((uintptr_t)in | (uintptr_t)out) % 16 == 0;
 }
+
+uint64_t round16(uint64_t n) { return (n + 15) / 16 * 16; }
+// scratch of one cut walk: the segments' states, then their `through`
+uint64_t walk_bytes(const hum_decay_attn_args* p, Cut c) {
+    const uint64_t units = (uint64_t)p->lanes * p->heads * c.segs;
+    return c.segs > 1 ? round16(4 * units * p->dk * p->dv) + round16(4 * units) : 0;
+}
+// fills the scratch with the segments' entering states: `walk` is a role whose y side is the keys' (or queries')
+void run_segments(const hum_decay_attn_args* p, Role walk, float* scratch, Cut c, hipStream_t s) {
+    const long units = (long)p->lanes * p->heads, size = (long)p->dk * p->dv;
+    float* through = (float*)((char*)scratch + round16(4 * units * c.segs * size));
+    const float* in = walk.state_in;
+    walk.x = Rows{};
+    walk.out = Rows{};
+    walk.x.shared = walk.out.shared = 1;
+    walk.state_in = nullptr;
+    walk.state_out = scratch;
+    walk.out_unit = size * c.segs;
+    walk.out_seg = size;
+    walk.through = through;
+    walk.s_vec = p->dk % 4 == 0;
+    launch_roles(p, &walk, 1, c, false, s);
+    if (size % 4 == 0 && (uintptr_t)in % 16 == 0)
+        hipLaunchKernelGGL(scan_kernel<4>, dim3((unsigned)((units * size / 4 + 255) / 256)), dim3(256), 0, s, in, scratch, through, c.segs, units, (int)size);
+    else
+        hipLaunchKernelGGL(scan_kernel<1>, dim3((unsigned)((units * size + 255) / 256)), dim3(256), 0, s, in, scratch, through, c.segs, units, (int)size);
+}
+void enter_segments(Role& r, const float* scratch, const hum_decay_attn_args* p, Cut c) {
+    r.state_in = scratch;
+    r.in_unit = (long)p->dk * p->dv * c.segs;
+    r.in_seg = (long)p->dk * p->dv;
+}
+int parts_of(const hum_decay_attn_args* p, int dy, int dz) {
+    const int s = z_slice(p->type, dy, dz);
+    return (dz + s - 1) / s;
+}
+Cut forward_cut(const hum_decay_attn_args* p) { return cut_of(p, parts_of(p, p->dk, p->dv)); }
+Cut backward_cut(const hum_decay_attn_args* p) { return cut_of(p, 2 * parts_of(p, p->dv, p->dk) + parts_of(p, p->dk, p->dv)); }
 
 int launched(const char* fn) {
     const hipError_t st = hipGetLastError();
@@ -746,9 +925,9 @@ int hum_decay_attn_workspace(const hum_decay_attn_args* p, int32_t backward, uin
     const char* fn = "hum_decay_attn_workspace";
     if (const int rc = check_args(fn, p)) return rc;
     if (!bytes) return derr(HUM_ERR_ARG, fn, "null argument");
-    *bytes = 0;
-    if (backward && p->kv_heads != p->heads)
-        *bytes = 4ull * p->lanes * p->steps * p->heads * (uint64_t)(p->dk + p->dv);
+    *bytes = backward ? 2 * walk_bytes(p, backward_cut(p)) : walk_bytes(p, forward_cut(p));
+    if (backward && p->kv_heads != p->heads)   // the heads' partial gradients of shared keys and values
+        *bytes += round16(4ull * p->lanes * p->steps * p->heads * p->dk) + 4ull * p->lanes * p->steps * p->heads * p->dv;
     return HUM_OK;
 }
 
@@ -775,7 +954,12 @@ int hum_decay_attn(const hum_decay_attn_args* p, const hum_rows* out, void* work
     r.s_pair = r.s_in = p->scale;
     r.s_add = 1.f;
     role_state(r, p->state_in, p->state_out, p, true);
-    launch_roles(p, &r, 1, (hipStream_t)stream);
+    const Cut c = forward_cut(p);
+    if (c.segs > 1) {
+        run_segments(p, r, (float*)workspace, c, (hipStream_t)stream);
+        enter_segments(r, (const float*)workspace, p, c);
+    }
+    launch_roles(p, &r, 1, c, true, (hipStream_t)stream);
     return launched(fn);
 }
 
@@ -808,8 +992,12 @@ int hum_decay_attn_backward(const hum_decay_attn_args* p, const hum_rows* d_out,
     if (!dev.ok) return derr(HUM_ERR_HIP, fn, "hipSetDevice");
     const Rows q = rows_of(p->q, 1, size, p->dk), k = rows_of(p->k, group, size, p->dk);
     const Rows v = rows_of(p->v, group, size, p->dv), g = rows_of(*d_out, 1, size, p->dv);
-    float* part_k = (float*)workspace;
-    float* part_v = part_k + (group > 1 ? (size_t)p->lanes * p->steps * p->heads * p->dk : 0);
+    hipStream_t s = (hipStream_t)stream;
+    const Cut c = backward_cut(p);
+    float* const seg_s = (float*)workspace;   // segments' states, their gradients, the shared heads' partial gradients
+    float* const seg_r = (float*)((char*)seg_s + walk_bytes(p, c));
+    float* const part_k = (float*)((char*)seg_r + walk_bytes(p, c));
+    float* const part_v = (float*)((char*)part_k + round16(4ull * p->lanes * p->steps * p->heads * p->dk));
     const hum_rows pk = {part_k, (int64_t)p->steps * p->heads * p->dk, (int64_t)p->heads * p->dk, p->dk};
     const hum_rows pv = {part_v, (int64_t)p->steps * p->heads * p->dv, (int64_t)p->heads * p->dv, p->dv};
     Role r[3];
@@ -846,8 +1034,27 @@ int hum_decay_attn_backward(const hum_decay_attn_args* p, const hum_rows* d_out,
         w.s_in = 1.f;
         role_state(w, d_state_out, d_state_in, p, true);
     }
-    hipStream_t s = (hipStream_t)stream;
-    launch_roles(p, r, n, s);
+    if (c.segs > 1) {
+        Role w = {};
+        if (gq.ptr) {
+            w.y = k; w.z = v;
+            w.dy = p->dk; w.dz = p->dv;
+            w.s_add = 1.f;
+            role_state(w, p->state_in, nullptr, p, true);
+            run_segments(p, w, seg_s, c, s);
+        }
+        if (gk.ptr || gv.ptr || d_state_in) {
+            w = Role{};
+            w.y = q; w.z = g;
+            w.dy = p->dk; w.dz = p->dv;
+            w.rev = 1;
+            w.s_add = p->scale;
+            role_state(w, d_state_out, nullptr, p, true);
+            run_segments(p, w, seg_r, c, s);
+        }
+        for (int i = 0; i < n; i++) enter_segments(r[i], r[i].rev ? seg_r : seg_s, p, c);
+    }
+    launch_roles(p, r, n, c, true, s);
     if (group > 1 && p->steps) {
         const long rows = (long)p->lanes * p->steps;
         struct { const hum_rows* o; const float* part; int d; } sums[2] = {{&gk, part_k, p->dk}, {&gv, part_v, p->dv}};
