@@ -34,6 +34,7 @@
 #include <cmath>
 #include <cstdint>
 #include <cstdio>
+#include <type_traits>
 
 #include "../../include/humanoid_env.h"
 
@@ -56,7 +57,7 @@ struct Rows {               // [lane, step, head, channel] with unit channel str
     void* p;
     long lane, step, head;  // strides in elements
     int shared;             // heads that read one of its heads
-    int vec;                // 16-byte loads of 8 channels are aligned
+    int vec;                // 8 channels are 16 aligned bytes, and 32 steps span less than 2^31 bytes
 };
 
 struct Role {
@@ -70,7 +71,7 @@ struct Role {
     float* through;         // [(lane, head), segment]: what the segment leaves of an entering state; NULL = not wanted
     long sy, sz;            // one of them is 1
     long in_unit, in_seg, out_unit, out_seg;   // from one (lane, head) / segment to the next
-    int s_vec;              // 16-byte aligned rows of the unit stride
+    int s_vec;              // the state's rows of unit stride are 16-byte aligned
     int slice0;             // first workgroup part of this role
 };
 
@@ -86,27 +87,42 @@ struct WalkArgs {
     const int* lengths;
 };
 
+// ---- buffer accesses: a uniform base in scalar registers, a 32-bit byte offset per lane; loads beyond the buffer give
+// zeros and stores there do nothing, so a masked lane takes an offset outside instead of a branch (a branch around each
+// load made the loads wait for one another: 16 of a 64 x 64 state took 25 800 cycles)
+typedef __amdgpu_buffer_rsrc_t Buf;
+constexpr int OUTSIDE = (int)0x80000000;
+__device__ __forceinline__ Buf buffer(const void* p) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, p ? 0x80000000u : 0u, 0x00020000);
+}
+__device__ __forceinline__ u32x4 buf_load(Buf b, int off) { return __builtin_amdgcn_raw_buffer_load_b128(b, off, 0, 0); }
+__device__ __forceinline__ void buf_store(Buf b, int off, u32x4 v) { __builtin_amdgcn_raw_buffer_store_b128(v, b, off, 0, 0); }
+__device__ __forceinline__ f32x4 buf_load4(Buf b, int off) { return __builtin_bit_cast(f32x4, buf_load(b, off)); }
+__device__ __forceinline__ void buf_store4(Buf b, int off, f32x4 v) { buf_store(b, off, __builtin_bit_cast(u32x4, v)); }
+
 // ---- the element types: ST storage, operands of 8 consecutive contraction indexes per lane
 template <int ST> struct Num;   // HUM_F32 / HUM_F16: float32 matrix instructions
 
 template <> struct Num<HUM_BF16> {
     typedef bf16x8 Op;
     typedef __bf16 Elem;
-    static constexpr int PAD = 8, PARTS = 3;
+    static constexpr int PAD = 8, PARTS = 3, SIZE = 2;
     static __device__ __forceinline__ Op zero() { return Op{}; }
-    static __device__ __forceinline__ Op load(const void* p, long off, int n, bool vec) {
+    static __device__ __forceinline__ Op load(Buf b, int off) { return __builtin_bit_cast(Op, buf_load(b, off)); }
+    static __device__ __forceinline__ void store(Buf b, int off, f32x8 v) {
+        buf_store(b, off, __builtin_bit_cast(u32x4, __builtin_convertvector(v, Op)));   // to nearest, ties to even
+    }
+    static __device__ __forceinline__ Op load(const void* p, long off, int n) {   // n of 8 elements, any alignment
         const __bf16* e = (const __bf16*)p + off;
-        if (vec) return *(const Op*)e;
         Op v = {};
 #pragma unroll
         for (int j = 0; j < 8; j++)
             if (j < n) v[j] = e[j];
         return v;
     }
-    static __device__ __forceinline__ void store(void* p, long off, int n, bool vec, f32x8 v) {
+    static __device__ __forceinline__ void store(void* p, long off, int n, f32x8 v) {
         __bf16* e = (__bf16*)p + off;
-        const Op o = __builtin_convertvector(v, Op);   // to nearest, ties to even
-        if (vec) { *(Op*)e = o; return; }
+        const Op o = __builtin_convertvector(v, Op);
 #pragma unroll
         for (int j = 0; j < 8; j++)
             if (j < n) e[j] = o[j];
@@ -145,49 +161,34 @@ template <> struct Num<HUM_BF16> {
 template <int ST> struct Num {
     typedef f32x8 Op;
     typedef float Elem;
-    static constexpr int PAD = 4, PARTS = 1;
+    static constexpr int PAD = 4, PARTS = 1, SIZE = ST == HUM_F16 ? 2 : 4;
     static __device__ __forceinline__ Op zero() { return Op{}; }
-    static __device__ __forceinline__ Op load(const void* p, long off, int n, bool vec) {
+    static __device__ __forceinline__ Op load(Buf b, int off) {
+        if constexpr (ST == HUM_F16) return __builtin_convertvector(__builtin_bit_cast(f16x8, buf_load(b, off)), Op);
+        else return __builtin_shufflevector(buf_load4(b, off), buf_load4(b, off + 16), 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+    static __device__ __forceinline__ void store(Buf b, int off, f32x8 v) {
         if constexpr (ST == HUM_F16) {
-            const _Float16* e = (const _Float16*)p + off;
-            if (vec) return __builtin_convertvector(*(const f16x8*)e, Op);
-            Op v = {};
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-                if (j < n) v[j] = (float)e[j];
-            return v;
+            buf_store(b, off, __builtin_bit_cast(u32x4, __builtin_convertvector(v, f16x8)));
         } else {
-            const float* e = (const float*)p + off;
-            if (vec) {
-                const f32x4 a = *(const f32x4*)e, b = *(const f32x4*)(e + 4);
-                return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-            }
-            Op v = {};
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-                if (j < n) v[j] = e[j];
-            return v;
+            buf_store4(b, off, __builtin_shufflevector(v, v, 0, 1, 2, 3));
+            buf_store4(b, off + 16, __builtin_shufflevector(v, v, 4, 5, 6, 7));
         }
     }
-    static __device__ __forceinline__ void store(void* p, long off, int n, bool vec, f32x8 v) {
-        if constexpr (ST == HUM_F16) {
-            _Float16* e = (_Float16*)p + off;
-            const f16x8 o = __builtin_convertvector(v, f16x8);
-            if (vec) { *(f16x8*)e = o; return; }
+    typedef typename std::conditional<ST == HUM_F16, _Float16, float>::type Stored;
+    static __device__ __forceinline__ Op load(const void* p, long off, int n) {
+        const Stored* e = (const Stored*)p + off;
+        Op v = {};
 #pragma unroll
-            for (int j = 0; j < 8; j++)
-                if (j < n) e[j] = o[j];
-        } else {
-            float* e = (float*)p + off;
-            if (vec) {
-                *(f32x4*)e = __builtin_shufflevector(v, v, 0, 1, 2, 3);
-                *(f32x4*)(e + 4) = __builtin_shufflevector(v, v, 4, 5, 6, 7);
-                return;
-            }
+        for (int j = 0; j < 8; j++)
+            if (j < n) v[j] = (float)e[j];
+        return v;
+    }
+    static __device__ __forceinline__ void store(void* p, long off, int n, f32x8 v) {
+        Stored* e = (Stored*)p + off;
 #pragma unroll
-            for (int j = 0; j < 8; j++)
-                if (j < n) e[j] = v[j];
-        }
+        for (int j = 0; j < 8; j++)
+            if (j < n) e[j] = (Stored)v[j];
     }
     static __device__ __forceinline__ bool finite(Op v) {
         bool bad = false;
@@ -249,8 +250,9 @@ __device__ __forceinline__ f32x4 quad_transpose(f32x4 v) {
 // 256 registers
 constexpr int walk_waves(int st, int dy, int dz) { return dy * dz * (st == HUM_BF16 ? 1 : 2) <= 4096 ? 2 : 1; }
 
-// One wave per workgroup.  DY, DZ: channels of y and of the z slice rounded up to 32.
-template <int ST, int DY, int DZ>
+// One wave per workgroup.  DY, DZ: channels of y and of the z slice rounded up to 32.  FAST: every operand may be accessed
+// 16 bytes at a time through buffers; else element by element, at any alignment and stride.
+template <int ST, int DY, int DZ, bool FAST>
 __global__ void __launch_bounds__(64, walk_waves(ST, DY, DZ)) walk_kernel(WalkArgs a) {
     typedef Num<ST> M;
     typedef typename M::Op Op;
@@ -278,7 +280,7 @@ __global__ void __launch_bounds__(64, walk_waves(ST, DY, DZ)) walk_kernel(WalkAr
     const int steps = a.steps;
     int len = steps;
     if (a.lengths) {
-        len = a.lengths[b];
+        len = __builtin_amdgcn_readfirstlane(a.lengths[b]);
         len = len < 0 ? 0 : len > steps ? steps : len;
     }
     const int rev = R.rev;
@@ -291,48 +293,74 @@ __global__ void __launch_bounds__(64, walk_waves(ST, DY, DZ)) walk_kernel(WalkAr
     auto row_of = [&](int tile) { return 8 * (r >> 2) + 4 * tile + (r & 3); };
 
     // ---- rows of a chunk: x by walk step 16 c + r, y and z by step row_of(t)
-    // (64-bit positions of the lane's first rows; its other rows and the next chunk's are uniform distances away)
-    const long dir = rev ? -1 : 1, first = rev ? len - 1 - seg0 : seg0;
-    auto start = [&](const Rows& m, int row) {
-        return (long)b * m.lane + (long)(h / m.shared) * m.head + (first + dir * row) * m.step;
-    };
-    long px = start(R.x, r), py = start(R.y, row_of(0)), pz = start(R.z, row_of(0)), po = start(R.out, r);
-    const long sx = dir * R.x.step, sy = dir * R.y.step, sz = dir * R.z.step, so = dir * R.out.step;
+    auto head_of = [&](const Rows& m) { return (long)b * m.lane + (long)(h / m.shared) * m.head; };
+    const long hx = head_of(R.x), hy = head_of(R.y), hz = head_of(R.z), ho = head_of(R.out);
     const unsigned char* marks = a.reset ? a.reset + (long)b * a.reset_lane : nullptr;
     auto time = [&](int n) { return rev ? len - 1 - n : n; };   // of walk step n
+    // a chunk's rows in a buffer that starts at the earliest of its times
+    auto chunk = [&](const Rows& m, long head, int n0, int L, int size) {
+        return buffer(m.p ? (const char*)m.p + (head + (long)(rev ? len - n0 - L : n0) * m.step) * size : nullptr);
+    };
+    auto offset = [&](const Rows& m, int n, int L, int size) { return (rev ? L - 1 - n : n) * (int)(m.step * size); };
+    auto steps_from = [&](int n0) { return end - n0 < CH ? end - n0 : CH; };
     Op X[2][KY], Y[2][KY], Z[2][KZ];
     bool mark = false;
     auto load_x = [&](int n0) {
+        const int L = steps_from(n0);
+        if constexpr (FAST) {
+            const Buf bx = chunk(R.x, hx, n0, L, M::SIZE);
 #pragma unroll
-        for (int c = 0; c < 2; c++) {
-            const int n = n0 + 16 * c + r;
-            const long at = px + 16 * c * sx;
+            for (int c = 0; c < 2; c++) {
+                const int n = 16 * c + r, at = offset(R.x, n, L, M::SIZE) + 8 * g * M::SIZE;
 #pragma unroll
-            for (int k = 0; k < KY; k++) {
-                const int d = 32 * k + 8 * g;
-                X[c][k] = n < end && d < R.dy ? M::load(R.x.p, at + d, R.dy - d, R.x.vec) : M::zero();
+                for (int k = 0; k < KY; k++)
+                    X[c][k] = M::load(bx, n < L && 32 * k + 8 * g < R.dy ? at + 32 * k * M::SIZE : OUTSIDE);
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                const int n = 16 * c + r;
+                const long at = hx + (long)time(n0 + n) * R.x.step;
+#pragma unroll
+                for (int k = 0; k < KY; k++) {
+                    const int d = 32 * k + 8 * g;
+                    X[c][k] = n < L && d < R.dy ? M::load(R.x.p, at + d, R.dy - d) : M::zero();
+                }
             }
         }
-        px += CH * sx;
     };
     auto load_yz = [&](int n0) {
+        const int L = steps_from(n0);
+        if constexpr (FAST) {
+            const Buf by = chunk(R.y, hy, n0, L, M::SIZE), bz = chunk(R.z, hz, n0, L, M::SIZE);
 #pragma unroll
-        for (int t = 0; t < 2; t++) {
-            const int n = n0 + row_of(t);
-            const long aty = py + 4 * t * sy, atz = pz + 4 * t * sz;
+            for (int t = 0; t < 2; t++) {
+                const int n = row_of(t);
+                const int aty = offset(R.y, n, L, M::SIZE) + 8 * g * M::SIZE, atz = offset(R.z, n, L, M::SIZE) + (dz0 + 8 * g) * M::SIZE;
 #pragma unroll
-            for (int k = 0; k < KY; k++) {
-                const int d = 32 * k + 8 * g;
-                Y[t][k] = n < end && d < R.dy ? M::load(R.y.p, aty + d, R.dy - d, R.y.vec) : M::zero();
+                for (int k = 0; k < KY; k++)
+                    Y[t][k] = M::load(by, n < L && 32 * k + 8 * g < R.dy ? aty + 32 * k * M::SIZE : OUTSIDE);
+#pragma unroll
+                for (int k = 0; k < KZ; k++)
+                    Z[t][k] = M::load(bz, n < L && dz0 + 32 * k + 8 * g < R.dz ? atz + 32 * k * M::SIZE : OUTSIDE);
             }
+        } else {
 #pragma unroll
-            for (int k = 0; k < KZ; k++) {
-                const int d = dz0 + 32 * k + 8 * g;
-                Z[t][k] = n < end && d < R.dz ? M::load(R.z.p, atz + d, R.dz - d, R.z.vec) : M::zero();
+            for (int t = 0; t < 2; t++) {
+                const int n = row_of(t);
+                const long aty = hy + (long)time(n0 + n) * R.y.step, atz = hz + (long)time(n0 + n) * R.z.step;
+#pragma unroll
+                for (int k = 0; k < KY; k++) {
+                    const int d = 32 * k + 8 * g;
+                    Y[t][k] = n < L && d < R.dy ? M::load(R.y.p, aty + d, R.dy - d) : M::zero();
+                }
+#pragma unroll
+                for (int k = 0; k < KZ; k++) {
+                    const int d = dz0 + 32 * k + 8 * g;
+                    Z[t][k] = n < L && d < R.dz ? M::load(R.z.p, atz + d, R.dz - d) : M::zero();
+                }
             }
         }
-        py += CH * sy;
-        pz += CH * sz;
         // bit j separates the chunk's walk steps j - 1 and j (bit 0 the entering state, bit L the leaving one).  An
         // episode's first step is cut off from what time puts before it, so the backward walk has it one later.
         if (marks) {
@@ -350,33 +378,35 @@ __global__ void __launch_bounds__(64, walk_waves(ST, DY, DZ)) walk_kernel(WalkAr
     auto zc = [&](int j) { return dz0 + 32 * (j >> 1) + 8 * (r >> 2) + 4 * (j & 1) + (r & 3); };
     // rows of unit stride are read 16 bytes at a time: along y directly, along z by one row a quad lane and a transpose
     const bool along_y = R.sy == 1;
+    auto state_at = [&](int i, int j) {   // byte offset of a tile's 16 bytes
+        const int y0 = 32 * (i >> 1) + 8 * g + 4 * (i & 1), z = zc(j);
+        const int y = along_y ? y0 : y0 + (r & 3), z0 = along_y ? z : z - (r & 3);
+        return y < R.dy && z0 < R.dz ? 4 * (int)(y * R.sy + z0 * R.sz) : OUTSIDE;
+    };
     {
         const float* s = R.state_in ? R.state_in + (long)unit * R.in_unit + (long)seg * R.in_seg : nullptr;
-#pragma unroll
-        for (int j = 0; j < 2 * KZ; j++)
-#pragma unroll
-            for (int i = 0; i < 2 * KY; i++) {
-                const int y0 = 32 * (i >> 1) + 8 * g + 4 * (i & 1), z = zc(j);
-                f32x4 v = {0.f, 0.f, 0.f, 0.f};
-                if (s) {
-                    if (!R.s_vec) {
-#pragma unroll
-                        for (int q = 0; q < 4; q++)
-                            if (z < R.dz && y0 + q < R.dy) v[q] = s[(long)z * R.sz + (long)(y0 + q) * R.sy];
-                    } else if (along_y) {
-                        if (z < R.dz && y0 < R.dy) v = *(const f32x4*)(s + (long)z * R.sz + y0);
-                    } else {
-                        const int y = y0 + (r & 3), z4 = z - (r & 3);
-                        if (z4 < R.dz && y < R.dy) v = *(const f32x4*)(s + (long)y * R.sy + z4);
-                    }
-                }
-                S[i][j] = v;
-            }
-        if (s && R.s_vec && !along_y)
+        if constexpr (FAST) {
+            const Buf bs = buffer(s);
 #pragma unroll
             for (int j = 0; j < 2 * KZ; j++)
 #pragma unroll
-                for (int i = 0; i < 2 * KY; i++) S[i][j] = quad_transpose(S[i][j]);
+                for (int i = 0; i < 2 * KY; i++) S[i][j] = buf_load4(bs, state_at(i, j));
+            if (!along_y)
+#pragma unroll
+                for (int j = 0; j < 2 * KZ; j++)
+#pragma unroll
+                    for (int i = 0; i < 2 * KY; i++) S[i][j] = quad_transpose(S[i][j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 2 * KZ; j++)
+#pragma unroll
+                for (int i = 0; i < 2 * KY; i++) {
+                    const int y0 = 32 * (i >> 1) + 8 * g + 4 * (i & 1), z = zc(j);
+#pragma unroll
+                    for (int q = 0; q < 4; q++)
+                        S[i][j][q] = s && z < R.dz && y0 + q < R.dy ? s[(long)z * R.sz + (long)(y0 + q) * R.sy] : 0.f;
+                }
+        }
     }
 
     float w_in[2];
@@ -489,10 +519,17 @@ __global__ void __launch_bounds__(64, walk_waves(ST, DY, DZ)) walk_kernel(WalkAr
 #pragma unroll
                     for (int c = 0; c < 2; c++) {
                         const int n = 16 * c + r;
-                        if (n >= lo && n < hi && d < R.dz) {
-                            const long at = po + 16 * c * so + d;
-                            if (R.out_f32) Num<HUM_F32>::store(R.out.p, at, R.dz - d, R.out.vec, pair(o[c][0], o[c][1]));
-                            else M::store(R.out.p, at, R.dz - d, R.out.vec, pair(o[c][0], o[c][1]));
+                        const bool in = n >= lo && n < hi && d < R.dz;
+                        const f32x8 v = pair(o[c][0], o[c][1]);
+                        if constexpr (FAST) {
+                            if (R.out_f32)
+                                Num<HUM_F32>::store(chunk(R.out, ho, n0, L, 4), in ? offset(R.out, n, L, 4) + 4 * d : OUTSIDE, v);
+                            else
+                                M::store(chunk(R.out, ho, n0, L, M::SIZE), in ? offset(R.out, n, L, M::SIZE) + M::SIZE * d : OUTSIDE, v);
+                        } else if (in) {
+                            const long at = ho + (long)time(n0 + n) * R.out.step + d;
+                            if (R.out_f32) Num<HUM_F32>::store(R.out.p, at, R.dz - d, v);
+                            else M::store(R.out.p, at, R.dz - d, v);
                         }
                     }
                 }
@@ -558,7 +595,6 @@ __global__ void __launch_bounds__(64, walk_waves(ST, DY, DZ)) walk_kernel(WalkAr
             }
             lo = hi;
         }
-        po += CH * so;
     }
 
     // ---- the steps behind the lane's length
@@ -568,28 +604,35 @@ __global__ void __launch_bounds__(64, walk_waves(ST, DY, DZ)) walk_kernel(WalkAr
             for (int k = 0; k < KZ; k++) {
                 const int d = dz0 + 32 * k + 8 * g;
                 if (d < R.dz) {
-                    const long at = (long)b * R.out.lane + (long)(h / R.out.shared) * R.out.head + (long)n * R.out.step + d;
-                    if (R.out_f32) Num<HUM_F32>::store(R.out.p, at, R.dz - d, R.out.vec, f32x8{});
-                    else M::store(R.out.p, at, R.dz - d, R.out.vec, f32x8{});
+                    if (R.out_f32) Num<HUM_F32>::store(R.out.p, ho + (long)n * R.out.step + d, R.dz - d, f32x8{});
+                    else M::store(R.out.p, ho + (long)n * R.out.step + d, R.dz - d, f32x8{});
                 }
             }
     if (R.through && l == 0 && dz0 == 0) R.through[item] = passed;
     if (R.state_out && (!a.last_only || seg + 1 == a.segs)) {
         float* s = R.state_out + (long)unit * R.out_unit + (long)seg * R.out_seg;
+        if constexpr (FAST) {
+            const Buf bs = buffer(s);
+            if (!along_y)
 #pragma unroll
-        for (int j = 0; j < 2 * KZ; j++)
+                for (int j = 0; j < 2 * KZ; j++)
 #pragma unroll
-            for (int i = 0; i < 2 * KY; i++) {
-                const int y0 = 32 * (i >> 1) + 8 * g + 4 * (i & 1), z = zc(j);
-                if (z >= R.dz) continue;
-                if (R.s_vec && along_y) {
-                    if (y0 < R.dy) *(f32x4*)(s + (long)z * R.sz + y0) = S[i][j];
-                } else {
+                    for (int i = 0; i < 2 * KY; i++) S[i][j] = quad_transpose(S[i][j]);
+#pragma unroll
+            for (int j = 0; j < 2 * KZ; j++)
+#pragma unroll
+                for (int i = 0; i < 2 * KY; i++) buf_store4(bs, state_at(i, j), S[i][j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 2 * KZ; j++)
+#pragma unroll
+                for (int i = 0; i < 2 * KY; i++) {
+                    const int y0 = 32 * (i >> 1) + 8 * g + 4 * (i & 1), z = zc(j);
 #pragma unroll
                     for (int q = 0; q < 4; q++)
-                        if (y0 + q < R.dy) s[(long)z * R.sz + (long)(y0 + q) * R.sy] = S[i][j][q];
+                        if (z < R.dz && y0 + q < R.dy) s[(long)z * R.sz + (long)(y0 + q) * R.sy] = S[i][j][q];
                 }
-            }
+        }
     }
 }
 
@@ -643,7 +686,7 @@ __global__ void __launch_bounds__(256) share_kernel(const float* part, Rows out,
 
 // ---- single step: S = a S + v k^T, o = scale S q, all in float32 on the vector units - the state is read and written
 // once (8 bytes for 4 operations), so HBM bounds it.  LPR lanes of 4 key channels hold one row of S; a wave has
-// 64 / LPR rows in one load and U loads in flight.
+// 64 / LPR rows in one load and U loads in flight, issued before anything that decides whether they are used.
 struct StepArgs {
     Rows q, k, v, out;
     const float* log_decay;
@@ -653,9 +696,7 @@ struct StepArgs {
     long reset_lane;
     const unsigned char* active;
     int heads, dk, dv, blocks;   // blocks: workgroups per (lane, head)
-    int s_vec;
     float scale;
-    long units;
 };
 
 template <int ST>
@@ -663,6 +704,13 @@ __device__ __forceinline__ float elem(const void* p, long at) {
     if constexpr (ST == HUM_F32) return ((const float*)p)[at];
     else if constexpr (ST == HUM_BF16) return (float)((const __bf16*)p)[at];
     else return (float)((const _Float16*)p)[at];
+}
+
+template <int ST>
+__device__ __forceinline__ void put_elem(void* p, long at, float v) {
+    if constexpr (ST == HUM_F32) ((float*)p)[at] = v;
+    else if constexpr (ST == HUM_BF16) ((__bf16*)p)[at] = (__bf16)v;
+    else ((_Float16*)p)[at] = (_Float16)v;
 }
 
 template <int LPR>
@@ -675,77 +723,80 @@ __device__ __forceinline__ float row_sum(float v) {   // over LPR neighbouring l
     return v;
 }
 
-template <int ST, int LPR>
+// VEC: rows of S are 16-byte aligned multiples of 4 channels
+template <int ST, int LPR, bool VEC>
 __global__ void __launch_bounds__(256) step_kernel(StepArgs a) {
     constexpr int U = 4, ROWS = 64 / LPR;
-    const long unit = blockIdx.x / a.blocks;
-    const int blk = (int)(blockIdx.x - unit * a.blocks);
-    const long b = unit / a.heads;
-    const int h = (int)(unit - b * a.heads);
+    const int unit = blockIdx.x / a.blocks, blk = blockIdx.x - unit * a.blocks;
+    const int b = unit / a.heads, h = unit - b * a.heads;
     const int wave = threadIdx.x >> 6, l = threadIdx.x & 63;
     const int c0 = 4 * (l % LPR), row0 = (blk * 4 + wave) * U * ROWS + l / LPR;
-    const bool on = !a.active || a.active[b];
-    const bool fresh = a.reset && a.reset[b * a.reset_lane];
-    const float* si = a.state_in ? a.state_in + unit * a.dv * a.dk : nullptr;
-    float* so = a.state_out + unit * a.dv * a.dk;
-    const float lambda = __builtin_amdgcn_exp2f(a.log_decay[h] * 1.44269504088896340736f);
-    if (!on && si == so) si = nullptr;   // an idle lane's state in place stays as it is
+    const long size = (long)a.dv * a.dk;
+    const Buf si = buffer(a.state_in ? a.state_in + unit * size : nullptr), so = buffer(a.state_out + unit * size);
+    int at[U];   // byte offsets of a lane's 4 channels (VEC), else of the first
     f32x4 s[U];
 #pragma unroll
     for (int u = 0; u < U; u++) {
         const int row = row0 + u * ROWS;
-        s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (row < a.dv && si && (!fresh || !on)) {
-            if (a.s_vec) {
-                if (c0 < a.dk) s[u] = *(const f32x4*)(si + (long)row * a.dk + c0);
-            } else {
+        at[u] = row < a.dv && c0 < a.dk ? 4 * (row * a.dk + c0) : OUTSIDE;
+        if constexpr (VEC) {
+            s[u] = buf_load4(si, at[u]);
+        } else {
 #pragma unroll
-                for (int j = 0; j < 4; j++)
-                    if (c0 + j < a.dk) s[u][j] = si[(long)row * a.dk + c0 + j];
-            }
+            for (int j = 0; j < 4; j++)
+                s[u][j] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(si, c0 + j < a.dk ? at[u] + 4 * j : OUTSIDE, 0, 0));
         }
     }
-    const long qo = b * a.q.lane + (long)(h / a.q.shared) * a.q.head, ko = b * a.k.lane + (long)(h / a.k.shared) * a.k.head;
-    const long vo = b * a.v.lane + (long)(h / a.v.shared) * a.v.head, oo = b * a.out.lane + (long)h * a.out.head;
-    float q[4], k[4];
+    const long qo = (long)b * a.q.lane + (long)(h / a.q.shared) * a.q.head, ko = (long)b * a.k.lane + (long)(h / a.k.shared) * a.k.head;
+    const long vo = (long)b * a.v.lane + (long)(h / a.v.shared) * a.v.head, oo = (long)b * a.out.lane + (long)h * a.out.head;
+    float q[4], k[4], v[U];
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-        q[j] = c0 + j < a.dk ? elem<ST>(a.q.p, qo + c0 + j) : 0.f;
-        k[j] = c0 + j < a.dk ? elem<ST>(a.k.p, ko + c0 + j) : 0.f;
+    for (int j = 0; j < 4; j++) {   // (a channel behind the last reads the last: its k is made 0)
+        const int c = c0 + j < a.dk ? c0 + j : a.dk - 1;
+        q[j] = elem<ST>(a.q.p, qo + c);
+        k[j] = elem<ST>(a.k.p, ko + c);
     }
 #pragma unroll
     for (int u = 0; u < U; u++) {
         const int row = row0 + u * ROWS;
-        float o = 0.f;
+        v[u] = elem<ST>(a.v.p, vo + (row < a.dv ? row : a.dv - 1));
+    }
+    const bool on = !a.active || a.active[b];
+    const bool fresh = a.reset && a.reset[(long)b * a.reset_lane];
+    const float lambda = __builtin_amdgcn_exp2f(a.log_decay[h] * 1.44269504088896340736f);
+    const bool keep = !on && a.state_in == a.state_out;   // an idle lane's state in place stays as it is
+    float o[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        o[u] = 0.f;
         if (on) {
-            const float v = row < a.dv ? elem<ST>(a.v.p, vo + row) : 0.f;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                s[u][j] = c0 + j < a.dk ? s[u][j] * lambda + v * k[j] : 0.f;
-                o += s[u][j] * q[j];
+                const bool in = c0 + j < a.dk;
+                s[u][j] = in ? (fresh ? 0.f : s[u][j] * lambda) + v[u] * k[j] : 0.f;
+                o[u] += in ? s[u][j] * q[j] : 0.f;
             }
-            o = row_sum<LPR>(o) * a.scale;
+            o[u] = row_sum<LPR>(o[u]) * a.scale;
         }
-        if (row < a.dv) {
-            if (on || si) {
-                if (a.s_vec) {
-                    if (c0 < a.dk) *(f32x4*)(so + (long)row * a.dk + c0) = s[u];
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        if (c0 + j < a.dk) so[(long)row * a.dk + c0 + j] = s[u][j];
-                }
-            } else if (a.state_in == nullptr) {   // idle and no state yet: an empty one
+        if (!keep) {
+            if constexpr (VEC) {
+                buf_store4(so, at[u], s[u]);
+            } else {
 #pragma unroll
                 for (int j = 0; j < 4; j++)
-                    if (c0 + j < a.dk) so[(long)row * a.dk + c0 + j] = 0.f;
-            }
-            if (l % LPR == 0) {
-                if constexpr (ST == HUM_F32) ((float*)a.out.p)[oo + row] = o;
-                else if constexpr (ST == HUM_BF16) ((__bf16*)a.out.p)[oo + row] = (__bf16)o;
-                else ((_Float16*)a.out.p)[oo + row] = (_Float16)o;
+                    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, (float)s[u][j]), so, c0 + j < a.dk ? at[u] + 4 * j : OUTSIDE, 0, 0);
             }
         }
+    }
+    // every lane of a row has its sum: lane u of the row stores the u-th
+    if constexpr (LPR >= U) {
+        const int u = l % LPR, row = row0 + u * ROWS;
+        const float x = u == 0 ? o[0] : u == 1 ? o[1] : u == 2 ? o[2] : o[3];
+        if (u < U && row < a.dv) put_elem<ST>(a.out.p, oo + row, x);
+    } else {
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (l % LPR == 0 && row0 + u * ROWS < a.dv) put_elem<ST>(a.out.p, oo + row0 + u * ROWS, o[u]);
     }
 }
 
@@ -770,7 +821,8 @@ struct OnDevice {   // the caller's current device stays what it was
 int elem_size(int type) { return type == HUM_F32 ? 4 : 2; }
 
 Rows rows_of(const hum_rows& r, int shared, int size, int d) {
-    const bool vec = ((uintptr_t)r.ptr | (uintptr_t)(r.lane * size) | (uintptr_t)(r.step * size) | (uintptr_t)(r.head * size)) % 16 == 0 && d % 8 == 0;
+    const bool vec = ((uintptr_t)r.ptr | (uintptr_t)(r.lane * size) | (uintptr_t)(r.step * size) | (uintptr_t)(r.head * size)) % 16 == 0 &&
+                     d % 8 == 0 && r.step >= 0 && r.step < (1l << 31) / (CH * size);
     return Rows{r.ptr, (long)r.lane, (long)r.step, (long)r.head, shared, vec};
 }
 
@@ -798,16 +850,26 @@ int y_width(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
 // leave too few registers (a 128 x 64 state spills there)
 int z_slice(int type, int dy, int d) { return d <= 32 || (type != HUM_BF16 && y_width(dy) == 128) ? 32 : 64; }
 
-template <int ST, int DY>
-void launch_walk_z(const WalkArgs& a, int dzs, hipStream_t s) {
+template <int ST, int DY, int DZ>
+void launch_walk_f(const WalkArgs& a, hipStream_t s) {
     const long units = (long)a.lanes * a.heads * a.segs;
     const dim3 grid((unsigned)((units + XCDS - 1) / XCDS * XCDS * a.parts));
+    bool fast = true;
+    for (int i = 0; i < a.nroles; i++) {
+        const Role& r = a.r[i];
+        fast = fast && (!r.x.p || r.x.vec) && r.y.vec && r.z.vec && (!r.out.p || r.out.vec) && r.s_vec;
+    }
+    if (fast) hipLaunchKernelGGL((walk_kernel<ST, DY, DZ, true>), grid, dim3(64), 0, s, a);
+    else hipLaunchKernelGGL((walk_kernel<ST, DY, DZ, false>), grid, dim3(64), 0, s, a);
+}
+template <int ST, int DY>
+void launch_walk_z(const WalkArgs& a, int dzs, hipStream_t s) {
     if constexpr (ST == HUM_BF16 || DY < 128)
         if (dzs == 64) {
-            hipLaunchKernelGGL((walk_kernel<ST, DY, 64>), grid, dim3(64), 0, s, a);
+            launch_walk_f<ST, DY, 64>(a, s);
             return;
         }
-    hipLaunchKernelGGL((walk_kernel<ST, DY, 32>), grid, dim3(64), 0, s, a);
+    launch_walk_f<ST, DY, 32>(a, s);
 }
 template <int ST>
 void launch_walk_y(const WalkArgs& a, int dyw, int dzs, hipStream_t s) {
@@ -1074,16 +1136,20 @@ int hum_decay_attn_backward(const hum_decay_attn_args* p, const hum_rows* d_out,
 }  // extern "C"
 
 namespace {
+template <int ST, int LPR>
+void launch_step_v(const StepArgs& a, bool vec, dim3 grid, hipStream_t s) {
+    if (vec) hipLaunchKernelGGL((step_kernel<ST, LPR, true>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((step_kernel<ST, LPR, false>), grid, dim3(256), 0, s, a);
+}
 template <int ST>
-void launch_step(const StepArgs& a, int lpr, long grid, hipStream_t s) {
-    const dim3 g((unsigned)grid), b(256);
+void launch_step(const StepArgs& a, int lpr, bool vec, dim3 grid, hipStream_t s) {
     switch (lpr) {
-        case 1: hipLaunchKernelGGL((step_kernel<ST, 1>), g, b, 0, s, a); break;
-        case 2: hipLaunchKernelGGL((step_kernel<ST, 2>), g, b, 0, s, a); break;
-        case 4: hipLaunchKernelGGL((step_kernel<ST, 4>), g, b, 0, s, a); break;
-        case 8: hipLaunchKernelGGL((step_kernel<ST, 8>), g, b, 0, s, a); break;
-        case 16: hipLaunchKernelGGL((step_kernel<ST, 16>), g, b, 0, s, a); break;
-        default: hipLaunchKernelGGL((step_kernel<ST, 32>), g, b, 0, s, a); break;
+        case 1: launch_step_v<ST, 1>(a, vec, grid, s); break;
+        case 2: launch_step_v<ST, 2>(a, vec, grid, s); break;
+        case 4: launch_step_v<ST, 4>(a, vec, grid, s); break;
+        case 8: launch_step_v<ST, 8>(a, vec, grid, s); break;
+        case 16: launch_step_v<ST, 16>(a, vec, grid, s); break;
+        default: launch_step_v<ST, 32>(a, vec, grid, s); break;
     }
 }
 }  // namespace
@@ -1113,15 +1179,14 @@ extern "C" int hum_decay_attn_step(const hum_decay_attn_args* p, const uint8_t* 
     a.dk = p->dk;
     a.dv = p->dv;
     a.scale = p->scale;
-    a.units = (long)p->lanes * p->heads;
-    a.s_vec = p->dk % 4 == 0 && ((uintptr_t)p->state_in | (uintptr_t)p->state_out) % 16 == 0;
+    const bool vec = p->dk % 4 == 0 && ((uintptr_t)p->state_in | (uintptr_t)p->state_out) % 16 == 0;
     int lpr = 1;
     while (4 * lpr < p->dk) lpr *= 2;
     const int rows = 4 * 4 * (64 / lpr);
     a.blocks = (p->dv + rows - 1) / rows;
-    const long grid = a.units * a.blocks;
-    if (p->type == HUM_BF16) launch_step<HUM_BF16>(a, lpr, grid, (hipStream_t)stream);
-    else if (p->type == HUM_F16) launch_step<HUM_F16>(a, lpr, grid, (hipStream_t)stream);
-    else launch_step<HUM_F32>(a, lpr, grid, (hipStream_t)stream);
+    const dim3 grid((unsigned)(p->lanes * p->heads * a.blocks));
+    if (p->type == HUM_BF16) launch_step<HUM_BF16>(a, lpr, vec, grid, (hipStream_t)stream);
+    else if (p->type == HUM_F16) launch_step<HUM_F16>(a, lpr, vec, grid, (hipStream_t)stream);
+    else launch_step<HUM_F32>(a, lpr, vec, grid, (hipStream_t)stream);
     return launched(fn);
 }
