@@ -45,6 +45,7 @@ namespace {
 constexpr int CH = 32;             // steps per chunk: the contraction length of one bf16 matrix instruction
 constexpr int MAX_D = 128;         // channels per head
 constexpr int XCDS = 8;            // consecutive workgroups go to different XCDs
+constexpr int NEAR = 8;
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
@@ -57,7 +58,7 @@ struct Rows {               // [lane, step, head, channel] with unit channel str
     void* p;
     long lane, step, head;  // strides in elements
     int shared;             // heads that read one of its heads
-    int vec;                // 8 channels are 16 aligned bytes, and 32 steps span less than 2^31 bytes
+    int vec;                // 8 channels are 16 aligned bytes, steps do not overlap, 32 of them span less than 2^31 bytes
 };
 
 struct Role {
@@ -87,14 +88,16 @@ struct WalkArgs {
     const int* lengths;
 };
 
-// ---- buffer accesses: a uniform base in scalar registers, a 32-bit byte offset per lane; loads beyond the buffer give
-// zeros and stores there do nothing, so a masked lane takes an offset outside instead of a branch (a branch around each
-// load made the loads wait for one another: 16 of a 64 x 64 state took 25 800 cycles)
+// ---- buffer accesses: a uniform base in scalar registers, a 32-bit byte offset per lane; loads beyond the buffer's size
+// give zeros and stores there do nothing, so a masked lane takes an offset outside instead of a branch (a branch around
+// each load made the loads wait for one another: 16 of a 64 x 64 state took 25 800 cycles)
 typedef __amdgpu_buffer_rsrc_t Buf;
 constexpr int OUTSIDE = (int)0x80000000;
-__device__ __forceinline__ Buf buffer(const void* p) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, p ? 0x80000000u : 0u, 0x00020000);
+__device__ __forceinline__ Buf buffer(const void* p, int bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, p ? bytes : 0, 0x00020000);
 }
+// bit 31 where a is not below b: or'ed into an offset it puts it outside (no compare and select, no branch)
+__device__ __forceinline__ int beyond(int a, int b) { return ~((a - b) >> 31) & OUTSIDE; }
 __device__ __forceinline__ u32x4 buf_load(Buf b, int off) { return __builtin_amdgcn_raw_buffer_load_b128(b, off, 0, 0); }
 __device__ __forceinline__ void buf_store(Buf b, int off, u32x4 v) { __builtin_amdgcn_raw_buffer_store_b128(v, b, off, 0, 0); }
 __device__ __forceinline__ f32x4 buf_load4(Buf b, int off) { return __builtin_bit_cast(f32x4, buf_load(b, off)); }
@@ -268,9 +271,11 @@ __global__ void __launch_bounds__(64, walk_waves(ST, DY, DZ)) walk_kernel(WalkAr
     __shared__ float pow_pair[2 * CH], pow_add[2 * CH];
 
     const int l = threadIdx.x, g = l >> 4, r = l & 15;
-    // the parts (roles, slices) of one segment read the same rows: they go to one XCD, one after the other
-    const int block = blockIdx.x, part = block / XCDS % a.parts;
-    const int item = block / (XCDS * a.parts) * XCDS + block % XCDS;
+    // the parts (roles, slices) of one segment read the same rows, and NEAR segments in a row are neighbours in memory (the
+    // heads of a lane, lanes of a time-major step): they go to one XCD, one after the other.  Gradient of 4096 lanes x 32
+    // steps: 380 us, 407 with NEAR = 1, 377 with 32 (which leaves XCDs idle at few lanes)
+    const int block = blockIdx.x, part = block / XCDS % a.parts, turn = block / (XCDS * a.parts);
+    const int item = (turn / NEAR * XCDS + block % XCDS) * NEAR + turn % NEAR;
     if (item >= a.lanes * a.heads * a.segs) return;
     const int unit = item / a.segs, seg = item - unit * a.segs;
     const int ri = (a.nroles > 1 && part >= a.r[1].slice0) + (a.nroles > 2 && part >= a.r[2].slice0);
@@ -297,24 +302,27 @@ __global__ void __launch_bounds__(64, walk_waves(ST, DY, DZ)) walk_kernel(WalkAr
     const long hx = head_of(R.x), hy = head_of(R.y), hz = head_of(R.z), ho = head_of(R.out);
     const unsigned char* marks = a.reset ? a.reset + (long)b * a.reset_lane : nullptr;
     auto time = [&](int n) { return rev ? len - 1 - n : n; };   // of walk step n
-    // a chunk's rows in a buffer that starts at the earliest of its times
-    auto chunk = [&](const Rows& m, long head, int n0, int L, int size) {
-        return buffer(m.p ? (const char*)m.p + (head + (long)(rev ? len - n0 - L : n0) * m.step) * size : nullptr);
-    };
-    auto offset = [&](const Rows& m, int n, int L, int size) { return (rev ? L - 1 - n : n) * (int)(m.step * size); };
     auto steps_from = [&](int n0) { return end - n0 < CH ? end - n0 : CH; };
+    // a chunk of L steps as a buffer from its earliest time to its last row's end: the steps behind L lie outside (walking
+    // backwards: before it, at negative offsets)
+    const int dy = R.dy, dz = R.dz, out_size = R.out_f32 ? 4 : M::SIZE;
+    const int sx = (int)R.x.step * M::SIZE, sy = (int)R.y.step * M::SIZE, sz = (int)R.z.step * M::SIZE, so = (int)R.out.step * out_size;
+    auto chunk = [&](const void* p, long head, long step, int d, int n0, int L, int size) {
+        const char* at = (const char*)p + (head + (long)(rev ? len - n0 - L : n0) * step) * size;
+        return buffer(p ? at : nullptr, ((L - 1) * (int)step + d) * size);
+    };
+    auto row_at = [&](int n, int L, int step) { return (rev ? L - 1 - n : n) * step; };
     Op X[2][KY], Y[2][KY], Z[2][KZ];
     bool mark = false;
     auto load_x = [&](int n0) {
         const int L = steps_from(n0);
         if constexpr (FAST) {
-            const Buf bx = chunk(R.x, hx, n0, L, M::SIZE);
+            const Buf bx = chunk(R.x.p, hx, R.x.step, dy, n0, L, M::SIZE);
 #pragma unroll
             for (int c = 0; c < 2; c++) {
-                const int n = 16 * c + r, at = offset(R.x, n, L, M::SIZE) + 8 * g * M::SIZE;
+                const int at = row_at(16 * c + r, L, sx) + 8 * g * M::SIZE;
 #pragma unroll
-                for (int k = 0; k < KY; k++)
-                    X[c][k] = M::load(bx, n < L && 32 * k + 8 * g < R.dy ? at + 32 * k * M::SIZE : OUTSIDE);
+                for (int k = 0; k < KY; k++) X[c][k] = M::load(bx, (at + 32 * k * M::SIZE) | beyond(32 * k + 8 * g, dy));
             }
         } else {
 #pragma unroll
@@ -332,17 +340,14 @@ __global__ void __launch_bounds__(64, walk_waves(ST, DY, DZ)) walk_kernel(WalkAr
     auto load_yz = [&](int n0) {
         const int L = steps_from(n0);
         if constexpr (FAST) {
-            const Buf by = chunk(R.y, hy, n0, L, M::SIZE), bz = chunk(R.z, hz, n0, L, M::SIZE);
+            const Buf by = chunk(R.y.p, hy, R.y.step, dy, n0, L, M::SIZE), bz = chunk(R.z.p, hz, R.z.step, dz, n0, L, M::SIZE);
 #pragma unroll
             for (int t = 0; t < 2; t++) {
-                const int n = row_of(t);
-                const int aty = offset(R.y, n, L, M::SIZE) + 8 * g * M::SIZE, atz = offset(R.z, n, L, M::SIZE) + (dz0 + 8 * g) * M::SIZE;
+                const int aty = row_at(row_of(t), L, sy) + 8 * g * M::SIZE, atz = row_at(row_of(t), L, sz) + (dz0 + 8 * g) * M::SIZE;
 #pragma unroll
-                for (int k = 0; k < KY; k++)
-                    Y[t][k] = M::load(by, n < L && 32 * k + 8 * g < R.dy ? aty + 32 * k * M::SIZE : OUTSIDE);
+                for (int k = 0; k < KY; k++) Y[t][k] = M::load(by, (aty + 32 * k * M::SIZE) | beyond(32 * k + 8 * g, dy));
 #pragma unroll
-                for (int k = 0; k < KZ; k++)
-                    Z[t][k] = M::load(bz, n < L && dz0 + 32 * k + 8 * g < R.dz ? atz + 32 * k * M::SIZE : OUTSIDE);
+                for (int k = 0; k < KZ; k++) Z[t][k] = M::load(bz, (atz + 32 * k * M::SIZE) | beyond(dz0 + 32 * k + 8 * g, dz));
             }
         } else {
 #pragma unroll
@@ -378,15 +383,15 @@ __global__ void __launch_bounds__(64, walk_waves(ST, DY, DZ)) walk_kernel(WalkAr
     auto zc = [&](int j) { return dz0 + 32 * (j >> 1) + 8 * (r >> 2) + 4 * (j & 1) + (r & 3); };
     // rows of unit stride are read 16 bytes at a time: along y directly, along z by one row a quad lane and a transpose
     const bool along_y = R.sy == 1;
+    const int quad = along_y ? 0 : r & 3, s_y = along_y ? 1 : dz, s_z = along_y ? dy : 1;
     auto state_at = [&](int i, int j) {   // byte offset of a tile's 16 bytes
-        const int y0 = 32 * (i >> 1) + 8 * g + 4 * (i & 1), z = zc(j);
-        const int y = along_y ? y0 : y0 + (r & 3), z0 = along_y ? z : z - (r & 3);
-        return y < R.dy && z0 < R.dz ? 4 * (int)(y * R.sy + z0 * R.sz) : OUTSIDE;
+        const int y = 32 * (i >> 1) + 8 * g + 4 * (i & 1) + quad, z = zc(j) - quad;
+        return 4 * (__mul24(z, s_z) + __mul24(y, s_y)) | beyond(y, dy) | beyond(z, dz);
     };
     {
         const float* s = R.state_in ? R.state_in + (long)unit * R.in_unit + (long)seg * R.in_seg : nullptr;
         if constexpr (FAST) {
-            const Buf bs = buffer(s);
+            const Buf bs = buffer(s, 4 * dy * dz);
 #pragma unroll
             for (int j = 0; j < 2 * KZ; j++)
 #pragma unroll
@@ -427,18 +432,18 @@ __global__ void __launch_bounds__(64, walk_waves(ST, DY, DZ)) walk_kernel(WalkAr
             for (int k = 0; k < KZ; k++) sane = sane && M::finite(Z[t][k]);
         const bool slow = __any(!sane);
 
+        // the last cut at or before step n of the chunk: step n sees the steps from there on, and what entered the chunk only
+        // if there is none
+        auto cuts_to = [&](int n) { return cut & ((2ull << n) - 1); };
+        auto last_cut = [&](unsigned long long m) { return m ? 63 - __builtin_clzll(m) : 0; };
+        int seen[2];
         float wi[2];
-        int ct[2] = {0, 0}, cs[8] = {0, 0, 0, 0, 0, 0, 0, 0};   // cuts at or before a step
-        const int cl = __builtin_popcountll(cut);
-        if (cut) {
-            auto upto = [&](int j) { return __builtin_popcountll(cut & ((2ull << j) - 1)); };
 #pragma unroll
-            for (int c = 0; c < 2; c++) ct[c] = upto(16 * c + r);
-#pragma unroll
-            for (int j = 0; j < 8; j++) cs[j] = upto(8 * g + j);
+        for (int c = 0; c < 2; c++) {
+            const unsigned long long m = cuts_to(16 * c + r);
+            seen[c] = last_cut(m) - 8 * g;
+            wi[c] = m ? 0.f : w_in[c];
         }
-#pragma unroll
-        for (int c = 0; c < 2; c++) wi[c] = ct[c] == 0 ? w_in[c] : 0.f;
 
         lds_order();
 #pragma unroll
@@ -466,7 +471,7 @@ __global__ void __launch_bounds__(64, walk_waves(ST, DY, DZ)) walk_kernel(WalkAr
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     const float w = pow_pair[CH - 1 + 16 * c + r - 8 * g - j];
-                    v[j] = w != 0.f && cs[j] == ct[c] ? v[j] * w : 0.f;
+                    v[j] = w != 0.f && j >= seen[c] ? v[j] * w : 0.f;
                 }
                 M::template split<PO>(v, P[c]);
             }
@@ -481,8 +486,7 @@ __global__ void __launch_bounds__(64, walk_waves(ST, DY, DZ)) walk_kernel(WalkAr
 #pragma unroll
             for (int j = 0; j < 2 * KZ; j++) T[j] = M::column(lz, PZ, 8 * g, 32 * (j >> 1) + 4 * (j & 1), r);
             if (slow) {     // of which step lo sees its episode's, up to itself
-                const unsigned long long seen = cut & ((2ull << lo) - 1) & ~1ull;
-                const int from = seen ? 63 - __builtin_clzll(seen) : 0;
+                const int from = last_cut(cuts_to(lo));
 #pragma unroll
                 for (int j = 0; j < 2 * KZ; j++)
 #pragma unroll
@@ -510,7 +514,7 @@ __global__ void __launch_bounds__(64, walk_waves(ST, DY, DZ)) walk_kernel(WalkAr
 #pragma unroll
                         for (int c = 0; c < 2; c++) {
 #pragma unroll
-                            for (int q = 0; q < 4; q++) o[c][e][q] = ct[c] == 0 ? o[c][e][q] * wi[c] : 0.f;
+                            for (int q = 0; q < 4; q++) o[c][e][q] = wi[c] != 0.f ? o[c][e][q] * wi[c] : 0.f;
 #pragma unroll
                             for (int u = 0; u < PO; u++) M::mma(o[c][e], T[j], P[c][u]);
                         }
@@ -519,13 +523,14 @@ __global__ void __launch_bounds__(64, walk_waves(ST, DY, DZ)) walk_kernel(WalkAr
 #pragma unroll
                     for (int c = 0; c < 2; c++) {
                         const int n = 16 * c + r;
-                        const bool in = n >= lo && n < hi && d < R.dz;
                         const f32x8 v = pair(o[c][0], o[c][1]);
+                        const bool in = n >= lo && n < hi && d < dz;
                         if constexpr (FAST) {
-                            if (R.out_f32)
-                                Num<HUM_F32>::store(chunk(R.out, ho, n0, L, 4), in ? offset(R.out, n, L, 4) + 4 * d : OUTSIDE, v);
-                            else
-                                M::store(chunk(R.out, ho, n0, L, M::SIZE), in ? offset(R.out, n, L, M::SIZE) + M::SIZE * d : OUTSIDE, v);
+                            const Buf bo = chunk(R.out.p, ho, R.out.step, dz, n0, L, out_size);
+                            int at = (row_at(n, L, so) + d * out_size) | beyond(d, dz);
+                            if (slow) at = in ? at : OUTSIDE;
+                            if (R.out_f32) Num<HUM_F32>::store(bo, at, v);
+                            else M::store(bo, at, v);
                         } else if (in) {
                             const long at = ho + (long)time(n0 + n) * R.out.step + d;
                             if (R.out_f32) Num<HUM_F32>::store(R.out.p, at, R.dz - d, v);
@@ -538,9 +543,9 @@ __global__ void __launch_bounds__(64, walk_waves(ST, DY, DZ)) walk_kernel(WalkAr
             __builtin_amdgcn_sched_barrier(0);
             // ---- the state behind the chunk
             if (hi == L && (more || R.state_out)) {
-                const float through = cl == 0 ? power(L) : 0.f;
+                const float through = cut ? 0.f : power(L);
                 passed *= through;
-                if (cl == 0) {
+                if (!cut) {
 #pragma unroll
                     for (int i = 0; i < 2 * KY; i++)
 #pragma unroll
@@ -551,11 +556,12 @@ __global__ void __launch_bounds__(64, walk_waves(ST, DY, DZ)) walk_kernel(WalkAr
 #pragma unroll
                         for (int j = 0; j < 2 * KZ; j++) S[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
                 }
+                const int leaving = last_cut(cut);
                 float wo[8];   // (rows behind the chunk's last step are zeros)
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     const float w = pow_add[CH - 1 + L - 1 + rev - 8 * g - j];
-                    wo[j] = cs[j] == cl ? w : 0.f;
+                    wo[j] = 8 * g + j >= leaving ? w : 0.f;
                 }
                 // nothing joins it where an episode starts right behind (before, in time)
                 auto weigh = [&](Op x) {
@@ -612,7 +618,7 @@ __global__ void __launch_bounds__(64, walk_waves(ST, DY, DZ)) walk_kernel(WalkAr
     if (R.state_out && (!a.last_only || seg + 1 == a.segs)) {
         float* s = R.state_out + (long)unit * R.out_unit + (long)seg * R.out_seg;
         if constexpr (FAST) {
-            const Buf bs = buffer(s);
+            const Buf bs = buffer(s, 4 * dy * dz);
             if (!along_y)
 #pragma unroll
                 for (int j = 0; j < 2 * KZ; j++)
@@ -732,19 +738,19 @@ __global__ void __launch_bounds__(256) step_kernel(StepArgs a) {
     const int wave = threadIdx.x >> 6, l = threadIdx.x & 63;
     const int c0 = 4 * (l % LPR), row0 = (blk * 4 + wave) * U * ROWS + l / LPR;
     const long size = (long)a.dv * a.dk;
-    const Buf si = buffer(a.state_in ? a.state_in + unit * size : nullptr), so = buffer(a.state_out + unit * size);
+    const Buf si = buffer(a.state_in ? a.state_in + unit * size : nullptr, 4 * (int)size), so = buffer(a.state_out + unit * size, 4 * (int)size);
     int at[U];   // byte offsets of a lane's 4 channels (VEC), else of the first
     f32x4 s[U];
 #pragma unroll
     for (int u = 0; u < U; u++) {
         const int row = row0 + u * ROWS;
-        at[u] = row < a.dv && c0 < a.dk ? 4 * (row * a.dk + c0) : OUTSIDE;
+        at[u] = 4 * (__mul24(row, a.dk) + c0) | beyond(row, a.dv) | beyond(c0, a.dk);
         if constexpr (VEC) {
             s[u] = buf_load4(si, at[u]);
         } else {
 #pragma unroll
             for (int j = 0; j < 4; j++)
-                s[u][j] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(si, c0 + j < a.dk ? at[u] + 4 * j : OUTSIDE, 0, 0));
+                s[u][j] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(si, (at[u] + 4 * j) | beyond(c0 + j, a.dk), 0, 0));
         }
     }
     const long qo = (long)b * a.q.lane + (long)(h / a.q.shared) * a.q.head, ko = (long)b * a.k.lane + (long)(h / a.k.shared) * a.k.head;
@@ -784,7 +790,7 @@ __global__ void __launch_bounds__(256) step_kernel(StepArgs a) {
             } else {
 #pragma unroll
                 for (int j = 0; j < 4; j++)
-                    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, (float)s[u][j]), so, c0 + j < a.dk ? at[u] + 4 * j : OUTSIDE, 0, 0);
+                    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, (float)s[u][j]), so, (at[u] + 4 * j) | beyond(c0 + j, a.dk), 0, 0);
             }
         }
     }
@@ -822,7 +828,7 @@ int elem_size(int type) { return type == HUM_F32 ? 4 : 2; }
 
 Rows rows_of(const hum_rows& r, int shared, int size, int d) {
     const bool vec = ((uintptr_t)r.ptr | (uintptr_t)(r.lane * size) | (uintptr_t)(r.step * size) | (uintptr_t)(r.head * size)) % 16 == 0 &&
-                     d % 8 == 0 && r.step >= 0 && r.step < (1l << 31) / (CH * size);
+                     d % 8 == 0 && r.step >= d && r.step < (1l << 31) / (CH * size);
     return Rows{r.ptr, (long)r.lane, (long)r.step, (long)r.head, shared, vec};
 }
 
@@ -846,14 +852,14 @@ int check_args(const char* fn, const hum_decay_attn_args* p) {
 }
 
 int y_width(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
-// channels of z per workgroup: 64 (half as many waves form P twice), but 32 where float32 operands of 128 channels would
-// leave too few registers (a 128 x 64 state spills there)
-int z_slice(int type, int dy, int d) { return d <= 32 || (type != HUM_BF16 && y_width(dy) == 128) ? 32 : 64; }
+// channels of z per workgroup: 64 for bf16 (P is formed once for them), 32 where float32 matrix instructions take the time
+// and twice the waves shorten it (37 lanes x 203 steps, 6 heads, 40 / 72 channels: 51 us, 76 with 64)
+int z_slice(int type, int d) { return type != HUM_BF16 || d <= 32 ? 32 : 64; }
 
 template <int ST, int DY, int DZ>
 void launch_walk_f(const WalkArgs& a, hipStream_t s) {
     const long units = (long)a.lanes * a.heads * a.segs;
-    const dim3 grid((unsigned)((units + XCDS - 1) / XCDS * XCDS * a.parts));
+    const dim3 grid((unsigned)((units + XCDS * NEAR - 1) / (XCDS * NEAR) * (XCDS * NEAR) * a.parts));
     bool fast = true;
     for (int i = 0; i < a.nroles; i++) {
         const Role& r = a.r[i];
@@ -864,7 +870,7 @@ void launch_walk_f(const WalkArgs& a, hipStream_t s) {
 }
 template <int ST, int DY>
 void launch_walk_z(const WalkArgs& a, int dzs, hipStream_t s) {
-    if constexpr (ST == HUM_BF16 || DY < 128)
+    if constexpr (ST == HUM_BF16)
         if (dzs == 64) {
             launch_walk_f<ST, DY, 64>(a, s);
             return;
@@ -902,10 +908,10 @@ void launch_roles(const hum_decay_attn_args* p, Role* r, int n, Cut c, bool last
     bool done[3] = {};
     for (int i = 0; i < n; i++) {
         if (done[i]) continue;
-        const int dyw = y_width(r[i].dy), dzs = z_slice(p->type, r[i].dy, r[i].dz);
+        const int dyw = y_width(r[i].dy), dzs = z_slice(p->type, r[i].dz);
         WalkArgs a = {};
         for (int j = i; j < n; j++) {
-            if (done[j] || y_width(r[j].dy) != dyw || z_slice(p->type, r[j].dy, r[j].dz) != dzs) continue;
+            if (done[j] || y_width(r[j].dy) != dyw || z_slice(p->type, r[j].dz) != dzs) continue;
             done[j] = true;
             r[j].slice0 = a.parts;
             a.parts += (r[j].dz + dzs - 1) / dzs;
@@ -968,7 +974,7 @@ void enter_segments(Role& r, const float* scratch, const hum_decay_attn_args* p,
     r.in_seg = (long)p->dk * p->dv;
 }
 int parts_of(const hum_decay_attn_args* p, int dy, int dz) {
-    const int s = z_slice(p->type, dy, dz);
+    const int s = z_slice(p->type, dz);
     return (dz + s - 1) / s;
 }
 Cut forward_cut(const hum_decay_attn_args* p) { return cut_of(p, parts_of(p, p->dk, p->dv)); }
