@@ -29,36 +29,51 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 
 template <int ST> struct El;
-template <> struct El<HUM_F32> { typedef float T; };
-template <> struct El<HUM_BF16> { typedef __bf16 T; typedef bf16x8 V; };
-template <> struct El<HUM_F16> { typedef _Float16 T; typedef f16x8 V; };
+template <> struct El<HUM_F32> { typedef float T; static constexpr int SIZE = 4; };
+template <> struct El<HUM_BF16> { typedef __bf16 T; typedef bf16x8 V; static constexpr int SIZE = 2; };
+template <> struct El<HUM_F16> { typedef _Float16 T; typedef f16x8 V; static constexpr int SIZE = 2; };
+
+// buffer accesses: a wave's base in scalar registers, a 32-bit byte offset per lane; what lies beyond reads as zero and is
+// not written, so a masked lane takes an offset outside instead of a branch (which would make the loads wait for each other)
+typedef __amdgpu_buffer_rsrc_t Buf;
+constexpr int OUTSIDE = (int)0x80000000;
+__device__ __forceinline__ Buf buffer(const void* p, long bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc((char*)const_cast<void*>(p) + (p ? bytes : 0), 0, p ? 0x7fffffff : 0, 0x00020000);
+}
+__device__ __forceinline__ int beyond(int a, int b) { return ~((a - b) >> 31) & OUTSIDE; }   // bit 31 where a >= b
 
 template <int ST>
-__device__ __forceinline__ f32x8 load8(const void* p, long at) {
-    const typename El<ST>::T* e = (const typename El<ST>::T*)p + at;
+__device__ __forceinline__ f32x8 load8(Buf b, int at) {
+    const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(b, at, 0, 0);
     if constexpr (ST == HUM_F32) {
-        const f32x4 a = *(const f32x4*)e, b = *(const f32x4*)(e + 4);
-        return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+        const u32x4 w = __builtin_amdgcn_raw_buffer_load_b128(b, at + 16, 0, 0);
+        return __builtin_shufflevector(__builtin_bit_cast(f32x4, v), __builtin_bit_cast(f32x4, w), 0, 1, 2, 3, 4, 5, 6, 7);
     } else {
-        return __builtin_convertvector(*(const typename El<ST>::V*)e, f32x8);
+        return __builtin_convertvector(__builtin_bit_cast(typename El<ST>::V, v), f32x8);
     }
 }
 template <int ST>
-__device__ __forceinline__ void store8(void* p, long at, f32x8 v) {
-    typename El<ST>::T* e = (typename El<ST>::T*)p + at;
+__device__ __forceinline__ void store8(Buf b, int at, f32x8 v) {
     if constexpr (ST == HUM_F32) {
-        *(f32x4*)e = __builtin_shufflevector(v, v, 0, 1, 2, 3);
-        *(f32x4*)(e + 4) = __builtin_shufflevector(v, v, 4, 5, 6, 7);
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, __builtin_shufflevector(v, v, 0, 1, 2, 3)), b, at, 0, 0);
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, __builtin_shufflevector(v, v, 4, 5, 6, 7)), b, at + 16, 0, 0);
     } else {
-        *(typename El<ST>::V*)e = __builtin_convertvector(v, typename El<ST>::V);
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, __builtin_convertvector(v, typename El<ST>::V)), b, at, 0, 0);
     }
 }
 template <int ST>
-__device__ __forceinline__ float load1(const void* p, long at) { return (float)((const typename El<ST>::T*)p)[at]; }
+__device__ __forceinline__ float load1(Buf b, int at) {
+    if constexpr (ST == HUM_F32) return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(b, at, 0, 0));
+    else return (float)__builtin_bit_cast(typename El<ST>::T, (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(b, at, 0, 0));
+}
 template <int ST>
-__device__ __forceinline__ void store1(void* p, long at, float v) { ((typename El<ST>::T*)p)[at] = (typename El<ST>::T)v; }
+__device__ __forceinline__ void store1(Buf b, int at, float v) {
+    if constexpr (ST == HUM_F32) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, v), b, at, 0, 0);
+    else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, (typename El<ST>::T)v), b, at, 0, 0);
+}
 
 // channel of a thread's element i: VEC takes 8 neighbours at a time (16-byte loads), else neighbouring threads take
 // neighbouring channels
@@ -66,28 +81,27 @@ template <int TPR, bool VEC>
 __device__ __forceinline__ int channel(int j, int i) {
     return VEC ? 8 * ((i / 8) * TPR + j) + i % 8 : i * TPR + j;
 }
-// a thread's 8 NV channels of a row, zeros behind c
+// a thread's 8 NV channels of a row at byte offset `at` of the buffer (bit 31: no row), zeros behind c
 template <int ST, int TPR, int NV, bool VEC>
-__device__ __forceinline__ void load_row(const void* p, long at, int j, int c, float (&v)[8 * NV]) {
+__device__ __forceinline__ void load_row(Buf b, int at, int j, int c, float (&v)[8 * NV]) {
 #pragma unroll
     for (int n = 0; n < NV; n++) {
         if constexpr (VEC) {
             const int e = channel<TPR, true>(j, 8 * n);
-            f32x8 t = {};
-            if (e < c) t = load8<ST>(p, at + e);
+            const f32x8 t = load8<ST>(b, (at + e * El<ST>::SIZE) | beyond(e, c));
 #pragma unroll
             for (int i = 0; i < 8; i++) v[8 * n + i] = t[i];
         } else {
 #pragma unroll
             for (int i = 8 * n; i < 8 * n + 8; i++) {
                 const int e = channel<TPR, false>(j, i);
-                v[i] = e < c ? load1<ST>(p, at + e) : 0.f;
+                v[i] = load1<ST>(b, (at + e * El<ST>::SIZE) | beyond(e, c));
             }
         }
     }
 }
 template <int ST, int TPR, int NV, bool VEC>
-__device__ __forceinline__ void store_row(void* p, long at, int j, int c, const float (&v)[8 * NV]) {
+__device__ __forceinline__ void store_row(Buf b, int at, int j, int c, const float (&v)[8 * NV]) {
 #pragma unroll
     for (int n = 0; n < NV; n++) {
         if constexpr (VEC) {
@@ -95,12 +109,12 @@ __device__ __forceinline__ void store_row(void* p, long at, int j, int c, const 
             f32x8 t;
 #pragma unroll
             for (int i = 0; i < 8; i++) t[i] = v[8 * n + i];
-            if (e < c) store8<ST>(p, at + e, t);
+            store8<ST>(b, (at + e * El<ST>::SIZE) | beyond(e, c), t);
         } else {
 #pragma unroll
             for (int i = 8 * n; i < 8 * n + 8; i++) {
                 const int e = channel<TPR, false>(j, i);
-                if (e < c) store1<ST>(p, at + e, v[i]);
+                store1<ST>(b, (at + e * El<ST>::SIZE) | beyond(e, c), v[i]);
             }
         }
     }
@@ -112,11 +126,26 @@ __device__ __forceinline__ void load_param(const void* p, bool wide, int j, int 
 #pragma unroll
         for (int i = 0; i < 8 * NV; i++) v[i] = none;
     } else if (wide) {
-        load_row<HUM_F32, TPR, NV, VEC>(p, 0, j, c, v);
+        load_row<HUM_F32, TPR, NV, VEC>(buffer(p, 0), 0, j, c, v);
     } else {
-        load_row<ST, TPR, NV, VEC>(p, 0, j, c, v);
+        load_row<ST, TPR, NV, VEC>(buffer(p, 0), 0, j, c, v);
     }
 }
+// where the rows of a wave begin: its first row is uniform, a lane's is `below` further (several rows a wave if TPR < 64)
+template <int TPR>
+struct Place {
+    long first;
+    int below;
+    bool in;
+    __device__ __forceinline__ Place(long row0, long rows) {
+        constexpr int PER = TPR < 64 ? 64 / TPR : 1;   // rows per wave
+        const int t = __builtin_amdgcn_readfirstlane(threadIdx.x & ~63);
+        first = row0 + t / TPR;
+        below = PER > 1 ? (threadIdx.x & 63) / TPR : 0;
+        in = first + below < rows;
+    }
+    __device__ __forceinline__ int at(long pitch, int size) const { return in ? below * (int)(pitch * size) : OUTSIDE; }
+};
 
 // the sum over a row's TPR threads, the same bits in every one of them
 template <int TPR>
@@ -159,10 +188,9 @@ __global__ void __launch_bounds__(TPR > THREADS ? TPR : THREADS) norm_kernel(Nor
     load_param<ST, TPR, NV, VEC>(a.b, a.wide, j, a.c, 0.f, b);
     // every thread of a workgroup makes the same number of turns (row_sum may hold a barrier)
     for (long row0 = (long)blockIdx.x * GROUPS; row0 < a.rows; row0 += (long)gridDim.x * GROUPS) {
-        const long row = row0 + threadIdx.x / TPR;
-        const bool in = row < a.rows;
+        const Place<TPR> row(row0, a.rows);
         float x[8 * NV];
-        load_row<ST, TPR, NV, VEC>(a.x, row * a.x_row, j, in ? a.c : 0, x);
+        load_row<ST, TPR, NV, VEC>(buffer(a.x, row.first * a.x_row * El<ST>::SIZE), row.at(a.x_row, El<ST>::SIZE), j, a.c, x);
         float s = 0.f;
 #pragma unroll
         for (int i = 0; i < 8 * NV; i++) s += x[i];
@@ -176,12 +204,10 @@ __global__ void __launch_bounds__(TPR > THREADS ? TPR : THREADS) norm_kernel(Nor
         const float rstd = 1.f / sqrtf(row_sum<TPR>(s, scratch) * inv + a.eps);
 #pragma unroll
         for (int i = 0; i < 8 * NV; i++) x[i] = x[i] * rstd * w[i] + b[i];
-        if (in) {
-            store_row<ST, TPR, NV, VEC>(a.y, row * a.y_row, j, a.c, x);
-            if (j == 0 && a.mean) {
-                a.mean[row] = mean;
-                a.rstd[row] = rstd;
-            }
+        store_row<ST, TPR, NV, VEC>(buffer(a.y, row.first * a.y_row * El<ST>::SIZE), row.at(a.y_row, El<ST>::SIZE), j, a.c, x);
+        if (j == 0 && a.mean && row.in) {
+            a.mean[row.first + row.below] = mean;
+            a.rstd[row.first + row.below] = rstd;
         }
     }
 }
@@ -207,12 +233,11 @@ __global__ void __launch_bounds__(TPR > THREADS ? TPR : THREADS) grad_kernel(Gra
 #pragma unroll
     for (int i = 0; i < 8 * NV; i++) dw[i] = db[i] = 0.f;
     for (long row0 = (long)blockIdx.x * GROUPS; row0 < a.rows; row0 += (long)gridDim.x * GROUPS) {
-        const long row = row0 + grp;
-        const bool in = row < a.rows;
+        const Place<TPR> row(row0, a.rows);
         float x[8 * NV], d[8 * NV];
-        load_row<ST, TPR, NV, VEC>(a.x, row * a.x_row, j, in ? a.c : 0, x);
-        load_row<ST, TPR, NV, VEC>(a.dy, row * a.dy_row, j, in ? a.c : 0, d);
-        const float mean = in ? a.mean[row] : 0.f, rstd = in ? a.rstd[row] : 0.f;
+        load_row<ST, TPR, NV, VEC>(buffer(a.x, row.first * a.x_row * El<ST>::SIZE), row.at(a.x_row, El<ST>::SIZE), j, a.c, x);
+        load_row<ST, TPR, NV, VEC>(buffer(a.dy, row.first * a.dy_row * El<ST>::SIZE), row.at(a.dy_row, El<ST>::SIZE), j, a.c, d);
+        const float mean = load1<HUM_F32>(buffer(a.mean, row.first * 4), row.at(1, 4)), rstd = load1<HUM_F32>(buffer(a.rstd, row.first * 4), row.at(1, 4));
         float s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int i = 0; i < 8 * NV; i++) {
@@ -228,7 +253,7 @@ __global__ void __launch_bounds__(TPR > THREADS ? TPR : THREADS) grad_kernel(Gra
             s2 = row_sum<TPR>(s2, scratch) * inv;
 #pragma unroll
             for (int i = 0; i < 8 * NV; i++) d[i] = rstd * (d[i] - s1 - x[i] * s2);
-            if (in) store_row<ST, TPR, NV, VEC>(a.dx, row * a.dx_row, j, a.c, d);
+            store_row<ST, TPR, NV, VEC>(buffer(a.dx, row.first * a.dx_row * El<ST>::SIZE), row.at(a.dx_row, El<ST>::SIZE), j, a.c, d);
         }
     }
     if (!a.part) return;
@@ -263,25 +288,27 @@ __global__ void __launch_bounds__(TPR > THREADS ? TPR : THREADS) grad_kernel(Gra
     }
 }
 
-// dw, db from the workgroups' partial rows: 16 columns x 16 strided partial sums per workgroup, joined in order
+// dw, db from the workgroups' partial rows: 16 columns x 64 strided partial sums per workgroup, joined in order
 template <int ST>
-__global__ void __launch_bounds__(256) param_kernel(const float* part, int blocks, int c, void* dw, void* db, int wide) {
-    __shared__ double sums[256];
+__global__ void __launch_bounds__(1024) param_kernel(const float* part, int blocks, int c, void* dw, void* db, int wide) {
+    __shared__ double sums[1024];
     const int col = blockIdx.x * 16 + threadIdx.x % 16, k = threadIdx.x / 16;
     double s = 0.;
-    if (col < 2 * c)
-        for (int i = k; i < blocks; i += 16) s += (double)part[(long)i * 2 * c + col];
+    if (col < 2 * c) {
+#pragma unroll 8
+        for (int i = k; i < blocks; i += 64) s += (double)part[(long)i * 2 * c + col];
+    }
     sums[threadIdx.x] = s;
     __syncthreads();
     if (k || col >= 2 * c) return;
     s = 0.;
-#pragma unroll
-    for (int i = 0; i < 16; i++) s += sums[i * 16 + threadIdx.x];
+#pragma unroll 8
+    for (int i = 0; i < 64; i++) s += sums[i * 16 + threadIdx.x];
     void* o = col < c ? dw : db;
     if (!o) return;
     const int e = col < c ? col : col - c;
     if (wide) ((float*)o)[e] = (float)s;
-    else store1<ST>(o, e, (float)s);
+    else ((typename El<ST>::T*)o)[e] = (typename El<ST>::T)(float)s;
 }
 
 int nerr(int code, const char* fn, const char* m) {
@@ -303,12 +330,13 @@ struct OnDevice {   // the caller's current device stays what it was
 
 // threads per row: 8 channels a thread as long as a wave holds the row, then more channels, then a whole workgroup
 struct Shape { int tpr, nv; };
-Shape shape_of(int c) {
-    if (c <= 64) return {8, 1};
-    if (c <= 128) return {16, 1};
-    if (c <= 256) return {32, 1};
+Shape shape_of(int c, bool near) {   // near: a wave's rows lie within 2^31 bytes
+    if (c <= 64 && near) return {8, 1};
+    if (c <= 128 && near) return {16, 1};
+    if (c <= 256 && near) return {32, 1};
     if (c <= 512) return {64, 1};
     if (c <= 1024) return {64, 2};
+    if (c <= 1536) return {64, 3};
     if (c <= 2048) return {256, 1};
     if (c <= 4096) return {256, 2};
     if (c <= 8192) return {1024, 1};
@@ -339,7 +367,8 @@ void launch_norm_s(const A& a, Shape sh, bool vec, long blocks, hipStream_t s) {
     else if (sh.tpr == 16) launch_norm_v<ST, 16, 1>(a, vec, blocks, s);
     else if (sh.tpr == 32) launch_norm_v<ST, 32, 1>(a, vec, blocks, s);
     else if (sh.tpr == 64 && sh.nv == 1) launch_norm_v<ST, 64, 1>(a, vec, blocks, s);
-    else if (sh.tpr == 64) launch_norm_v<ST, 64, 2>(a, vec, blocks, s);
+    else if (sh.tpr == 64 && sh.nv == 2) launch_norm_v<ST, 64, 2>(a, vec, blocks, s);
+    else if (sh.tpr == 64) launch_norm_v<ST, 64, 3>(a, vec, blocks, s);
     else if (sh.tpr == 256 && sh.nv == 1) launch_norm_v<ST, 256, 1>(a, vec, blocks, s);
     else if (sh.tpr == 256) launch_norm_v<ST, 256, 2>(a, vec, blocks, s);
     else if (sh.nv == 1) launch_norm_v<ST, 1024, 1>(a, vec, blocks, s);
@@ -362,6 +391,8 @@ int check_sizes(const char* fn, const hum_norm_args* p) {
     if ((uintptr_t)p->x % es || (uintptr_t)p->weight % ps) return nerr(HUM_ERR_ARG, fn, "rows and parameters must be aligned to their elements");
     return HUM_OK;
 }
+// rows of 8 lanes to a wave at most
+bool near(int64_t row, int size) { return row >= 0 && row < (1l << 28) / size; }
 bool aligned(const void* p, int64_t row, int size) { return ((uintptr_t)p | (uintptr_t)(row * size)) % 16 == 0; }
 
 int launched(const char* fn) {
@@ -386,7 +417,7 @@ int hum_layer_norm(const hum_norm_args* p, const void* bias, float eps, void* y,
     const OnDevice dev(p->device);
     if (!dev.ok) return nerr(HUM_ERR_HIP, fn, "hipSetDevice");
     NormArgs a = {p->x, p->weight, bias, y, mean, rstd, (long)p->rows, (long)p->x_row, (long)y_row, p->channels, p->param_type == HUM_F32, eps};
-    const Shape sh = shape_of(p->channels);
+    const Shape sh = shape_of(p->channels, near(p->x_row, es) && near(y_row, es));
     const bool vec = p->channels % 8 == 0 && aligned(p->x, p->x_row, es) && aligned(y, y_row, es) && ((uintptr_t)p->weight | (uintptr_t)bias) % 16 == 0;
     const long g = groups_of(sh), blocks = (p->rows + g - 1) / g;
     launch_norm(p->type, a, sh, vec, blocks < 16384 ? blocks : 16384, (hipStream_t)stream);
@@ -397,7 +428,8 @@ int hum_layer_norm_workspace(const hum_norm_args* p, uint64_t* bytes) {
     const char* fn = "hum_layer_norm_workspace";
     if (const int rc = check_sizes(fn, p)) return rc;
     if (!bytes) return nerr(HUM_ERR_ARG, fn, "null argument");
-    *bytes = (uint64_t)grad_blocks(p->rows, shape_of(p->channels)) * 2 * p->channels * sizeof(float);
+    const uint64_t a = grad_blocks(p->rows, shape_of(p->channels, true)), b = grad_blocks(p->rows, shape_of(p->channels, false));
+    *bytes = (a > b ? a : b) * 2 * p->channels * sizeof(float);
     return HUM_OK;
 }
 
@@ -410,7 +442,7 @@ int hum_layer_norm_backward(const hum_norm_args* p, const void* dy, int64_t dy_r
     if (p->rows && (!dy || !mean || !rstd)) return nerr(HUM_ERR_ARG, fn, "dy, mean and rstd are required");
     if (((uintptr_t)dy | (uintptr_t)dx) % es || ((uintptr_t)d_weight | (uintptr_t)d_bias) % ps || ((uintptr_t)mean | (uintptr_t)rstd) % 4)
         return nerr(HUM_ERR_ARG, fn, "rows, statistics and parameters must be aligned to their elements");
-    const Shape sh = shape_of(p->channels);
+    const Shape sh = shape_of(p->channels, near(p->x_row, es) && near(dy_row, es) && near(dx_row, es));
     const bool params = d_weight || d_bias;
     uint64_t need = 0;
     if (params)
@@ -426,9 +458,9 @@ int hum_layer_norm_backward(const hum_norm_args* p, const void* dy, int64_t dy_r
     launch_norm(p->type, a, sh, vec, blocks, (hipStream_t)stream);
     if (params) {
         const dim3 grid((2 * p->channels + 15) / 16);
-        if (p->type == HUM_F32) hipLaunchKernelGGL(param_kernel<HUM_F32>, grid, dim3(256), 0, (hipStream_t)stream, a.part, (int)blocks, p->channels, d_weight, d_bias, a.wide);
-        else if (p->type == HUM_BF16) hipLaunchKernelGGL(param_kernel<HUM_BF16>, grid, dim3(256), 0, (hipStream_t)stream, a.part, (int)blocks, p->channels, d_weight, d_bias, a.wide);
-        else hipLaunchKernelGGL(param_kernel<HUM_F16>, grid, dim3(256), 0, (hipStream_t)stream, a.part, (int)blocks, p->channels, d_weight, d_bias, a.wide);
+        if (p->type == HUM_F32) hipLaunchKernelGGL(param_kernel<HUM_F32>, grid, dim3(1024), 0, (hipStream_t)stream, a.part, (int)blocks, p->channels, d_weight, d_bias, a.wide);
+        else if (p->type == HUM_BF16) hipLaunchKernelGGL(param_kernel<HUM_BF16>, grid, dim3(1024), 0, (hipStream_t)stream, a.part, (int)blocks, p->channels, d_weight, d_bias, a.wide);
+        else hipLaunchKernelGGL(param_kernel<HUM_F16>, grid, dim3(1024), 0, (hipStream_t)stream, a.part, (int)blocks, p->channels, d_weight, d_bias, a.wide);
     }
     return launched(fn);
 }

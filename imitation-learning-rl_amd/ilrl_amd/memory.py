@@ -17,26 +17,59 @@ x.transpose(0, 1), no copy.  float32, bfloat16 and float16; 1 to 128 channels a 
 equal groups of query heads.  There is no CPU path.
 """
 import ctypes
+import struct
 
 from . import _native as N
 
 MAX_HEAD_CHANNELS, MAX_NORM_CHANNELS = 128, 16384
 
+# The argument structures as packed bytes (hum_decay_attn_args, hum_rows, hum_norm_args): building them field by field with
+# ctypes took longer than a single step's kernel
+_ATTN = struct.Struct("=8if4xQ" + "Qqqq" * 3 + "QQQqqQ")
+_ROWS = struct.Struct("=Qqqq")
+_NORM = struct.Struct("=4i2q2Q")
 
-def _torch():
-    import torch
-    return torch
+_entry = None
 
 
-_TYPES = None
+class _Entry:
+    """torch and the entry points, found once (torch is only imported when an operator is called)."""
+
+    def __init__(self):
+        import torch
+        self.t = torch
+        self.types = {torch.float32: N.HUM_F32, torch.bfloat16: N.HUM_BF16, torch.float16: N.HUM_F16}
+        self.marks = (torch.uint8, torch.bool)
+        L, c = N.lib(), ctypes
+        b, vp, i32, i64, u64, f32 = c.c_char_p, c.c_void_p, c.c_int32, c.c_int64, c.c_uint64, c.c_float
+        need = c.POINTER(u64)
+
+        def bind(name, *args):
+            return c.CFUNCTYPE(c.c_int, *args)((name, L))
+        self.workspace = bind("hum_decay_attn_workspace", b, i32, need)
+        self.attn = bind("hum_decay_attn", b, b, vp, u64, vp)
+        self.attn_backward = bind("hum_decay_attn_backward", b, b, vp, b, b, b, vp, vp, u64, vp)
+        self.step = bind("hum_decay_attn_step", b, vp, b, vp)
+        self.norm = bind("hum_layer_norm", b, vp, f32, vp, i64, vp, vp, vp)
+        self.norm_workspace = bind("hum_layer_norm_workspace", b, need)
+        self.norm_backward = bind("hum_layer_norm_backward", b, vp, i64, vp, vp, vp, i64, vp, vp, vp, u64, vp)
+        self.raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+    def stream(self, index):
+        if self.raw_stream is not None:
+            return self.raw_stream(index)
+        return self.t.cuda.current_stream(index).cuda_stream
 
 
-def _type(x, what):
-    global _TYPES
-    if _TYPES is None:
-        t = _torch()
-        _TYPES = {t.float32: N.HUM_F32, t.bfloat16: N.HUM_BF16, t.float16: N.HUM_F16}
-    code = _TYPES.get(x.dtype)
+def _e():
+    global _entry
+    if _entry is None:
+        _entry = _Entry()
+    return _entry
+
+
+def _type(e, x, what):
+    code = e.types.get(x.dtype)
     if code is None:
         raise ValueError("%s: float32, bfloat16 or float16, got %s" % (what, x.dtype))
     return code
@@ -46,22 +79,19 @@ def _p(x):
     return x.data_ptr() if x is not None else None
 
 
-def _stream(device):
-    return _torch().cuda.current_stream(device).cuda_stream
-
-
 def _unit(x):
     """x with adjacent channels."""
     return x if x.stride(-1) == 1 or x.shape[-1] <= 1 else x.contiguous()
 
 
 def _rows(x):
-    return N.HumRows(x.data_ptr(), x.stride(0), x.stride(1), x.stride(2))
+    s = x.stride()
+    return _ROWS.pack(x.data_ptr(), s[0], s[1], s[2])
 
 
 def _same_order(like, shape):
     """An empty [lanes, steps, ...] tensor in `like`'s memory order (time-major where its steps are the outer axis)."""
-    t = _torch()
+    t = _e().t
     if like.stride(0) < like.stride(1):
         return t.empty((shape[1], shape[0]) + shape[2:], dtype=like.dtype, device=like.device).transpose(0, 1)
     return t.empty(shape, dtype=like.dtype, device=like.device)
@@ -70,70 +100,74 @@ def _same_order(like, shape):
 def _on(x, device, what, shape=None, dtypes=None):
     if x.device != device:
         raise ValueError("%s is on %s, expected %s" % (what, x.device, device))
-    if shape is not None and tuple(x.shape) != shape:
+    if shape is not None and x.shape != shape:
         raise ValueError("%s must be %s, got %s" % (what, list(shape), list(x.shape)))
     if dtypes is not None and x.dtype not in dtypes:
         raise ValueError("%s must be of type %s, got %s" % (what, " or ".join(str(d) for d in dtypes), x.dtype))
     return x
 
 
-def _check(q, k, v, log_decay, state, reset, lengths):
-    """The operands of a fragment as (q, k, v with adjacent channels, HumDecayAttnArgs); [lanes, steps, ...]."""
-    t = _torch()
-    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
-        raise ValueError("q, k, v must be [lanes, steps, heads, channels], got %s, %s, %s"
-                         % (list(q.shape), list(k.shape), list(v.shape)))
+def _check(e, q, k, v, log_decay, state, reset, lengths, axes):
+    """The checks fragments (axes 4: [lanes, steps, heads, channels]) and single steps (axes 3) share; returns (q, k, v with
+    adjacent channels, log_decay, lengths, the sizes (lanes, steps, heads, kv_heads, dk, dv))."""
+    t, f32 = e.t, e.t.float32
+    qs, ks, vs = q.shape, k.shape, v.shape
+    if len(qs) != axes or len(ks) != axes or len(vs) != axes:
+        raise ValueError("q, k, v must be [lanes, %sheads, channels], got %s, %s, %s"
+                         % ("steps, " if axes == 4 else "", list(qs), list(ks), list(vs)))
     if not q.is_cuda:
         raise ValueError("q must be on a GPU (there is no CPU path)")
-    b, s, h, dk = q.shape
-    g, dv = k.shape[2], v.shape[3]
-    _on(k, q.device, "k", (b, s, g, dk), (q.dtype,))
-    _on(v, q.device, "v", (b, s, g, dv), (q.dtype,))
+    dev, dt = q.device, q.dtype
+    lead, h, dk = qs[:-2], qs[-2], qs[-1]
+    g, dv = ks[-2], vs[-1]
+    _on(k, dev, "k", lead + (g, dk), (dt,))
+    _on(v, dev, "v", lead + (g, dv), (dt,))
     if g < 1 or h % g:
         raise ValueError("%d key / value heads cannot be shared evenly by %d query heads" % (g, h))
     if not (1 <= dk <= MAX_HEAD_CHANNELS and 1 <= dv <= MAX_HEAD_CHANNELS):
         raise ValueError("1 to %d channels a head, got %d (keys) and %d (values)" % (MAX_HEAD_CHANNELS, dk, dv))
-    _on(log_decay, q.device, "log_decay", (h,), (t.float32,))
+    _on(log_decay, dev, "log_decay", (h,), (f32,))
     if log_decay.requires_grad:
         raise ValueError("log_decay is a constant schedule and has no gradient: pass log_decay.detach()")
     if not log_decay.is_contiguous():
         log_decay = log_decay.contiguous()
     if state is not None:
-        _on(state, q.device, "state", (b, h, dv, dk), (t.float32,))
+        _on(state, dev, "state", (lead[0], h, dv, dk), (f32,))
         if not state.is_contiguous():
             raise ValueError("state must be contiguous")
     if reset is not None:
-        _on(reset, q.device, "reset", (b, s), (t.uint8, t.bool))
+        _on(reset, dev, "reset", lead, e.marks)
     if lengths is not None:
-        _on(lengths, q.device, "lengths", (b,), (t.int32,))
+        _on(lengths, dev, "lengths", lead[:1], (t.int32,))
         lengths = lengths.contiguous()
-    q, k, v = _unit(q), _unit(k), _unit(v)
-    a = N.HumDecayAttnArgs(q.device.index, _type(q, "q"), b, s, h, g, dk, dv, 0.0, log_decay.data_ptr(), _rows(q),
-                           _rows(k), _rows(v), _p(state), None, _p(reset), 0, 0, _p(lengths))
-    if reset is not None:
-        a.reset_lane, a.reset_step = reset.stride(0), reset.stride(1)
-    return q, k, v, log_decay, lengths, a
+    return _unit(q), _unit(k), _unit(v), log_decay, lengths, (lead[0], lead[1] if axes == 4 else 1, h, g, dk, dv)
 
 
-def _scratch(a, backward, device):
+def _attn(e, q, k, v, log_decay, state, state_out, reset, lengths, scale, sizes):
+    """hum_decay_attn_args of a fragment."""
+    sq, sk, sv = q.stride(), k.stride(), v.stride()
+    sr = reset.stride() if reset is not None else (0, 0)
+    return _ATTN.pack(q.get_device(), _type(e, q, "q"), *sizes, sizes[4] ** -0.5 if scale is None else float(scale),
+                      log_decay.data_ptr(), q.data_ptr(), sq[0], sq[1], sq[2], k.data_ptr(), sk[0], sk[1], sk[2],
+                      v.data_ptr(), sv[0], sv[1], sv[2], _p(state) or 0, _p(state_out) or 0, _p(reset) or 0, sr[0], sr[1],
+                      _p(lengths) or 0)
+
+
+def _scratch(e, a, backward, device):
     need = ctypes.c_uint64(0)
-    N.check(N.lib().hum_decay_attn_workspace(ctypes.byref(a), backward, ctypes.byref(need)), "hum_decay_attn_workspace")
-    if not need.value:
-        return None
-    t = _torch()
-    return t.empty(need.value, dtype=t.uint8, device=device)
+    N.check(e.workspace(a, backward, ctypes.byref(need)), "hum_decay_attn_workspace")
+    return e.t.empty(need.value, dtype=e.t.uint8, device=device) if need.value else None
 
 
 def _forward(q, k, v, log_decay, state, reset, lengths, scale):
-    t = _torch()
-    q, k, v, log_decay, lengths, a = _check(q, k, v, log_decay, state, reset, lengths)
-    a.scale = q.shape[3] ** -0.5 if scale is None else float(scale)
-    out = _same_order(q, tuple(q.shape[:3]) + (v.shape[3],))
-    state_out = t.empty(q.shape[0], q.shape[2], v.shape[3], q.shape[3], dtype=t.float32, device=q.device)
-    a.state_out = state_out.data_ptr()
-    ws = _scratch(a, 0, q.device)
-    N.check(N.lib().hum_decay_attn(ctypes.byref(a), ctypes.byref(_rows(out)), _p(ws), ws.numel() if ws is not None else 0,
-                                   _stream(q.device)), "hum_decay_attn")
+    e = _e()
+    q, k, v, log_decay, lengths, sizes = _check(e, q, k, v, log_decay, state, reset, lengths, 4)
+    n, s, h, _, dk, dv = sizes
+    out = _same_order(q, (n, s, h, dv))
+    state_out = e.t.empty(n, h, dv, dk, dtype=e.t.float32, device=q.device)
+    a = _attn(e, q, k, v, log_decay, state, state_out, reset, lengths, scale, sizes)
+    ws = _scratch(e, a, 0, q.device)
+    N.check(e.attn(a, _rows(out), _p(ws), ws.numel() if ws is not None else 0, e.stream(q.get_device())), "hum_decay_attn")
     return out, state_out
 
 
@@ -142,20 +176,19 @@ def decay_attention_backward(d_out, d_state, q, k, v, log_decay, state=None, res
     """(dq, dk, dv, d_state_in) of decay_attention for the gradients d_out [lanes, steps, heads, dv] of its output and
     d_state [lanes, heads, dv, dk] of its final state (None = zeros), from the same inputs.  needs: which of the four to
     compute (the others are None)."""
-    t = _torch()
-    q, k, v, log_decay, lengths, a = _check(q, k, v, log_decay, state, reset, lengths)
-    a.scale = q.shape[3] ** -0.5 if scale is None else float(scale)
-    d_out = _unit(_on(d_out, q.device, "d_out", tuple(q.shape[:3]) + (v.shape[3],), (q.dtype,)))
-    sshape = (q.shape[0], q.shape[2], v.shape[3], q.shape[3])
+    e = _e()
+    q, k, v, log_decay, lengths, sizes = _check(e, q, k, v, log_decay, state, reset, lengths, 4)
+    n, s, h, _, dk, dv = sizes
+    a = _attn(e, q, k, v, log_decay, state, None, reset, lengths, scale, sizes)
+    d_out = _unit(_on(d_out, q.device, "d_out", (n, s, h, dv), (q.dtype,)))
     if d_state is not None:
-        d_state = _on(d_state, q.device, "d_state", sshape, (t.float32,)).contiguous()
+        d_state = _on(d_state, q.device, "d_state", (n, h, dv, dk), (e.t.float32,)).contiguous()
     grads = [_same_order(x, tuple(x.shape)) if need else None for x, need in zip((q, k, v), needs)]
-    d_in = t.empty(sshape, dtype=t.float32, device=q.device) if needs[3] else None
-    ws = _scratch(a, 1, q.device)
-    rows = [ctypes.byref(_rows(x)) if x is not None else None for x in grads]
-    N.check(N.lib().hum_decay_attn_backward(ctypes.byref(a), ctypes.byref(_rows(d_out)), _p(d_state), *rows, _p(d_in),
-                                            _p(ws), ws.numel() if ws is not None else 0, _stream(q.device)),
-            "hum_decay_attn_backward")
+    d_in = e.t.empty(n, h, dv, dk, dtype=e.t.float32, device=q.device) if needs[3] else None
+    ws = _scratch(e, a, 1, q.device)
+    rows = [_rows(x) if x is not None else None for x in grads]
+    N.check(e.attn_backward(a, _rows(d_out), _p(d_state), *rows, _p(d_in), _p(ws), ws.numel() if ws is not None else 0,
+                            e.stream(q.get_device())), "hum_decay_attn_backward")
     return grads[0], grads[1], grads[2], d_in
 
 
@@ -167,7 +200,7 @@ def _autograd():
     global _functions
     if _functions is not None:
         return _functions
-    t = _torch()
+    t = _e().t
     once = t.autograd.function.once_differentiable
 
     class DecayAttention(t.autograd.Function):
@@ -221,7 +254,7 @@ def decay_attention(q, k, v, log_decay, state=None, reset=None, lengths=None, sc
     whatever came before is not seen from there on, also where it is not finite.  lengths [lanes] int32: steps behind a
     lane's length are not read and give zeros; the final state is the one after the last step held.  scale: default
     dk ** -0.5.  Differentiable in q, k, v and state."""
-    t = _torch()
+    t = _e().t
     if t.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
                                 or (state is not None and state.requires_grad)):
         if log_decay.requires_grad:
@@ -236,77 +269,75 @@ def decay_attention_step(q, k, v, log_decay, state, reset=None, active=None, sca
     itself.  reset [lanes] uint8 or bool: this step starts an episode; active [lanes] uint8 or bool: lanes that step
     (None = all), the others keep their state and give zeros.  Not differentiable (the learner's pass over the recorded
     fragment is): inputs that require a gradient are refused while gradients are recorded."""
-    t = _torch()
-    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
-        raise ValueError("q, k, v must be [lanes, heads, channels], got %s, %s, %s" % (list(q.shape), list(k.shape), list(v.shape)))
-    if t.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, v, state)):
+    e = _e()
+    t = e.t
+    if t.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (state is not None and state.requires_grad)):
         raise ValueError("decay_attention_step is not differentiable: use decay_attention, or torch.no_grad()")
-    n = q.shape[0]
-    if reset is not None and reset.dim() != 1:
-        raise ValueError("reset must be [%d], got %s" % (n, list(reset.shape)))
     if state is None:
         raise ValueError("state is required (PolicyMemory.begin, or zeros)")
-    q4, k4, v4, log_decay, _, a = _check(q[:, None], k[:, None], v[:, None], log_decay, state,
-                                         reset[:, None] if reset is not None else None, None)
-    a.scale = q.shape[2] ** -0.5 if scale is None else float(scale)
+    q, k, v, log_decay, _, sizes = _check(e, q, k, v, log_decay, state, reset, None, 3)
+    dev, n = q.device, sizes[0]
     if active is not None:
-        active = _on(active, q.device, "active", (n,), (t.uint8, t.bool)).contiguous()
+        active = _on(active, dev, "active", (n,), e.marks).contiguous()
     if state_out is None:
         state_out = state
     elif state_out is not state:
-        _on(state_out, q.device, "state_out", tuple(state.shape), (t.float32,))
+        _on(state_out, dev, "state_out", state.shape, (t.float32,))
         if not state_out.is_contiguous():
             raise ValueError("state_out must be contiguous")
-    a.state_out = state_out.data_ptr()
-    shape = (n, q.shape[1], v.shape[2])
+    shape = (n, sizes[2], sizes[5])
     if out is None:
-        out = t.empty(shape, dtype=q.dtype, device=q.device)
-    elif _unit(_on(out, q.device, "out", shape, (q.dtype,))) is not out:
+        out = t.empty(shape, dtype=q.dtype, device=dev)
+    elif _unit(_on(out, dev, "out", shape, (q.dtype,))) is not out:
         raise ValueError("out must have adjacent channels")
-    N.check(N.lib().hum_decay_attn_step(ctypes.byref(a), _p(active),
-                                        ctypes.byref(N.HumRows(out.data_ptr(), out.stride(0), 0, out.stride(1))),
-                                        _stream(q.device)), "hum_decay_attn_step")
+    sq, sk, sv, so, index = q.stride(), k.stride(), v.stride(), out.stride(), q.get_device()
+    a = _ATTN.pack(index, _type(e, q, "q"), *sizes, sizes[4] ** -0.5 if scale is None else float(scale), log_decay.data_ptr(),
+                   q.data_ptr(), sq[0], 0, sq[1], k.data_ptr(), sk[0], 0, sk[1], v.data_ptr(), sv[0], 0, sv[1],
+                   state.data_ptr(), state_out.data_ptr(), reset.data_ptr() if reset is not None else 0,
+                   reset.stride(0) if reset is not None else 0, 0, 0)
+    N.check(e.step(a, active.data_ptr() if active is not None else None, _ROWS.pack(out.data_ptr(), so[0], 0, so[1]),
+                   e.stream(index)), "hum_decay_attn_step")
     return out
 
 
 # ---------------------------------------------------------------------------------------------- layer norm
-def _norm_args(x, weight, param_dtype):
-    t = _torch()
+def _norm_args(e, x, weight, bias, param_dtype):
+    """(x as rows with adjacent channels, weight, bias, hum_norm_args)."""
     if not x.is_cuda:
         raise ValueError("x must be on a GPU (there is no CPU path)")
-    if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_NORM_CHANNELS:
+    c = x.shape[-1] if x.dim() else 0
+    if not 1 <= c <= MAX_NORM_CHANNELS:
         raise ValueError("layer norm takes 1 to %d channels, got %s" % (MAX_NORM_CHANNELS, list(x.shape)))
-    c = x.shape[-1]
-    x2 = _unit(x.reshape(-1, c))
+    code = _type(e, x, "x")
+    x2 = _unit(x if x.dim() == 2 else x.reshape(-1, c))
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise ValueError("weight and bias must have one type, got %s and %s" % (weight.dtype, bias.dtype))
     if weight is not None:
-        _on(weight, x.device, "weight", (c,), (t.float32, x.dtype))
-        weight = weight.contiguous()
-    a = N.HumNormArgs(x.device.index, _type(x, "x"), N.HUM_F32 if param_dtype == t.float32 else _type(x, "x"), c, x2.shape[0],
-                      x2.stride(0), x2.data_ptr(), _p(weight))
-    return x2, weight, a
+        weight = _on(weight, x.device, "weight", (c,), (e.t.float32, x.dtype)).contiguous()
+    if bias is not None:
+        bias = _on(bias, x.device, "bias", (c,), (e.t.float32, x.dtype)).contiguous()
+    a = _NORM.pack(x2.get_device(), code, N.HUM_F32 if param_dtype == e.t.float32 else code, c, x2.shape[0], x2.stride(0),
+                   x2.data_ptr(), weight.data_ptr() if weight is not None else 0)
+    return x2, weight, bias, a
 
 
 def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, out=None, stats=True):
     """(y, mean, rstd): layer_norm without autograd and what its backward pass needs (mean, rstd [rows] float32, None
     without stats)."""
-    t = _torch()
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise ValueError("weight and bias must have one type, got %s and %s" % (weight.dtype, bias.dtype))
+    e = _e()
+    t, dev = e.t, x.device
     p = weight if weight is not None else bias
-    x2, weight, a = _norm_args(x, weight, p.dtype if p is not None else t.float32)
-    if bias is not None:
-        bias = _on(bias, x.device, "bias", (x.shape[-1],), (t.float32, x.dtype)).contiguous()
+    x2, weight, bias, a = _norm_args(e, x, weight, bias, p.dtype if p is not None else t.float32)
     if out is None:
-        out = t.empty(x.shape, dtype=x.dtype, device=x.device)
+        out = t.empty(x.shape, dtype=x.dtype, device=dev)
     else:
-        _on(out, x.device, "out", tuple(x.shape), (x.dtype,))
+        _on(out, dev, "out", x.shape, (x.dtype,))
         if not out.is_contiguous():
             raise ValueError("out must be contiguous")
     rows, c = x2.shape
-    mean = t.empty(rows, dtype=t.float32, device=x.device) if stats else None
-    rstd = t.empty(rows, dtype=t.float32, device=x.device) if stats else None
-    N.check(N.lib().hum_layer_norm(ctypes.byref(a), _p(bias), eps, out.data_ptr(), c, _p(mean), _p(rstd), _stream(x.device)),
-            "hum_layer_norm")
+    mean = t.empty(rows, dtype=t.float32, device=dev) if stats else None
+    rstd = t.empty(rows, dtype=t.float32, device=dev) if stats else None
+    N.check(e.norm(a, _p(bias), eps, out.data_ptr(), c, _p(mean), _p(rstd), e.stream(x.get_device())), "hum_layer_norm")
     return out, mean, rstd
 
 
@@ -314,27 +345,26 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, needs=(True, True, True)
     """(dx, d_weight, d_bias) for the gradient dy of layer_norm's output, from its input x and the statistics
     layer_norm_forward returned.  needs: which of the three to compute (the others are None).  Without a weight the
     parameter gradients are computed only if param_dtype names their type."""
-    t = _torch()
+    e = _e()
+    t, dev = e.t, x.device
     if param_dtype is None:
         param_dtype = weight.dtype if weight is not None else None
-    x2, weight, a = _norm_args(x, weight, param_dtype if param_dtype is not None else t.float32)
+    x2, weight, _, a = _norm_args(e, x, weight, None, param_dtype if param_dtype is not None else t.float32)
     rows, c = x2.shape
-    dy2 = _unit(_on(dy, x.device, "dy", tuple(x.shape), (x.dtype,)).reshape(-1, c))
-    _on(mean, x.device, "mean", (rows,), (t.float32,))
-    _on(rstd, x.device, "rstd", (rows,), (t.float32,))
-    mean, rstd = mean.contiguous(), rstd.contiguous()
-    dx = t.empty(x.shape, dtype=x.dtype, device=x.device) if needs[0] else None
-    dw = t.empty(c, dtype=param_dtype, device=x.device) if needs[1] and param_dtype is not None else None
-    db = t.empty(c, dtype=param_dtype, device=x.device) if needs[2] and param_dtype is not None else None
+    dy2 = _unit(_on(dy, dev, "dy", x.shape, (x.dtype,)).reshape(-1, c))
+    mean = _on(mean, dev, "mean", (rows,), (t.float32,)).contiguous()
+    rstd = _on(rstd, dev, "rstd", (rows,), (t.float32,)).contiguous()
+    dx = t.empty(x.shape, dtype=x.dtype, device=dev) if needs[0] else None
+    dw = t.empty(c, dtype=param_dtype, device=dev) if needs[1] and param_dtype is not None else None
+    db = t.empty(c, dtype=param_dtype, device=dev) if needs[2] and param_dtype is not None else None
     ws, size = None, 0
     if dw is not None or db is not None:
         need = ctypes.c_uint64(0)
-        N.check(N.lib().hum_layer_norm_workspace(ctypes.byref(a), ctypes.byref(need)), "hum_layer_norm_workspace")
+        N.check(e.norm_workspace(a, ctypes.byref(need)), "hum_layer_norm_workspace")
         size = need.value
-        ws = t.empty(size, dtype=t.uint8, device=x.device)
-    N.check(N.lib().hum_layer_norm_backward(ctypes.byref(a), dy2.data_ptr(), dy2.stride(0), mean.data_ptr(), rstd.data_ptr(),
-                                            _p(dx), c, _p(dw), _p(db), _p(ws), size, _stream(x.device)),
-            "hum_layer_norm_backward")
+        ws = t.empty(size, dtype=t.uint8, device=dev)
+    N.check(e.norm_backward(a, dy2.data_ptr(), dy2.stride(0), mean.data_ptr(), rstd.data_ptr(), _p(dx), c, _p(dw), _p(db),
+                            _p(ws), size, e.stream(x.get_device())), "hum_layer_norm_backward")
     return dx, dw, db
 
 
@@ -342,9 +372,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """Layer norm over the last dimension of x (any leading shape, 1 to 16384 channels): (x - mean) / sqrt(var + eps) *
     weight + bias, sums in float32.  weight, bias: float32 or x's type, None = ones / zeros.  Differentiable in x, weight
     and bias; the parameter gradients have the same bits every time."""
-    t = _torch()
-    if t.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
-                                or (bias is not None and bias.requires_grad)):
+    if _e().t.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
+                                     or (bias is not None and bias.requires_grad)):
         return _autograd()[1].apply(x, weight, bias, eps)
     return layer_norm_forward(x, weight, bias, eps, stats=False)[0]
 
@@ -353,7 +382,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
 def decay_schedule(heads, shortest=2.5, longest=8.0, device="cuda"):
     """log_decay [heads]: the heads' decays 1 - 2^-e with e evenly spread from `shortest` to `longest` - half-lives from 4
     to some 180 steps, a step's reflex to a gait's cycle."""
-    t = _torch()
+    t = _e().t
     return t.log1p(-t.exp2(-t.linspace(shortest, longest, heads, dtype=t.float64))).float().to(device)
 
 
@@ -367,7 +396,7 @@ class PolicyMemory:
     NAMES = ("norm_weight", "norm_bias", "w_qkv", "head_weight", "head_bias", "w_out")
 
     def __init__(self, n_in=N.HUM_NOBS, heads=4, channels=32, device=0, seed=0, log_decay=None):
-        t = _torch()
+        t = _e().t
         self.device = t.device("cuda", device)
         self.n_in, self.heads, self.channels = n_in, heads, channels
         g = t.Generator().manual_seed(seed)
@@ -385,7 +414,7 @@ class PolicyMemory:
 
     def begin(self, n):
         """The empty state of n lanes [n, heads, channels, channels]."""
-        t = _torch()
+        t = _e().t
         return t.zeros(n, self.heads, self.channels, self.channels, dtype=t.float32, device=self.device)
 
     def _project(self, obs):
@@ -401,7 +430,7 @@ class PolicyMemory:
     def step(self, obs, state, reset=None, active=None):
         """Features [n, n_in] for the lanes' observations obs [n, n_in]; `state` moves on in place.  reset [n]: this step
         starts an episode (the previous step's done flags); active [n]: lanes that step."""
-        with _torch().no_grad():
+        with _e().t.no_grad():
             q, k, v = self._project(obs)
             return self._join(obs, decay_attention_step(q, k, v, self.log_decay, state, reset=reset, active=active))
 

@@ -30,6 +30,17 @@ def test_struct_layouts_match_header(tmp_path, cname, cls):
         assert getattr(S, f).offset == off, f
 
 
+def test_packed_arguments_are_the_structures():
+    """memory.py packs the argument structures itself: the same bytes as the ctypes mirror's."""
+    from ilrl_amd import memory as M
+    rows = [N.HumRows(0x1000 * i, i, 2 * i, 3 * i) for i in (1, 2, 3)]
+    a = N.HumDecayAttnArgs(1, 2, 3, 4, 5, 6, 7, 8, 0.25, 9, *rows, 10, 11, 12, 13, 14, 15)
+    flat = [v for r in rows for v in (r.ptr, r.lane, r.step, r.head)]
+    assert M._ATTN.pack(1, 2, 3, 4, 5, 6, 7, 8, 0.25, 9, *flat, 10, 11, 12, 13, 14, 15) == bytes(a)
+    assert M._ROWS.pack(0x3000, 3, 6, 9) == bytes(rows[2])
+    assert M._NORM.pack(1, 2, 3, 4, 5, 6, 7, 8) == bytes(N.HumNormArgs(1, 2, 3, 4, 5, 6, 7, 8))
+
+
 def _attn(**kw):
     rows = N.HumRows(0x1000, 64, 64, 8)
     d = dict(device=0, type=N.HUM_F32, lanes=2, steps=3, heads=4, kv_heads=2, dk=8, dv=8, scale=1.0, log_decay=0x1000, q=rows,
