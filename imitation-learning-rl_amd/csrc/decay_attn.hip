@@ -27,8 +27,8 @@
 // float16 inputs use the float32 matrix instruction (16 times slower, 153 TFLOP/s on this card) and are not split.
 //
 // Non-finite values.  A row of Z multiplies zeros of P for the steps that must not see it (earlier steps, other
-// episodes), and 0 x inf is NaN: a chunk whose z rows hold one is walked step by step with the unseen rows zeroed, so
-// an episode that diverged leaves the next one, and its own earlier steps, untouched.
+// episodes), and 0 x inf is NaN: such values of z enter the products as zeros and make NaN of the channels of exactly the
+// steps that see them, so an episode that diverged leaves the next one, and its own earlier steps, untouched.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -53,12 +53,13 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 
 struct Rows {               // [lane, step, head, channel] with unit channel stride
     void* p;
     long lane, step, head;  // strides in elements
     int shared;             // heads that read one of its heads
-    int vec;                // 8 channels are 16 aligned bytes, steps do not overlap, 32 of them span less than 2^31 bytes
+    int vec;                // rows of 16-byte units, aligned; steps do not overlap and lie less than 2^25 bytes apart
 };
 
 struct Role {
@@ -73,12 +74,11 @@ struct Role {
     long sy, sz;            // one of them is 1
     long in_unit, in_seg, out_unit, out_seg;   // from one (lane, head) / segment to the next
     int s_vec;              // the state's rows of unit stride are 16-byte aligned
-    int slice0;             // first workgroup part of this role
 };
 
 struct WalkArgs {
     Role r[3];
-    int nroles, parts;
+    int nroles;
     int lanes, steps, heads;
     int segs, seg_steps;    // the walk of a (lane, head) is cut into segs pieces of seg_steps (a multiple of 32) steps
     int last_only;          // state_out is the last segment's
@@ -103,128 +103,129 @@ __device__ __forceinline__ void buf_store(Buf b, int off, u32x4 v) { __builtin_a
 __device__ __forceinline__ f32x4 buf_load4(Buf b, int off) { return __builtin_bit_cast(f32x4, buf_load(b, off)); }
 __device__ __forceinline__ void buf_store4(Buf b, int off, f32x4 v) { buf_store(b, off, __builtin_bit_cast(u32x4, v)); }
 
-// ---- the element types: ST storage, operands of 8 consecutive contraction indexes per lane
-template <int ST> struct Num;   // HUM_F32 / HUM_F16: float32 matrix instructions
-
-template <> struct Num<HUM_BF16> {
-    typedef bf16x8 Op;
-    typedef __bf16 Elem;
-    static constexpr int PAD = 8, PARTS = 3, SIZE = 2;
-    static __device__ __forceinline__ Op zero() { return Op{}; }
-    static __device__ __forceinline__ Op load(Buf b, int off) { return __builtin_bit_cast(Op, buf_load(b, off)); }
-    static __device__ __forceinline__ void store(Buf b, int off, f32x8 v) {
-        buf_store(b, off, __builtin_bit_cast(u32x4, __builtin_convertvector(v, Op)));   // to nearest, ties to even
-    }
-    static __device__ __forceinline__ Op load(const void* p, long off, int n) {   // n of 8 elements, any alignment
-        const __bf16* e = (const __bf16*)p + off;
-        Op v = {};
-#pragma unroll
-        for (int j = 0; j < 8; j++)
-            if (j < n) v[j] = e[j];
-        return v;
-    }
-    static __device__ __forceinline__ void store(void* p, long off, int n, f32x8 v) {
-        __bf16* e = (__bf16*)p + off;
-        const Op o = __builtin_convertvector(v, Op);
-#pragma unroll
-        for (int j = 0; j < 8; j++)
-            if (j < n) e[j] = o[j];
-    }
-    static __device__ __forceinline__ bool finite(Op v) {
-        const u32x4 u = __builtin_bit_cast(u32x4, v);
-        bool bad = false;
-#pragma unroll
-        for (int i = 0; i < 4; i++) bad |= (u[i] & 0x7f80u) == 0x7f80u || (u[i] & 0x7f800000u) == 0x7f800000u;
-        return !bad;
-    }
-    static __device__ __forceinline__ void mma(f32x4& c, Op a, Op b) {
-        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-    }
-    // v as N bf16 parts: each the rounding of what the ones before leave
-    template <int N>
-    static __device__ __forceinline__ void split(f32x8 v, Op (&o)[N]) {
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-            o[i] = __builtin_convertvector(v, Op);
-            if (i + 1 < N) v -= __builtin_convertvector(o[i], f32x8);
-        }
-    }
-    static __device__ __forceinline__ f32x8 wide(Op a) { return __builtin_convertvector(a, f32x8); }
-    // rows s0 .. s0 + 7 of column c (4 columns per quarter of 16 lanes: the transposing LDS load)
-    static __device__ __forceinline__ void put(Elem* m, Op v) { *(Op*)m = v; }
-    static __device__ __forceinline__ Op column(const Elem* m, int pitch, int s0, int c0, int r) {
-        typedef __attribute__((address_space(3))) bf16x4 L4;
-        const Elem* p = m + (s0 + (r >> 2)) * pitch + c0 + 8 * (r & 3);
-        const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((L4*)p);
-        const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((L4*)(p + 4 * pitch));
-        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-    }
-};
-
-template <int ST> struct Num {
-    typedef f32x8 Op;
-    typedef float Elem;
-    static constexpr int PAD = 4, PARTS = 1, SIZE = ST == HUM_F16 ? 2 : 4;
-    static __device__ __forceinline__ Op zero() { return Op{}; }
-    static __device__ __forceinline__ Op load(Buf b, int off) {
-        if constexpr (ST == HUM_F16) return __builtin_convertvector(__builtin_bit_cast(f16x8, buf_load(b, off)), Op);
-        else return __builtin_shufflevector(buf_load4(b, off), buf_load4(b, off + 16), 0, 1, 2, 3, 4, 5, 6, 7);
-    }
-    static __device__ __forceinline__ void store(Buf b, int off, f32x8 v) {
-        if constexpr (ST == HUM_F16) {
-            buf_store(b, off, __builtin_bit_cast(u32x4, __builtin_convertvector(v, f16x8)));
-        } else {
-            buf_store4(b, off, __builtin_shufflevector(v, v, 0, 1, 2, 3));
-            buf_store4(b, off + 16, __builtin_shufflevector(v, v, 4, 5, 6, 7));
-        }
-    }
-    typedef typename std::conditional<ST == HUM_F16, _Float16, float>::type Stored;
-    static __device__ __forceinline__ Op load(const void* p, long off, int n) {
-        const Stored* e = (const Stored*)p + off;
-        Op v = {};
-#pragma unroll
-        for (int j = 0; j < 8; j++)
-            if (j < n) v[j] = (float)e[j];
-        return v;
-    }
-    static __device__ __forceinline__ void store(void* p, long off, int n, f32x8 v) {
-        Stored* e = (Stored*)p + off;
-#pragma unroll
-        for (int j = 0; j < 8; j++)
-            if (j < n) e[j] = (Stored)v[j];
-    }
-    static __device__ __forceinline__ bool finite(Op v) {
-        bool bad = false;
-#pragma unroll
-        for (int i = 0; i < 8; i++) bad |= (__builtin_bit_cast(unsigned, (float)v[i]) & 0x7f800000u) == 0x7f800000u;
-        return !bad;
-    }
-    static __device__ __forceinline__ void mma(f32x4& c, Op a, Op b) {
-#pragma unroll
-        for (int j = 0; j < 8; j++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
-    }
-    template <int N>
-    static __device__ __forceinline__ void split(f32x8 v, Op (&o)[N]) { o[0] = v; }
-    static __device__ __forceinline__ f32x8 wide(Op a) { return a; }
-    static __device__ __forceinline__ void put(Elem* m, Op v) {
-        *(f32x4*)m = __builtin_shufflevector(v, v, 0, 1, 2, 3);
-        *(f32x4*)(m + 4) = __builtin_shufflevector(v, v, 4, 5, 6, 7);
-    }
-    static __device__ __forceinline__ Op column(const Elem* m, int pitch, int s0, int c0, int r) {
-        const Elem* p = m + s0 * pitch + c0 + 8 * (r >> 2) + (r & 3);
-        Op v;
-#pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = p[j * pitch];
-        return v;
-    }
-};
-
 __device__ __forceinline__ f32x8 pair(f32x4 a, f32x4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
+// a * b with 0 times anything 0, infinities and NaN too: a weight of zero is a mask
+extern "C" __device__ float mul0(float a, float b) __asm("llvm.amdgcn.fmul.legacy");
 
-// LDS operations of one wave execute in order; this keeps the compiler from moving them past each other
-__device__ __forceinline__ void lds_order() {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
+// v as N bf16 parts, each the rounding of what the ones before leave
+template <int N>
+__device__ __forceinline__ void split(f32x8 v, bf16x8 (&o)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        o[i] = __builtin_convertvector(v, bf16x8);   // to nearest, ties to even
+        if (i + 1 < N) {
+            const u32x4 u = __builtin_bit_cast(u32x4, o[i]);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                v[2 * j] -= __builtin_bit_cast(float, u[j] << 16);
+                v[2 * j + 1] -= __builtin_bit_cast(float, u[j] & 0xffff0000u);
+            }
+        }
+    }
+}
+template <int N>
+__device__ __forceinline__ f32x8 whole(const bf16x8 (&o)[N]) {
+    f32x8 v = {};
+#pragma unroll
+    for (int i = N - 1; i >= 0; i--) {
+        const u32x4 u = __builtin_bit_cast(u32x4, o[i]);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float lo = __builtin_bit_cast(float, u[j] << 16), hi = __builtin_bit_cast(float, u[j] & 0xffff0000u);
+            v[2 * j] = i == N - 1 ? lo : v[2 * j] + lo;
+            v[2 * j + 1] = i == N - 1 ? hi : v[2 * j + 1] + hi;
+        }
+    }
+    return v;
+}
+// c += a b over 32 contraction indexes; parts i, j with i + j > 2 stay below 2^-27 of the product
+template <int NA, int NB>
+__device__ __forceinline__ void mma(f32x4& c, const bf16x8 (&a)[NA], const bf16x8 (&b)[NB]) {
+#pragma unroll
+    for (int i = 0; i < NA; i++)
+#pragma unroll
+        for (int j = 0; j < NB; j++)
+            if (i + j < 3) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[j], c, 0, 0, 0);
+}
+// rows s0 .. s0 + 7 of 16 columns, 4 neighbours per quarter of 16 lanes: the transposing LDS load
+__device__ __forceinline__ bf16x8 column(const __bf16* m, int pitch, int s0, int c0, int r) {
+    typedef __attribute__((address_space(3))) bf16x4 L4;
+    const __bf16* p = m + (s0 + (r >> 2)) * pitch + c0 + 8 * (r & 3);
+    const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((L4*)p);
+    const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((L4*)(p + 4 * pitch));
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// ---- the element types.  Every one goes through the bf16 matrix cores: a float16 is the sum of two bf16 parts, a float32
+// of three, exactly (up to 2^-27), and the product of two such sums takes up to six matrix instructions - 96 cycles where the
+// float32 instruction takes 256.  IN: parts of an input, MID: of P and of the state that O reads
+template <int ST> struct Num;
+template <> struct Num<HUM_BF16> { typedef __bf16 T; static constexpr int IN = 1, MID = 2, SIZE = 2; };
+template <> struct Num<HUM_F16> { typedef _Float16 T; static constexpr int IN = 2, MID = 2, SIZE = 2; };
+template <> struct Num<HUM_F32> { typedef float T; static constexpr int IN = 3, MID = 3, SIZE = 4; };
+
+// 16 loaded bytes into the planes of an LDS tile
+template <int ST>
+__device__ __forceinline__ void put(__bf16* m, int plane, u32x4 raw) {
+    if constexpr (ST == HUM_BF16) {
+        *(u32x4*)m = raw;
+    } else if constexpr (ST == HUM_F16) {
+        bf16x8 o[2];
+        split<2>(__builtin_convertvector(__builtin_bit_cast(f16x8, raw), f32x8), o);
+        *(bf16x8*)m = o[0];
+        *(bf16x8*)(m + plane) = o[1];
+    } else {
+        f32x4 v = __builtin_bit_cast(f32x4, raw);
+#pragma unroll
+        for (int i = 0; i < 3; i++) {
+            const bf16x4 o = __builtin_convertvector(v, bf16x4);
+            *(bf16x4*)(m + i * plane) = o;
+            const u32x2 u = __builtin_bit_cast(u32x2, o);
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                v[2 * j] -= __builtin_bit_cast(float, u[j] << 16);
+                v[2 * j + 1] -= __builtin_bit_cast(float, u[j] & 0xffff0000u);
+            }
+        }
+    }
+}
+// sign bits of the result: whether an element's exponent is all ones
+template <int ST>
+__device__ __forceinline__ unsigned odd_bits(u32x4 u) {
+    constexpr unsigned exponent = ST == HUM_BF16 ? 0x7f807f80u : ST == HUM_F16 ? 0x7c007c00u : 0x7f800000u;
+    constexpr unsigned one = ST == HUM_BF16 ? 0x00800080u : ST == HUM_F16 ? 0x04000400u : 0x00800000u;
+    unsigned bad = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) bad |= (u[i] & exponent) + one;
+    return bad & (ST == HUM_F32 ? 0x80000000u : 0x80008000u);
+}
+// 8 channels of a row, rounded once; bytes `second` on are the upper half of a float32 row's
+template <int ST>
+__device__ __forceinline__ void store(Buf b, int at, int second, f32x8 v) {
+    if constexpr (ST == HUM_F32) {
+        buf_store4(b, at, __builtin_shufflevector(v, v, 0, 1, 2, 3));
+        buf_store4(b, second, __builtin_shufflevector(v, v, 4, 5, 6, 7));
+    } else if constexpr (ST == HUM_F16) {
+        buf_store(b, at, __builtin_bit_cast(u32x4, __builtin_convertvector(v, f16x8)));
+    } else {
+        buf_store(b, at, __builtin_bit_cast(u32x4, __builtin_convertvector(v, bf16x8)));
+    }
+}
+template <int ST>
+__device__ __forceinline__ void store_some(void* p, long at, int n, f32x8 v) {   // n of 8, any alignment
+    typename Num<ST>::T* e = (typename Num<ST>::T*)p + at;
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+        if (j < n) e[j] = (typename Num<ST>::T)v[j];
+}
+
+// what the workgroup's waves wrote to LDS before it, all of them read behind it (loads in flight stay in flight)
+template <int WAVES>
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    if constexpr (WAVES > 1) __builtin_amdgcn_s_barrier();
+    else __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
 // 4 x 4 transposes inside quads of lanes: v[q] of quad lane i <-> v[i] of quad lane q
@@ -249,38 +250,37 @@ __device__ __forceinline__ f32x4 quad_transpose(f32x4 v) {
     return v;
 }
 
-// waves per SIMD that the registers are limited for: two hide each other's loads, where the state and operands fit into
-// 256 registers
-constexpr int walk_waves(int st, int dy, int dz) { return dy * dz * (st == HUM_BF16 ? 1 : 2) <= 4096 ? 2 : 1; }
+// waves per SIMD that the registers are limited for
+constexpr int walk_waves(int st, int d) { return st == HUM_BF16 ? (d <= 64 ? 3 : 2) : st == HUM_F32 && d > 64 ? 1 : 2; }
 
-// One wave per workgroup.  DY, DZ: channels of y and of the z slice rounded up to 32.  FAST: every operand may be accessed
-// 16 bytes at a time through buffers; else element by element, at any alignment and stride.
-template <int ST, int DY, int DZ, bool FAST>
-__global__ void __launch_bounds__(64, walk_waves(ST, DY, DZ)) walk_kernel(WalkArgs a) {
-    typedef Num<ST> M;
-    typedef typename M::Op Op;
-    constexpr int KY = DY / 32, KZ = DZ / 32;
-    constexpr int PO = M::PARTS > 1 ? 2 : 1;   // parts of P and of the state's reading
-    constexpr int PS = M::PARTS;               // parts of what joins the state
-    constexpr int PY = DY + M::PAD, PZ = DZ + M::PAD;
-    constexpr bool WEIGH_Y = KY <= KZ;         // the side with fewer tiles carries the weights into the state
-    __shared__ __attribute__((aligned(16))) typename M::Elem ly[CH * PY];
-    __shared__ __attribute__((aligned(16))) typename M::Elem lz[CH * PZ];
+// One workgroup per (lane, head), role and segment; D / 32 waves, each with 32 of z's channels and its slice of the state.
+// The waves share the chunk's x and y rows and P.  D: channels rounded up, the larger of y's and z's.  FAST: every operand may
+// be accessed 16 bytes at a time through buffers; else element by element, at any alignment and stride.  OUTS: rows come out
+// (else the states of the segments are wanted only).
+template <int ST, int D, bool FAST, bool OUTS>
+__global__ void __launch_bounds__(2 * D, walk_waves(ST, D)) walk_kernel(WalkArgs a) {
+    constexpr int W = D / 32, K = D / 32;      // waves; operands of 32 channels
+    constexpr int IN = Num<ST>::IN, MID = Num<ST>::MID, SIZE = Num<ST>::SIZE, UNIT = 16 / SIZE;
+    constexpr int PITCH = D + 8;               // of x and y in LDS: 16-byte reads of 16 rows meet no bank twice
+    constexpr int PLANE = CH * PITCH, ZPLANE = CH * 32;
+    __shared__ __attribute__((aligned(16))) __bf16 lx[OUTS ? IN * PLANE : 8], ly[IN * PLANE], lz[W][IN * ZPLANE];
+    __shared__ __attribute__((aligned(16))) bf16x8 lp[OUTS ? 2 : 1][MID][64];
     // lambda^d times the scale's part for d = -31 .. 32 steps, zeros for d < 0: between two steps of a chunk, and from a
     // step to the chunk's end
     __shared__ float pow_pair[2 * CH], pow_add[2 * CH];
+    __shared__ unsigned lodd[W][32];
 
-    const int l = threadIdx.x, g = l >> 4, r = l & 15;
-    // the parts (roles, slices) of one segment read the same rows, and NEAR segments in a row are neighbours in memory (the
-    // heads of a lane, lanes of a time-major step): they go to one XCD, one after the other.  Gradient of 4096 lanes x 32
-    // steps: 380 us, 407 with NEAR = 1, 377 with 32 (which leaves XCDs idle at few lanes)
-    const int block = blockIdx.x, part = block / XCDS % a.parts, turn = block / (XCDS * a.parts);
+    const int tid = threadIdx.x, l = tid & 63, g = l >> 4, r = l & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // the roles of one segment read the same rows, and NEAR segments in a row are neighbours in memory (the heads of a lane,
+    // lanes of a time-major step): they go to one XCD, one after the other.  Gradient of 4096 lanes x 32 steps: 380 us,
+    // 407 with NEAR = 1, 377 with 32 (which leaves XCDs idle at few lanes)
+    const int block = blockIdx.x, ri = block / XCDS % a.nroles, turn = block / (XCDS * a.nroles);
     const int item = (turn / NEAR * XCDS + block % XCDS) * NEAR + turn % NEAR;
     if (item >= a.lanes * a.heads * a.segs) return;
     const int unit = item / a.segs, seg = item - unit * a.segs;
-    const int ri = (a.nroles > 1 && part >= a.r[1].slice0) + (a.nroles > 2 && part >= a.r[2].slice0);
     const Role& R = a.r[ri];
-    const int dz0 = (part - R.slice0) * DZ;
+    const int dz0 = 32 * wave;
     const int b = unit / a.heads, h = unit - b * a.heads;
     const int steps = a.steps;
     int len = steps;
@@ -288,99 +288,105 @@ __global__ void __launch_bounds__(64, walk_waves(ST, DY, DZ)) walk_kernel(WalkAr
         len = __builtin_amdgcn_readfirstlane(a.lengths[b]);
         len = len < 0 ? 0 : len > steps ? steps : len;
     }
-    const int rev = R.rev;
+    const int rev = R.rev, dy = R.dy, dz = R.dz;
     const float lg = a.log_decay[h] * 1.44269504088896340736f;
     auto power = [&](int n) { return n == 0 ? 1.f : __builtin_amdgcn_exp2f(lg * (float)n); };
-    pow_pair[l] = l < CH - 1 ? 0.f : R.s_pair * power(l - (CH - 1));
-    pow_add[l] = l < CH - 1 ? 0.f : R.s_add * power(l - (CH - 1));
+    if (tid < 2 * CH) {
+        pow_pair[l] = l < CH - 1 ? 0.f : R.s_pair * power(l - (CH - 1));
+        pow_add[l] = l < CH - 1 ? 0.f : R.s_add * power(l - (CH - 1));
+    }
     const int seg0 = seg * a.seg_steps, seg1 = seg + 1 < a.segs ? seg0 + a.seg_steps : steps;
     const int end = len < seg1 ? len : seg1;
     auto row_of = [&](int tile) { return 8 * (r >> 2) + 4 * tile + (r & 3); };
-
-    // ---- rows of a chunk: x by walk step 16 c + r, y and z by step row_of(t)
-    auto head_of = [&](const Rows& m) { return (long)b * m.lane + (long)(h / m.shared) * m.head; };
-    const long hx = head_of(R.x), hy = head_of(R.y), hz = head_of(R.z), ho = head_of(R.out);
-    const unsigned char* marks = a.reset ? a.reset + (long)b * a.reset_lane : nullptr;
     auto time = [&](int n) { return rev ? len - 1 - n : n; };   // of walk step n
-    auto steps_from = [&](int n0) { return end - n0 < CH ? end - n0 : CH; };
-    // a chunk of L steps as a buffer from its earliest time to its last row's end: the steps behind L lie outside (walking
-    // backwards: before it, at negative offsets)
-    const int dy = R.dy, dz = R.dz, out_size = R.out_f32 ? 4 : M::SIZE;
-    const int sx = (int)R.x.step * M::SIZE, sy = (int)R.y.step * M::SIZE, sz = (int)R.z.step * M::SIZE, so = (int)R.out.step * out_size;
-    auto chunk = [&](const void* p, long head, long step, int d, int n0, int L, int size) {
-        const char* at = (const char*)p + (head + (long)(rev ? len - n0 - L : n0) * step) * size;
-        return buffer(p ? at : nullptr, ((L - 1) * (int)step + d) * size);
+    auto head_of = [&](const Rows& m) { return (long)b * m.lane + (long)(h / m.shared) * m.head; };
+
+    // ---- rows of a chunk: x and y by all waves, z by each wave its channels, in units of 16 bytes along a row: unit u of
+    // thread t is unit t % PER of row u T / PER + t / PER.  FAST: a chunk of L steps is a buffer from its earliest time to its
+    // last row's end, so the steps behind L lie outside (walking backwards: before it, at negative offsets, which are
+    // large ones); `at` is the address of the walk's next chunk's first row
+    struct View {
+        const char* at;
+        long hop;       // to the next chunk
+        int step, row;  // bytes from walk step to walk step forwards in time, bytes of a row
+        int off;        // the thread's byte offset
     };
-    auto row_at = [&](int n, int L, int step) { return (rev ? L - 1 - n : n) * step; };
-    Op X[2][KY], Y[2][KY], Z[2][KZ];
-    bool mark = false;
-    auto load_x = [&](int n0) {
-        const int L = steps_from(n0);
-        if constexpr (FAST) {
-            const Buf bx = chunk(R.x.p, hx, R.x.step, dy, n0, L, M::SIZE);
-#pragma unroll
-            for (int c = 0; c < 2; c++) {
-                const int at = row_at(16 * c + r, L, sx) + 8 * g * M::SIZE;
-#pragma unroll
-                for (int k = 0; k < KY; k++) X[c][k] = M::load(bx, (at + 32 * k * M::SIZE) | beyond(32 * k + 8 * g, dy));
-            }
-        } else {
-#pragma unroll
-            for (int c = 0; c < 2; c++) {
-                const int n = 16 * c + r;
-                const long at = hx + (long)time(n0 + n) * R.x.step;
-#pragma unroll
-                for (int k = 0; k < KY; k++) {
-                    const int d = 32 * k + 8 * g;
-                    X[c][k] = n < L && d < R.dy ? M::load(R.x.p, at + d, R.dy - d) : M::zero();
-                }
-            }
-        }
+    const int dir = rev ? -1 : 1;
+    auto view = [&](const Rows& m, int size, int d, int row, int channel) {
+        View v;
+        v.step = (int)m.step * size;
+        v.at = (const char*)m.p + (head_of(m) + (long)time(seg0) * m.step) * size;
+        v.hop = (long)dir * CH * v.step;
+        v.row = d * size;
+        v.off = channel < d ? dir * row * v.step + channel * size : OUTSIDE;
+        return v;
     };
-    auto load_yz = [&](int n0) {
-        const int L = steps_from(n0);
-        if constexpr (FAST) {
-            const Buf by = chunk(R.y.p, hy, R.y.step, dy, n0, L, M::SIZE), bz = chunk(R.z.p, hz, R.z.step, dz, n0, L, M::SIZE);
-#pragma unroll
-            for (int t = 0; t < 2; t++) {
-                const int aty = row_at(row_of(t), L, sy) + 8 * g * M::SIZE, atz = row_at(row_of(t), L, sz) + (dz0 + 8 * g) * M::SIZE;
-#pragma unroll
-                for (int k = 0; k < KY; k++) Y[t][k] = M::load(by, (aty + 32 * k * M::SIZE) | beyond(32 * k + 8 * g, dy));
-#pragma unroll
-                for (int k = 0; k < KZ; k++) Z[t][k] = M::load(bz, (atz + 32 * k * M::SIZE) | beyond(dz0 + 32 * k + 8 * g, dz));
-            }
-        } else {
-#pragma unroll
-            for (int t = 0; t < 2; t++) {
-                const int n = row_of(t);
-                const long aty = hy + (long)time(n0 + n) * R.y.step, atz = hz + (long)time(n0 + n) * R.z.step;
-#pragma unroll
-                for (int k = 0; k < KY; k++) {
-                    const int d = 32 * k + 8 * g;
-                    Y[t][k] = n < L && d < R.dy ? M::load(R.y.p, aty + d, R.dy - d) : M::zero();
-                }
-#pragma unroll
-                for (int k = 0; k < KZ; k++) {
-                    const int d = dz0 + 32 * k + 8 * g;
-                    Z[t][k] = n < L && d < R.dz ? M::load(R.z.p, atz + d, R.dz - d) : M::zero();
-                }
-            }
+    auto chunk = [&](const View& v, int L) { return buffer(rev ? v.at - (long)(L - 1) * v.step : v.at, (L - 1) * v.step + v.row); };
+    constexpr int PER = D / UNIT, PERZ = 32 / UNIT, N = CH * 32 / UNIT / 64;   // units of a row, of a wave's part; of a thread
+    View vx = {}, vy = {}, vz = {}, vo = {};
+    const int out_size = R.out_f32 ? 4 : SIZE;
+    const unsigned char* marks = a.reset ? a.reset + (long)b * a.reset_lane : nullptr;
+    const char* at_mark = nullptr;
+    const int mark_step = (int)a.reset_step, mark_off = (rev ? 1 - l : l) * mark_step;
+    if constexpr (FAST) {
+        vy = view(R.y, SIZE, dy, tid / PER, tid % PER * UNIT);
+        vz = view(R.z, SIZE, dz, l / PERZ, dz0 + l % PERZ * UNIT);
+        if constexpr (OUTS) {
+            vx = view(R.x, SIZE, dy, tid / PER, tid % PER * UNIT);
+            vo = view(R.out, out_size, dz, r, dz0 + 8 * g);
         }
-        // bit j separates the chunk's walk steps j - 1 and j (bit 0 the entering state, bit L the leaving one).  An
-        // episode's first step is cut off from what time puts before it, so the backward walk has it one later.
-        if (marks) {
-            const int n = n0 + l - rev;
-            mark = l <= CH && l >= rev && l - rev < CH && n < end && marks[(long)time(n) * a.reset_step] != 0;
-        }
-    };
-    if (seg0 < end) {
-        if (R.out.p) load_x(seg0);
-        load_yz(seg0);
+        at_mark = marks ? (const char*)marks + (long)time(seg0) * a.reset_step : nullptr;
     }
+    u32x4 rx[OUTS ? N : 1], ry[N], rz[N];
+    int mark = 0;
+    auto fetch = [&](const Rows& m, View& v, int rows, int row, int channel, int d, int n0, int L, u32x4* raw) {
+        if constexpr (FAST) {
+            const Buf bm = chunk(v, L);
+            const int base = rev ? (L - 1) * v.step : 0;
+#pragma unroll
+            for (int u = 0; u < N; u++) raw[u] = buf_load(bm, v.off + (base + dir * u * rows * v.step));
+            v.at += v.hop;
+        } else {
+            typedef typename Num<ST>::T E;
+            typedef E EU __attribute__((ext_vector_type(UNIT)));
+#pragma unroll
+            for (int u = 0; u < N; u++) {
+                const int n = u * rows + row;
+                const E* e = (const E*)m.p + head_of(m) + (long)time(n0 + n) * m.step + channel;
+                EU x = {};
+#pragma unroll
+                for (int j = 0; j < UNIT; j++)
+                    if (n < L && channel + j < d) x[j] = e[j];
+                raw[u] = __builtin_bit_cast(u32x4, x);
+            }
+        }
+    };
+    auto load_rows = [&](int n0) {
+        const int L = end - n0 < CH ? end - n0 : CH;
+        if constexpr (OUTS) fetch(R.x, vx, 64 * W / PER, tid / PER, tid % PER * UNIT, dy, n0, L, rx);
+        fetch(R.y, vy, 64 * W / PER, tid / PER, tid % PER * UNIT, dy, n0, L, ry);
+        fetch(R.z, vz, 64 / PERZ, l / PERZ, dz0 + l % PERZ * UNIT, dz, n0, L, rz);
+        // lane j has the mark that separates the chunk's walk steps j - 1 and j (0: from the entering state, L: from the
+        // leaving one).  An episode's first step is cut off from what time puts before it, so the backward walk has it one
+        // later.
+        if constexpr (FAST) {
+            const Buf bm = buffer(rev ? at_mark - (long)(L - 1) * mark_step : at_mark, marks ? (L - 1) * mark_step + 1 : 0);
+            mark = __builtin_amdgcn_raw_buffer_load_b8(bm, mark_off + (rev ? (L - 1) * mark_step : 0), 0, 0);
+            at_mark += (long)dir * CH * mark_step;
+        } else if (marks) {
+            const int n = l - rev;
+            mark = n >= 0 && n < L ? marks[(long)time(n0 + n) * a.reset_step] : 0;
+        }
+    };
+    auto lay = [&](__bf16* m, int pitch, int plane, int rows, int row, int channel, const u32x4* raw) {
+#pragma unroll
+        for (int u = 0; u < N; u++) put<ST>(m + (u * rows + row) * pitch + channel, plane, raw[u]);
+    };
+    if (seg0 < end) load_rows(seg0);
 
     // ---- the entering state: tile (i, j) holds y channels 32 (i / 2) + 8 g + 4 (i & 1) + 0..3 of z channel zc(j)
-    f32x4 S[2 * KY][2 * KZ];
-    auto zc = [&](int j) { return dz0 + 32 * (j >> 1) + 8 * (r >> 2) + 4 * (j & 1) + (r & 3); };
+    f32x4 S[2 * K][2];
+    auto zc = [&](int j) { return dz0 + 8 * (r >> 2) + 4 * j + (r & 3); };
     // rows of unit stride are read 16 bytes at a time: along y directly, along z by one row a quad lane and a transpose
     const bool along_y = R.sy == 1;
     const int quad = along_y ? 0 : r & 3, s_y = along_y ? 1 : dz, s_z = along_y ? dy : 1;
@@ -388,32 +394,34 @@ __global__ void __launch_bounds__(64, walk_waves(ST, DY, DZ)) walk_kernel(WalkAr
         const int y = 32 * (i >> 1) + 8 * g + 4 * (i & 1) + quad, z = zc(j) - quad;
         return 4 * (__mul24(z, s_z) + __mul24(y, s_y)) | beyond(y, dy) | beyond(z, dz);
     };
+    auto turn_state = [&] {
+        if (!along_y)
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int i = 0; i < 2 * K; i++) S[i][j] = quad_transpose(S[i][j]);
+    };
     {
         const float* s = R.state_in ? R.state_in + (long)unit * R.in_unit + (long)seg * R.in_seg : nullptr;
         if constexpr (FAST) {
             const Buf bs = buffer(s, 4 * dy * dz);
 #pragma unroll
-            for (int j = 0; j < 2 * KZ; j++)
+            for (int j = 0; j < 2; j++)
 #pragma unroll
-                for (int i = 0; i < 2 * KY; i++) S[i][j] = buf_load4(bs, state_at(i, j));
-            if (!along_y)
-#pragma unroll
-                for (int j = 0; j < 2 * KZ; j++)
-#pragma unroll
-                    for (int i = 0; i < 2 * KY; i++) S[i][j] = quad_transpose(S[i][j]);
+                for (int i = 0; i < 2 * K; i++) S[i][j] = buf_load4(bs, state_at(i, j));
+            turn_state();
         } else {
 #pragma unroll
-            for (int j = 0; j < 2 * KZ; j++)
+            for (int j = 0; j < 2; j++)
 #pragma unroll
-                for (int i = 0; i < 2 * KY; i++) {
+                for (int i = 0; i < 2 * K; i++) {
                     const int y0 = 32 * (i >> 1) + 8 * g + 4 * (i & 1), z = zc(j);
 #pragma unroll
                     for (int q = 0; q < 4; q++)
-                        S[i][j][q] = s && z < R.dz && y0 + q < R.dy ? s[(long)z * R.sz + (long)(y0 + q) * R.sy] : 0.f;
+                        S[i][j][q] = s && z < dz && y0 + q < dy ? s[(long)z * R.sz + (long)(y0 + q) * R.sy] : 0.f;
                 }
         }
     }
-
     float w_in[2];
 #pragma unroll
     for (int c = 0; c < 2; c++) w_in[c] = R.s_in * power(16 * c + r + 1 - rev);
@@ -422,221 +430,231 @@ __global__ void __launch_bounds__(64, walk_waves(ST, DY, DZ)) walk_kernel(WalkAr
     for (int n0 = seg0; n0 < end; n0 += CH) {
         const int L = end - n0 < CH ? end - n0 : CH;
         const bool more = n0 + CH < end;
-        // a mark beyond the chunk's last step (its bit L when walking backwards) is this chunk's as well as the first
-        // of the next
-        const unsigned long long cut = marks ? __ballot(mark) & ((2ull << (L - 1 + rev)) - 1) : 0;
-        bool sane = true;
+        // a mark behind the chunk's last step (lane L's, walking backwards) is this chunk's as well as the next one's first
+        const unsigned long long cut = __ballot(mark != 0) & ((2ull << (L - 1 + rev)) - 1) & ~(unsigned long long)rev;
+        unsigned bad = 0;
 #pragma unroll
-        for (int t = 0; t < 2; t++)
-#pragma unroll
-            for (int k = 0; k < KZ; k++) sane = sane && M::finite(Z[t][k]);
-        const bool slow = __any(!sane);
-
+        for (int u = 0; u < N; u++) bad |= odd_bits<ST>(rz[u]);
+        const bool slow = __any(bad != 0);
         // the last cut at or before step n of the chunk: step n sees the steps from there on, and what entered the chunk only
         // if there is none
         auto cuts_to = [&](int n) { return cut & ((2ull << n) - 1); };
         auto last_cut = [&](unsigned long long m) { return m ? 63 - __builtin_clzll(m) : 0; };
-        int seen[2];
-        float wi[2];
-#pragma unroll
-        for (int c = 0; c < 2; c++) {
-            const unsigned long long m = cuts_to(16 * c + r);
-            seen[c] = last_cut(m) - 8 * g;
-            wi[c] = m ? 0.f : w_in[c];
-        }
+        const int leaving = last_cut(cut);   // what leaves the chunk is of the steps from here on
 
-        lds_order();
+        lds_barrier<W>();   // the chunk before has been read
+        if constexpr (OUTS) lay(lx, PITCH, PLANE, 64 * W / PER, tid / PER, tid % PER * UNIT, rx);
+        lay(ly, PITCH, PLANE, 64 * W / PER, tid / PER, tid % PER * UNIT, ry);
+        lay(lz[wave], 32, ZPLANE, 64 / PERZ, l / PERZ, l % PERZ * UNIT, rz);
+        lds_barrier<W>();
+        if (more) load_rows(n0 + CH);   // the chunk is in LDS: the registers take the next one's rows
+        auto read = [&](const __bf16* m, int row, int k, bf16x8 (&o)[IN]) {
 #pragma unroll
-        for (int t = 0; t < 2; t++) {
-#pragma unroll
-            for (int k = 0; k < KY; k++) M::put(ly + row_of(t) * PY + 32 * k + 8 * g, Y[t][k]);
-#pragma unroll
-            for (int k = 0; k < KZ; k++) M::put(lz + row_of(t) * PZ + 32 * k + 8 * g, Z[t][k]);
-        }
-        lds_order();
+            for (int i = 0; i < IN; i++) o[i] = *(const bf16x8*)(m + i * PLANE + row * PITCH + 32 * k + 8 * g);
+        };
 
-        // ---- P^T: rows s, columns t; masked entries are chosen away, not multiplied
-        Op P[2][PO];
-        if (R.out.p) {
+        // ---- P^T: rows s (step row_of(t)), columns t (walk step 16 c + r).  Columns 16 c .. are formed by wave c (by the only
+        // one) for all
+        if constexpr (OUTS) {
 #pragma unroll
             for (int c = 0; c < 2; c++) {
+                if (W > 1 && wave != c) continue;
                 f32x4 p[2];
 #pragma unroll
-                for (int t = 0; t < 2; t++) {
-                    p[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+                for (int t = 0; t < 2; t++) p[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int k = 0; k < KY; k++) M::mma(p[t], Y[t][k], X[c][k]);
+                for (int k = 0; k < K; k++) {
+                    bf16x8 x[IN], y[IN];
+                    read(lx, 16 * c + r, k, x);
+#pragma unroll
+                    for (int t = 0; t < 2; t++) {
+                        read(ly, row_of(t), k, y);
+                        mma(p[t], y, x);
+                    }
                 }
                 f32x8 v = pair(p[0], p[1]);
+                float w[8];
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const float w = pow_pair[CH - 1 + 16 * c + r - 8 * g - j];
-                    v[j] = w != 0.f && j >= seen[c] ? v[j] * w : 0.f;
+                for (int j = 0; j < 8; j++) w[j] = pow_pair[CH - 1 + 16 * c + r - 8 * g - j];
+                if (cut) {
+                    const int seen = last_cut(cuts_to(16 * c + r)) - 8 * g;
+#pragma unroll
+                    for (int j = 0; j < 8; j++) w[j] = j >= seen ? w[j] : 0.f;
                 }
-                M::template split<PO>(v, P[c]);
+#pragma unroll
+                for (int j = 0; j < 8; j++) v[j] = mul0(v[j], w[j]);
+                bf16x8 parts[MID];
+                split(v, parts);
+#pragma unroll
+                for (int u = 0; u < MID; u++) lp[c][u][l] = parts[u];
             }
+            lds_barrier<W>();
         }
-        __builtin_amdgcn_sched_barrier(0);
-        if (more) load_yz(n0 + CH);   // y and z are in LDS: their registers take the next chunk's rows
-
-        // ---- one pass over the chunk's steps, or one per step where a z row is not finite
-        for (int lo = 0; lo < L;) {
-            const int hi = slow ? lo + 1 : L;
-            Op T[2 * KZ];   // Z^T
-#pragma unroll
-            for (int j = 0; j < 2 * KZ; j++) T[j] = M::column(lz, PZ, 8 * g, 32 * (j >> 1) + 4 * (j & 1), r);
-            if (slow) {     // of which step lo sees its episode's, up to itself
-                const int from = last_cut(cuts_to(lo));
-#pragma unroll
-                for (int j = 0; j < 2 * KZ; j++)
-#pragma unroll
-                    for (int e = 0; e < 8; e++) T[j][e] = 8 * g + e >= from && 8 * g + e < hi ? T[j][e] : (typename M::Elem)0.f;
+        if (leaving > 0) {   // z's weights will be zeros for these steps, which a y row that is not finite would not heed
+            for (int e = tid; e < leaving * IN * (D / 8); e += 64 * W) {
+                const int row = e / (IN * (D / 8)), at = e % (IN * (D / 8));
+                *(u32x4*)(ly + at / (D / 8) * PLANE + row * PITCH + at % (D / 8) * 8) = u32x4{0, 0, 0, 0};
             }
-            // ---- O^T: rows z channels, columns t
-            if (R.out.p) {
+            lds_barrier<W>();
+        }
+
+        __builtin_amdgcn_sched_barrier(0);   // (what the scheduler would move across costs more registers than there are)
+        if (dz0 < dz) {   // a wave behind z's channels only helps to load
+            bf16x8 T[2][IN];   // Z^T
 #pragma unroll
-                for (int k = 0; k < KZ; k++) {
-                    f32x4 o[2][2];
+            for (int j = 0; j < 2; j++)
 #pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        const int j = 2 * k + e;
+                for (int i = 0; i < IN; i++) T[j][i] = column(lz[wave] + i * ZPLANE, 32, 8 * g, 4 * j, r);
+            // z values that are not finite: zeros to the products, and NaN to what sees them.  The steps at which a channel
+            // has some go to odd[channel]
+            unsigned odd[2] = {0, 0};
+            if (slow) {
 #pragma unroll
-                        for (int c = 0; c < 2; c++) o[c][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+                for (int j = 0; j < 2; j++) {
 #pragma unroll
-                        for (int q = 0; q < KY; q++) {
-                            Op sp[PO];
-                            M::template split<PO>(pair(S[2 * q][j], S[2 * q + 1][j]), sp);
+                    for (int e = 0; e < 8; e++) {
+                        const bool is = (__builtin_bit_cast(unsigned short, (__bf16)T[j][0][e]) & 0x7f80) == 0x7f80;
+                        odd[j] |= is ? 1u << (8 * g + e) : 0u;
 #pragma unroll
-                            for (int u = 0; u < PO; u++)
-#pragma unroll
-                                for (int c = 0; c < 2; c++) M::mma(o[c][e], sp[u], X[c][q]);
-                        }
-#pragma unroll
-                        for (int c = 0; c < 2; c++) {
-#pragma unroll
-                            for (int q = 0; q < 4; q++) o[c][e][q] = wi[c] != 0.f ? o[c][e][q] * wi[c] : 0.f;
-#pragma unroll
-                            for (int u = 0; u < PO; u++) M::mma(o[c][e], T[j], P[c][u]);
-                        }
+                        for (int i = 0; i < IN; i++) T[j][i][e] = is ? (__bf16)0.f : T[j][i][e];
                     }
-                    const int d = dz0 + 32 * k + 8 * g;
+                    odd[j] |= __shfl_xor(odd[j], 16);
+                    odd[j] |= __shfl_xor(odd[j], 32);
+                    if (g == 0) lodd[wave][8 * (r >> 2) + 4 * j + (r & 3)] = odd[j];
+                }
+                lds_barrier<1>();
+            }
+            // O^T: rows z channels, columns t
+            if constexpr (OUTS) {
+                f32x4 o[2][2];
 #pragma unroll
-                    for (int c = 0; c < 2; c++) {
-                        const int n = 16 * c + r;
-                        const f32x8 v = pair(o[c][0], o[c][1]);
-                        const bool in = n >= lo && n < hi && d < dz;
-                        if constexpr (FAST) {
-                            const Buf bo = chunk(R.out.p, ho, R.out.step, dz, n0, L, out_size);
-                            int at = (row_at(n, L, so) + d * out_size) | beyond(d, dz);
-                            if (slow) at = in ? at : OUTSIDE;
-                            if (R.out_f32) Num<HUM_F32>::store(bo, at, v);
-                            else M::store(bo, at, v);
-                        } else if (in) {
-                            const long at = ho + (long)time(n0 + n) * R.out.step + d;
-                            if (R.out_f32) Num<HUM_F32>::store(R.out.p, at, R.dz - d, v);
-                            else M::store(R.out.p, at, R.dz - d, v);
-                        }
+                for (int c = 0; c < 2; c++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++) o[c][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < K; k++) {
+                    bf16x8 x[2][IN];
+                    read(lx, r, k, x[0]);
+                    read(lx, 16 + r, k, x[1]);
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        bf16x8 sp[MID];
+                        split(pair(S[2 * k][j], S[2 * k + 1][j]), sp);
+#pragma unroll
+                        for (int c = 0; c < 2; c++) mma(o[c][j], sp, x[c]);
                     }
                 }
-                if (hi == L && more) load_x(n0 + CH);
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    const int n = 16 * c + r, d = dz0 + 8 * g;
+                    float wi = w_in[c];
+                    if (cut) wi = cuts_to(n) ? 0.f : wi;
+                    bf16x8 P[MID];
+#pragma unroll
+                    for (int u = 0; u < MID; u++) P[u] = lp[c][u][l];
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+#pragma unroll
+                        for (int q = 0; q < 4; q++) o[c][j][q] = mul0(o[c][j][q], wi);
+                        mma(o[c][j], T[j], P);
+                    }
+                    if (slow) {
+                        const unsigned sees = ((2u << n) - 1) & ~((1u << last_cut(cuts_to(n))) - 1);
+#pragma unroll
+                        for (int j = 0; j < 2; j++)
+#pragma unroll
+                            for (int q = 0; q < 4; q++)
+                                if (lodd[wave][8 * g + 4 * j + q] & sees) o[c][j][q] = __builtin_nanf("");
+                    }
+                    const f32x8 v = pair(o[c][0], o[c][1]);
+                    if constexpr (FAST) {
+                        const Buf bo = buffer(R.out.p ? (rev ? vo.at - (long)(L - 1) * vo.step : vo.at) : nullptr, (L - 1) * vo.step + vo.row);
+                        int at = vo.off + ((rev ? (L - 1) * vo.step : 0) + dir * 16 * c * vo.step);
+                        const int second = (at + 16) | beyond(d + 4, dz);
+                        if (ST == HUM_F32 || R.out_f32) store<HUM_F32>(bo, at, second, v);
+                        else store<ST>(bo, at, second, v);
+                    } else if (R.out.p && n < L && d < dz) {
+                        const long at = head_of(R.out) + (long)time(n0 + n) * R.out.step + d;
+                        if (R.out_f32) store_some<HUM_F32>(R.out.p, at, dz - d, v);
+                        else store_some<ST>(R.out.p, at, dz - d, v);
+                    }
+                }
             }
+            // the state behind the chunk (rows behind the chunk's last step are zeros)
             __builtin_amdgcn_sched_barrier(0);
-            // ---- the state behind the chunk
-            if (hi == L && (more || R.state_out)) {
+            if (more || R.state_out) {
                 const float through = cut ? 0.f : power(L);
                 passed *= through;
-                if (!cut) {
 #pragma unroll
-                    for (int i = 0; i < 2 * KY; i++)
+                for (int i = 0; i < 2 * K; i++)
 #pragma unroll
-                        for (int j = 0; j < 2 * KZ; j++) S[i][j] *= through;
-                } else {
+                    for (int j = 0; j < 2; j++)
 #pragma unroll
-                    for (int i = 0; i < 2 * KY; i++)
+                        for (int q = 0; q < 4; q++) S[i][j][q] = mul0(S[i][j][q], through);
+                float w[8];
 #pragma unroll
-                        for (int j = 0; j < 2 * KZ; j++) S[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+                for (int j = 0; j < 8; j++) w[j] = pow_add[CH - 1 + L - 1 + rev - 8 * g - j];
+                if (cut)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) w[j] = 8 * g + j >= leaving ? w[j] : 0.f;
+                bf16x8 zp[2][3];
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    f32x8 v = whole(T[j]);
+#pragma unroll
+                    for (int q = 0; q < 8; q++) v[q] = mul0(v[q], w[q]);
+                    split(v, zp[j]);
                 }
-                const int leaving = last_cut(cut);
-                float wo[8];   // (rows behind the chunk's last step are zeros)
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const float w = pow_add[CH - 1 + L - 1 + rev - 8 * g - j];
-                    wo[j] = 8 * g + j >= leaving ? w : 0.f;
+                for (int i = 0; i < 2 * K; i++) {
+                    bf16x8 y[IN];
+#pragma unroll
+                    for (int u = 0; u < IN; u++) y[u] = column(ly + u * PLANE, PITCH, 8 * g, 32 * (i >> 1) + 4 * (i & 1), r);
+#pragma unroll
+                    for (int j = 0; j < 2; j++) mma(S[i][j], y, zp[j]);
                 }
-                // nothing joins it where an episode starts right behind (before, in time)
-                auto weigh = [&](Op x) {
-                    f32x8 v = M::wide(x);
+                if (slow) {
+                    const unsigned sees = (unsigned)((1ull << L) - 1) & ~(unsigned)((1ull << leaving) - 1);
 #pragma unroll
-                    for (int j = 0; j < 8; j++) v[j] = wo[j] != 0.f ? v[j] * wo[j] : 0.f;
-                    return v;
-                };
-                if (!(cut >> L & 1)) {
-                    if constexpr (WEIGH_Y) {
+                    for (int j = 0; j < 2; j++)
+                        if (odd[j] & sees)
 #pragma unroll
-                        for (int i = 0; i < 2 * KY; i++) {
-                            __builtin_amdgcn_sched_barrier(0);
-                            Op yp[PS];
-                            M::template split<PS>(weigh(M::column(ly, PY, 8 * g, 32 * (i >> 1) + 4 * (i & 1), r)), yp);
+                            for (int i = 0; i < 2 * K; i++)
 #pragma unroll
-                            for (int u = 0; u < PS; u++)
-#pragma unroll
-                                for (int j = 0; j < 2 * KZ; j++) M::mma(S[i][j], yp[u], T[j]);
-                        }
-                    } else {
-                        Op yt[2 * KY];
-#pragma unroll
-                        for (int i = 0; i < 2 * KY; i++) yt[i] = M::column(ly, PY, 8 * g, 32 * (i >> 1) + 4 * (i & 1), r);
-#pragma unroll
-                        for (int j = 0; j < 2 * KZ; j++) {
-                            __builtin_amdgcn_sched_barrier(0);
-                            Op zp[PS];
-                            M::template split<PS>(weigh(T[j]), zp);
-#pragma unroll
-                            for (int u = 0; u < PS; u++)
-#pragma unroll
-                                for (int i = 0; i < 2 * KY; i++) M::mma(S[i][j], yt[i], zp[u]);
-                        }
-                    }
+                                for (int q = 0; q < 4; q++) S[i][j][q] = __builtin_nanf("");
                 }
             }
-            lo = hi;
         }
+        if constexpr (FAST && OUTS) vo.at += vo.hop;
     }
 
     // ---- the steps behind the lane's length
-    if (R.out.p)
-        for (int n = (len > seg0 ? len : seg0) + r; n < seg1; n += 16)
-#pragma unroll
-            for (int k = 0; k < KZ; k++) {
-                const int d = dz0 + 32 * k + 8 * g;
-                if (d < R.dz) {
-                    if (R.out_f32) Num<HUM_F32>::store(R.out.p, ho + (long)n * R.out.step + d, R.dz - d, f32x8{});
-                    else M::store(R.out.p, ho + (long)n * R.out.step + d, R.dz - d, f32x8{});
-                }
-            }
-    if (R.through && l == 0 && dz0 == 0) R.through[item] = passed;
+    if (OUTS && R.out.p && dz0 + 8 * g < dz)
+        for (int n = (len > seg0 ? len : seg0) + r; n < seg1; n += 16) {
+            const int d = dz0 + 8 * g;
+            const long at = head_of(R.out) + (long)n * R.out.step + d;
+            if (R.out_f32) store_some<HUM_F32>(R.out.p, at, dz - d, f32x8{});
+            else store_some<ST>(R.out.p, at, dz - d, f32x8{});
+        }
+    if (R.through && tid == 0) R.through[item] = passed;
     if (R.state_out && (!a.last_only || seg + 1 == a.segs)) {
         float* s = R.state_out + (long)unit * R.out_unit + (long)seg * R.out_seg;
         if constexpr (FAST) {
             const Buf bs = buffer(s, 4 * dy * dz);
-            if (!along_y)
+            turn_state();
 #pragma unroll
-                for (int j = 0; j < 2 * KZ; j++)
+            for (int j = 0; j < 2; j++)
 #pragma unroll
-                    for (int i = 0; i < 2 * KY; i++) S[i][j] = quad_transpose(S[i][j]);
-#pragma unroll
-            for (int j = 0; j < 2 * KZ; j++)
-#pragma unroll
-                for (int i = 0; i < 2 * KY; i++) buf_store4(bs, state_at(i, j), S[i][j]);
+                for (int i = 0; i < 2 * K; i++) buf_store4(bs, state_at(i, j), S[i][j]);
         } else {
 #pragma unroll
-            for (int j = 0; j < 2 * KZ; j++)
+            for (int j = 0; j < 2; j++)
 #pragma unroll
-                for (int i = 0; i < 2 * KY; i++) {
+                for (int i = 0; i < 2 * K; i++) {
                     const int y0 = 32 * (i >> 1) + 8 * g + 4 * (i & 1), z = zc(j);
 #pragma unroll
                     for (int q = 0; q < 4; q++)
-                        if (z < R.dz && y0 + q < R.dy) s[(long)z * R.sz + (long)(y0 + q) * R.sy] = S[i][j][q];
+                        if (z < dz && y0 + q < dy) s[(long)z * R.sz + (long)(y0 + q) * R.sy] = S[i][j][q];
                 }
         }
     }
@@ -828,7 +846,7 @@ int elem_size(int type) { return type == HUM_F32 ? 4 : 2; }
 
 Rows rows_of(const hum_rows& r, int shared, int size, int d) {
     const bool vec = ((uintptr_t)r.ptr | (uintptr_t)(r.lane * size) | (uintptr_t)(r.step * size) | (uintptr_t)(r.head * size)) % 16 == 0 &&
-                     d % 8 == 0 && r.step >= d && r.step < (1l << 31) / (CH * size);
+                     d * size % 16 == 0 && r.step >= d && r.step < (1l << 25) / size;
     return Rows{r.ptr, (long)r.lane, (long)r.step, (long)r.head, shared, vec};
 }
 
@@ -851,50 +869,40 @@ int check_args(const char* fn, const hum_decay_attn_args* p) {
     return HUM_OK;
 }
 
-int y_width(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
-// channels of z per workgroup: 64 for bf16 (P is formed once for them), 32 where float32 matrix instructions take the time
-// and twice the waves shorten it (37 lanes x 203 steps, 6 heads, 40 / 72 channels: 51 us, 76 with 64)
-int z_slice(int type, int d) { return type != HUM_BF16 || d <= 32 ? 32 : 64; }
-
-template <int ST, int DY, int DZ>
-void launch_walk_f(const WalkArgs& a, hipStream_t s) {
+int width_of(const Role& r) {
+    const int d = r.dy > r.dz ? r.dy : r.dz;
+    return d <= 32 ? 32 : d <= 64 ? 64 : 128;
+}
+template <int ST, int D, bool OUTS>
+void launch_walk_o(const WalkArgs& a, hipStream_t s) {
     const long units = (long)a.lanes * a.heads * a.segs;
-    const dim3 grid((unsigned)((units + XCDS * NEAR - 1) / (XCDS * NEAR) * (XCDS * NEAR) * a.parts));
-    bool fast = true;
+    const dim3 grid((unsigned)((units + XCDS * NEAR - 1) / (XCDS * NEAR) * (XCDS * NEAR) * a.nroles));
+    bool fast = !a.reset || (a.reset_step >= 0 && a.reset_step < (1l << 25));
     for (int i = 0; i < a.nroles; i++) {
         const Role& r = a.r[i];
         fast = fast && (!r.x.p || r.x.vec) && r.y.vec && r.z.vec && (!r.out.p || r.out.vec) && r.s_vec;
     }
-    if (fast) hipLaunchKernelGGL((walk_kernel<ST, DY, DZ, true>), grid, dim3(64), 0, s, a);
-    else hipLaunchKernelGGL((walk_kernel<ST, DY, DZ, false>), grid, dim3(64), 0, s, a);
+    if (fast) hipLaunchKernelGGL((walk_kernel<ST, D, true, OUTS>), grid, dim3(2 * D), 0, s, a);
+    else hipLaunchKernelGGL((walk_kernel<ST, D, false, OUTS>), grid, dim3(2 * D), 0, s, a);
 }
-template <int ST, int DY>
-void launch_walk_z(const WalkArgs& a, int dzs, hipStream_t s) {
-    if constexpr (ST == HUM_BF16)
-        if (dzs == 64) {
-            launch_walk_f<ST, DY, 64>(a, s);
-            return;
-        }
-    launch_walk_f<ST, DY, 32>(a, s);
+template <int ST, int D>
+void launch_walk_d(const WalkArgs& a, hipStream_t s) {
+    if (a.r[0].x.p) launch_walk_o<ST, D, true>(a, s);
+    else launch_walk_o<ST, D, false>(a, s);
 }
 template <int ST>
-void launch_walk_y(const WalkArgs& a, int dyw, int dzs, hipStream_t s) {
-    if (dyw == 32) launch_walk_z<ST, 32>(a, dzs, s);
-    else if (dyw == 64) launch_walk_z<ST, 64>(a, dzs, s);
-    else launch_walk_z<ST, 128>(a, dzs, s);
-}
-void launch_walk(int type, const WalkArgs& a, int dyw, int dzs, hipStream_t s) {
-    if (type == HUM_BF16) launch_walk_y<HUM_BF16>(a, dyw, dzs, s);
-    else if (type == HUM_F16) launch_walk_y<HUM_F16>(a, dyw, dzs, s);
-    else launch_walk_y<HUM_F32>(a, dyw, dzs, s);
+void launch_walk_t(const WalkArgs& a, int d, hipStream_t s) {
+    if (d == 32) launch_walk_d<ST, 32>(a, s);
+    else if (d == 64) launch_walk_d<ST, 64>(a, s);
+    else launch_walk_d<ST, 128>(a, s);
 }
 
 // Few lanes and many steps: the walks are cut into segments that run side by side, each from the state that a first pass
 // over the segments before it and a scan have left for it (segments without outputs: half the work of a walk).
 struct Cut { int segs, steps; };
-constexpr int WAVES = 1024, MIN_CHUNKS = 4;   // one wave per SIMD; segments of 4 chunks at least
-Cut cut_of(const hum_decay_attn_args* p, int parts) {
-    const long waves = (long)p->lanes * p->heads * parts;
+constexpr int WAVES = 4096, MIN_CHUNKS = 4;   // four waves per SIMD; segments of 4 chunks at least
+Cut cut_of(const hum_decay_attn_args* p, int each) {   // waves of a (lane, head)
+    const long waves = (long)p->lanes * p->heads * each;
     const int chunks = (p->steps + CH - 1) / CH;
     if (waves == 0 || 2 * waves > WAVES || chunks < 2 * MIN_CHUNKS) return {1, p->steps};
     long segs = WAVES / waves;
@@ -903,33 +911,28 @@ Cut cut_of(const hum_decay_attn_args* p, int parts) {
     return {(chunks + per - 1) / per, per * CH};
 }
 
-// the roles of equal widths share a launch (their workgroups read the same rows at about the same time)
-void launch_roles(const hum_decay_attn_args* p, Role* r, int n, Cut c, bool last_only, hipStream_t s) {
-    bool done[3] = {};
-    for (int i = 0; i < n; i++) {
-        if (done[i]) continue;
-        const int dyw = y_width(r[i].dy), dzs = z_slice(p->type, r[i].dz);
-        WalkArgs a = {};
-        for (int j = i; j < n; j++) {
-            if (done[j] || y_width(r[j].dy) != dyw || z_slice(p->type, r[j].dz) != dzs) continue;
-            done[j] = true;
-            r[j].slice0 = a.parts;
-            a.parts += (r[j].dz + dzs - 1) / dzs;
-            a.r[a.nroles++] = r[j];
-        }
-        a.lanes = p->lanes;
-        a.steps = p->steps;
-        a.heads = p->heads;
-        a.segs = c.segs;
-        a.seg_steps = c.steps;
-        a.last_only = last_only;
-        a.log_decay = p->log_decay;
-        a.reset = p->reset;
-        a.reset_lane = p->reset_lane;
-        a.reset_step = p->reset_step;
-        a.lengths = p->lengths;
-        launch_walk(p->type, a, dyw, dzs, s);
-    }
+// the roles of a call share a launch (their widths differ by their order only): workgroups that read the same rows run at
+// about the same time
+void launch_roles(const hum_decay_attn_args* p, const Role* r, int n, Cut c, bool last_only, hipStream_t s) {
+    if (!n) return;
+    WalkArgs a = {};
+    for (int i = 0; i < n; i++) a.r[i] = r[i];
+    a.nroles = n;
+    a.lanes = p->lanes;
+    a.steps = p->steps;
+    a.heads = p->heads;
+    a.segs = c.segs;
+    a.seg_steps = c.steps;
+    a.last_only = last_only;
+    a.log_decay = p->log_decay;
+    a.reset = p->reset;
+    a.reset_lane = p->reset_lane;
+    a.reset_step = p->reset_step;
+    a.lengths = p->lengths;
+    const int d = width_of(r[0]);
+    if (p->type == HUM_BF16) launch_walk_t<HUM_BF16>(a, d, s);
+    else if (p->type == HUM_F16) launch_walk_t<HUM_F16>(a, d, s);
+    else launch_walk_t<HUM_F32>(a, d, s);
 }
 
 // a state [dv, dk] as the walk's sum over (y channel, z channel): y = keys' side or y = values' side
@@ -973,12 +976,9 @@ void enter_segments(Role& r, const float* scratch, const hum_decay_attn_args* p,
     r.in_unit = (long)p->dk * p->dv * c.segs;
     r.in_seg = (long)p->dk * p->dv;
 }
-int parts_of(const hum_decay_attn_args* p, int dy, int dz) {
-    const int s = z_slice(p->type, dz);
-    return (dz + s - 1) / s;
-}
-Cut forward_cut(const hum_decay_attn_args* p) { return cut_of(p, parts_of(p, p->dk, p->dv)); }
-Cut backward_cut(const hum_decay_attn_args* p) { return cut_of(p, 2 * parts_of(p, p->dv, p->dk) + parts_of(p, p->dk, p->dv)); }
+int waves_of(const hum_decay_attn_args* p) { return ((p->dk > p->dv ? p->dk : p->dv) + 31) / 32; }
+Cut forward_cut(const hum_decay_attn_args* p) { return cut_of(p, waves_of(p)); }
+Cut backward_cut(const hum_decay_attn_args* p) { return cut_of(p, 3 * waves_of(p)); }
 
 int launched(const char* fn) {
     const hipError_t st = hipGetLastError();
