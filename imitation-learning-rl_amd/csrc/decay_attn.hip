@@ -250,17 +250,20 @@ __device__ __forceinline__ f32x4 quad_transpose(f32x4 v) {
     return v;
 }
 
-// waves per SIMD that the registers are limited for
-constexpr int walk_waves(int st, int d) { return st == HUM_BF16 ? (d <= 64 ? 3 : 2) : st == HUM_F32 && d > 64 ? 1 : 2; }
+// waves per SIMD that the registers are limited for (the state takes 16 K of them)
+constexpr int walk_waves(int st, int k, int w) {   // (a single wave has all of a chunk's rows in flight)
+    const bool alone = k > 1 && w == 1;
+    return st == HUM_BF16 ? (k > 2 || alone ? 2 : 3) : st == HUM_F16 ? (k > 2 && alone ? 1 : 2) : k > 2 || alone ? 1 : 2;
+}
 
-// One workgroup per (lane, head), role and segment; D / 32 waves, each with 32 of z's channels and its slice of the state.
-// The waves share the chunk's x and y rows and P.  D: channels rounded up, the larger of y's and z's.  FAST: every operand may
-// be accessed 16 bytes at a time through buffers; else element by element, at any alignment and stride.  OUTS: rows come out
-// (else the states of the segments are wanted only).
-template <int ST, int D, bool FAST, bool OUTS>
-__global__ void __launch_bounds__(2 * D, walk_waves(ST, D)) walk_kernel(WalkArgs a) {
-    constexpr int W = D / 32, K = D / 32;      // waves; operands of 32 channels
+// One workgroup per (lane, head), role and segment; W waves, each with 32 of z's channels and its slice of the state.  The
+// waves share the chunk's x and y rows (K operands of 32 channels) and P.  FAST: every operand may be accessed 16 bytes at a
+// time through buffers; else element by element, at any alignment and stride.  OUTS: rows come out (else the states of the
+// segments are wanted only).
+template <int ST, int K, int W, bool FAST, bool OUTS>
+__global__ void __launch_bounds__(64 * W, walk_waves(ST, K, W)) walk_kernel(WalkArgs a) {
     constexpr int IN = Num<ST>::IN, MID = Num<ST>::MID, SIZE = Num<ST>::SIZE, UNIT = 16 / SIZE;
+    constexpr int D = 32 * K;                  // channels of x and y rounded up
     constexpr int PITCH = D + 8;               // of x and y in LDS: 16-byte reads of 16 rows meet no bank twice
     constexpr int PLANE = CH * PITCH, ZPLANE = CH * 32;
     __shared__ __attribute__((aligned(16))) __bf16 lx[OUTS ? IN * PLANE : 8], ly[IN * PLANE], lz[W][IN * ZPLANE];
@@ -322,7 +325,9 @@ __global__ void __launch_bounds__(2 * D, walk_waves(ST, D)) walk_kernel(WalkArgs
         return v;
     };
     auto chunk = [&](const View& v, int L) { return buffer(rev ? v.at - (long)(L - 1) * v.step : v.at, (L - 1) * v.step + v.row); };
-    constexpr int PER = D / UNIT, PERZ = 32 / UNIT, N = CH * 32 / UNIT / 64;   // units of a row, of a wave's part; of a thread
+    constexpr int PER = D / UNIT, PERZ = 32 / UNIT;   // units of a row, of a wave's part of it
+    constexpr int ROWS = 64 * W / PER, ROWSZ = 64 / PERZ;   // rows of a load
+    constexpr int N = ROWS < CH ? CH / ROWS : 1, NZ = CH / ROWSZ;   // loads of a thread
     View vx = {}, vy = {}, vz = {}, vo = {};
     const int out_size = R.out_f32 ? 4 : SIZE;
     const unsigned char* marks = a.reset ? a.reset + (long)b * a.reset_lane : nullptr;
@@ -337,20 +342,21 @@ __global__ void __launch_bounds__(2 * D, walk_waves(ST, D)) walk_kernel(WalkArgs
         }
         at_mark = marks ? (const char*)marks + (long)time(seg0) * a.reset_step : nullptr;
     }
-    u32x4 rx[OUTS ? N : 1], ry[N], rz[N];
+    u32x4 rx[OUTS ? N : 1], ry[N], rz[NZ];
     int mark = 0;
-    auto fetch = [&](const Rows& m, View& v, int rows, int row, int channel, int d, int n0, int L, u32x4* raw) {
+    auto fetch = [&](const Rows& m, View& v, int rows, int row, int channel, int d, int n0, int L, auto& raw) {
+        constexpr int M = sizeof(raw) / 16;
         if constexpr (FAST) {
             const Buf bm = chunk(v, L);
             const int base = rev ? (L - 1) * v.step : 0;
 #pragma unroll
-            for (int u = 0; u < N; u++) raw[u] = buf_load(bm, v.off + (base + dir * u * rows * v.step));
+            for (int u = 0; u < M; u++) raw[u] = buf_load(bm, v.off + (base + dir * u * rows * v.step));
             v.at += v.hop;
         } else {
             typedef typename Num<ST>::T E;
             typedef E EU __attribute__((ext_vector_type(UNIT)));
 #pragma unroll
-            for (int u = 0; u < N; u++) {
+            for (int u = 0; u < M; u++) {
                 const int n = u * rows + row;
                 const E* e = (const E*)m.p + head_of(m) + (long)time(n0 + n) * m.step + channel;
                 EU x = {};
@@ -363,9 +369,9 @@ __global__ void __launch_bounds__(2 * D, walk_waves(ST, D)) walk_kernel(WalkArgs
     };
     auto load_rows = [&](int n0) {
         const int L = end - n0 < CH ? end - n0 : CH;
-        if constexpr (OUTS) fetch(R.x, vx, 64 * W / PER, tid / PER, tid % PER * UNIT, dy, n0, L, rx);
-        fetch(R.y, vy, 64 * W / PER, tid / PER, tid % PER * UNIT, dy, n0, L, ry);
-        fetch(R.z, vz, 64 / PERZ, l / PERZ, dz0 + l % PERZ * UNIT, dz, n0, L, rz);
+        if constexpr (OUTS) fetch(R.x, vx, ROWS, tid / PER, tid % PER * UNIT, dy, n0, L, rx);
+        fetch(R.y, vy, ROWS, tid / PER, tid % PER * UNIT, dy, n0, L, ry);
+        fetch(R.z, vz, ROWSZ, l / PERZ, dz0 + l % PERZ * UNIT, dz, n0, L, rz);
         // lane j has the mark that separates the chunk's walk steps j - 1 and j (0: from the entering state, L: from the
         // leaving one).  An episode's first step is cut off from what time puts before it, so the backward walk has it one
         // later.
@@ -378,9 +384,11 @@ __global__ void __launch_bounds__(2 * D, walk_waves(ST, D)) walk_kernel(WalkArgs
             mark = n >= 0 && n < L ? marks[(long)time(n0 + n) * a.reset_step] : 0;
         }
     };
-    auto lay = [&](__bf16* m, int pitch, int plane, int rows, int row, int channel, const u32x4* raw) {
+    auto lay = [&](__bf16* m, int pitch, int plane, int rows, int row, int channel, const auto& raw) {
+        constexpr int M = sizeof(raw) / 16;
 #pragma unroll
-        for (int u = 0; u < N; u++) put<ST>(m + (u * rows + row) * pitch + channel, plane, raw[u]);
+        for (int u = 0; u < M; u++)
+            if (u * rows + row < CH) put<ST>(m + (u * rows + row) * pitch + channel, plane, raw[u]);
     };
     if (seg0 < end) load_rows(seg0);
 
@@ -426,6 +434,9 @@ __global__ void __launch_bounds__(2 * D, walk_waves(ST, D)) walk_kernel(WalkArgs
 #pragma unroll
     for (int c = 0; c < 2; c++) w_in[c] = R.s_in * power(16 * c + r + 1 - rev);
     float passed = 1.f;   // what is left of the entering state
+    // everything loaded so far (vmcnt 0): else each use of the state in the loop would wait for the next chunk's rows too,
+    // which the compiler cannot tell from the state's own loads
+    __builtin_amdgcn_s_waitcnt(0x0f70);
 
     for (int n0 = seg0; n0 < end; n0 += CH) {
         const int L = end - n0 < CH ? end - n0 : CH;
@@ -434,7 +445,7 @@ __global__ void __launch_bounds__(2 * D, walk_waves(ST, D)) walk_kernel(WalkArgs
         const unsigned long long cut = __ballot(mark != 0) & ((2ull << (L - 1 + rev)) - 1) & ~(unsigned long long)rev;
         unsigned bad = 0;
 #pragma unroll
-        for (int u = 0; u < N; u++) bad |= odd_bits<ST>(rz[u]);
+        for (int u = 0; u < NZ; u++) bad |= odd_bits<ST>(rz[u]);
         const bool slow = __any(bad != 0);
         // the last cut at or before step n of the chunk: step n sees the steps from there on, and what entered the chunk only
         // if there is none
@@ -443,9 +454,9 @@ __global__ void __launch_bounds__(2 * D, walk_waves(ST, D)) walk_kernel(WalkArgs
         const int leaving = last_cut(cut);   // what leaves the chunk is of the steps from here on
 
         lds_barrier<W>();   // the chunk before has been read
-        if constexpr (OUTS) lay(lx, PITCH, PLANE, 64 * W / PER, tid / PER, tid % PER * UNIT, rx);
-        lay(ly, PITCH, PLANE, 64 * W / PER, tid / PER, tid % PER * UNIT, ry);
-        lay(lz[wave], 32, ZPLANE, 64 / PERZ, l / PERZ, l % PERZ * UNIT, rz);
+        if constexpr (OUTS) lay(lx, PITCH, PLANE, ROWS, tid / PER, tid % PER * UNIT, rx);
+        lay(ly, PITCH, PLANE, ROWS, tid / PER, tid % PER * UNIT, ry);
+        lay(lz[wave], 32, ZPLANE, ROWSZ, l / PERZ, l % PERZ * UNIT, rz);
         lds_barrier<W>();
         if (more) load_rows(n0 + CH);   // the chunk is in LDS: the registers take the next one's rows
         auto read = [&](const __bf16* m, int row, int k, bf16x8 (&o)[IN]) {
@@ -660,51 +671,60 @@ __global__ void __launch_bounds__(2 * D, walk_waves(ST, D)) walk_kernel(WalkArgs
     }
 }
 
-// the segments' entering states from what each of them adds: seg[g] <- state before segment g, one thread per N elements
-template <int N>
-__global__ void __launch_bounds__(256) scan_kernel(const float* in, float* seg, const float* through, int segs, long units, int size) {
-    typedef float V __attribute__((ext_vector_type(N)));
-    const long e = ((long)blockIdx.x * 256 + threadIdx.x) * N;
-    if (e >= units * size) return;
-    const long unit = e / size;
-    const int at = (int)(e - unit * size);
-    V cur = {};
-    if (in) cur = *(const V*)(in + e);
-    float* s = seg + unit * segs * size + at;
-    const float* th = through + unit * segs;
-    constexpr int AHEAD = 8;   // loads in flight
+// the segments' entering states from what each of them adds: seg[g] <- state before segment g, one thread per element of
+// walk blockIdx.y.  A recurrence over the segments that only their loads' latency bounds: AHEAD of them are in flight
+// (64 segments of 8 heads x 128 x 128: 22 us with 8 of 16 bytes each)
+struct ScanArgs {
+    struct { const float* in; float* seg; const float* through; } w[2];
+    int segs, size;
+    long units;
+};
+__global__ void __launch_bounds__(256) scan_kernel(ScanArgs a) {
+    constexpr int AHEAD = 32;
+    const long e = (long)blockIdx.x * 256 + threadIdx.x;
+    if (e >= a.units * a.size) return;
+    const auto& w = a.w[blockIdx.y];
+    const int segs = a.segs;
+    const long unit = e / a.size, size = a.size;
+    float cur = w.in ? w.in[e] : 0.f;
+    float* s = w.seg + unit * segs * size + (e - unit * size);
+    const float* th = w.through + unit * segs;
     for (int g0 = 0; g0 < segs; g0 += AHEAD) {
-        V add[AHEAD];
+        float add[AHEAD], t[AHEAD];
 #pragma unroll
-        for (int i = 0; i < AHEAD; i++)
-            if (g0 + i + 1 < segs) add[i] = *(const V*)(s + (long)(g0 + i) * size);
+        for (int i = 0; i < AHEAD; i++) {   // (the last segment's own is not needed)
+            const int g = g0 + i < segs ? g0 + i : segs - 1;
+            add[i] = s[g * size];
+            t[i] = th[g];
+        }
 #pragma unroll
         for (int i = 0; i < AHEAD; i++)
             if (g0 + i < segs) {
-                *(V*)(s + (long)(g0 + i) * size) = cur;
-                if (g0 + i + 1 < segs) {
-                    const float t = th[g0 + i];
-                    cur = t != 0.f ? cur * t + add[i] : add[i];   // behind a cut nothing of the old state is left
-                }
+                s[(g0 + i) * size] = cur;
+                cur = mul0(cur, t[i]) + add[i];   // behind a cut (t 0) nothing of the old state is left
             }
     }
 }
 
-// gradients of keys and values that `group` heads share: the sum of the heads' float32 partial results
+// gradients of keys (blockIdx.y 0) and values (1) that `group` heads share: the sum of the heads' float32 partial results
 // part [lanes, steps, heads, d] -> out [lanes, steps, heads / group, d]; one thread per output channel
+struct ShareArgs {
+    struct { const float* part; Rows out; int d; } x[2];
+    long rows;
+    int steps, kv, group;
+};
 template <int ST>
-__global__ void __launch_bounds__(256) share_kernel(const float* part, Rows out, long rows, int steps, int kv, int group, int d) {
-    for (long e = (long)blockIdx.x * 256 + threadIdx.x; e < rows * kv * d; e += (long)gridDim.x * 256) {
-        const int c = (int)(e % d);
-        const long row = e / d;          // (lane, step, kv head)
-        const int g = (int)(row % kv);
-        const long bt = row / kv;
+__global__ void __launch_bounds__(256) share_kernel(ShareArgs a) {
+    const auto& x = a.x[blockIdx.y];
+    const int d = x.d, kv = a.kv, group = a.group;
+    if (!x.out.p) return;
+    for (long e = (long)blockIdx.x * 256 + threadIdx.x; e < a.rows * kv * d; e += (long)gridDim.x * 256) {
+        const long row = e / d, bt = row / kv;   // (lane, step, kv head), (lane, step)
+        const int c = (int)(e - row * d), g = (int)(row - bt * kv);
         float s = 0.f;
-        for (int i = 0; i < group; i++) s += part[((bt * kv + g) * group + i) * d + c];
-        const long at = bt / steps * out.lane + bt % steps * out.step + (long)g * out.head + c;
-        if constexpr (ST == HUM_F32) ((float*)out.p)[at] = s;
-        else if constexpr (ST == HUM_BF16) ((__bf16*)out.p)[at] = (__bf16)s;
-        else ((_Float16*)out.p)[at] = (_Float16)s;
+        for (int i = 0; i < group; i++) s += x.part[((bt * kv + g) * group + i) * d + c];
+        const long at = bt / a.steps * x.out.lane + bt % a.steps * x.out.step + (long)g * x.out.head + c;
+        ((typename Num<ST>::T*)x.out.p)[at] = (typename Num<ST>::T)s;
     }
 }
 
@@ -869,32 +889,37 @@ int check_args(const char* fn, const hum_decay_attn_args* p) {
     return HUM_OK;
 }
 
-int width_of(const Role& r) {
-    const int d = r.dy > r.dz ? r.dy : r.dz;
-    return d <= 32 ? 32 : d <= 64 ? 64 : 128;
-}
-template <int ST, int D, bool OUTS>
-void launch_walk_o(const WalkArgs& a, hipStream_t s) {
+int in_32(int d) { return d <= 32 ? 1 : d <= 64 ? 2 : 4; }
+template <int ST, int K, int W, bool OUTS>
+void launch_walk_o(const WalkArgs& a, bool fast, hipStream_t s) {
     const long units = (long)a.lanes * a.heads * a.segs;
     const dim3 grid((unsigned)((units + XCDS * NEAR - 1) / (XCDS * NEAR) * (XCDS * NEAR) * a.nroles));
+    if (fast) hipLaunchKernelGGL((walk_kernel<ST, K, W, true, OUTS>), grid, dim3(64 * W), 0, s, a);
+    else if constexpr (K == W) hipLaunchKernelGGL((walk_kernel<ST, K, W, false, OUTS>), grid, dim3(64 * W), 0, s, a);
+}
+template <int ST, int K, int W>
+void launch_walk_w(const WalkArgs& a, bool fast, hipStream_t s) {
+    if (a.r[0].x.p) launch_walk_o<ST, K, W, true>(a, fast, s);
+    else launch_walk_o<ST, K, W, false>(a, fast, s);
+}
+template <int ST, int K>
+void launch_walk_k(const WalkArgs& a, int w, bool fast, hipStream_t s) {
+    if (w == 1) launch_walk_w<ST, K, 1>(a, fast, s);
+    else if (w == 2) launch_walk_w<ST, K, 2>(a, fast, s);
+    else launch_walk_w<ST, K, 4>(a, fast, s);
+}
+template <int ST>
+void launch_walk_t(const WalkArgs& a, hipStream_t s) {
     bool fast = !a.reset || (a.reset_step >= 0 && a.reset_step < (1l << 25));
     for (int i = 0; i < a.nroles; i++) {
         const Role& r = a.r[i];
         fast = fast && (!r.x.p || r.x.vec) && r.y.vec && r.z.vec && (!r.out.p || r.out.vec) && r.s_vec;
     }
-    if (fast) hipLaunchKernelGGL((walk_kernel<ST, D, true, OUTS>), grid, dim3(2 * D), 0, s, a);
-    else hipLaunchKernelGGL((walk_kernel<ST, D, false, OUTS>), grid, dim3(2 * D), 0, s, a);
-}
-template <int ST, int D>
-void launch_walk_d(const WalkArgs& a, hipStream_t s) {
-    if (a.r[0].x.p) launch_walk_o<ST, D, true>(a, s);
-    else launch_walk_o<ST, D, false>(a, s);
-}
-template <int ST>
-void launch_walk_t(const WalkArgs& a, int d, hipStream_t s) {
-    if (d == 32) launch_walk_d<ST, 32>(a, s);
-    else if (d == 64) launch_walk_d<ST, 64>(a, s);
-    else launch_walk_d<ST, 128>(a, s);
+    int k = in_32(a.r[0].dy), w = in_32(a.r[0].dz);
+    if (!fast) k = w = k > w ? k : w;   // (that form is built for squares only)
+    if (k == 1) launch_walk_k<ST, 1>(a, w, fast, s);
+    else if (k == 2) launch_walk_k<ST, 2>(a, w, fast, s);
+    else launch_walk_k<ST, 4>(a, w, fast, s);
 }
 
 // Few lanes and many steps: the walks are cut into segments that run side by side, each from the state that a first pass
@@ -911,13 +936,9 @@ Cut cut_of(const hum_decay_attn_args* p, int each) {   // waves of a (lane, head
     return {(chunks + per - 1) / per, per * CH};
 }
 
-// the roles of a call share a launch (their widths differ by their order only): workgroups that read the same rows run at
-// about the same time
+// roles of equal widths share a launch: workgroups that read the same rows run at about the same time
 void launch_roles(const hum_decay_attn_args* p, const Role* r, int n, Cut c, bool last_only, hipStream_t s) {
-    if (!n) return;
     WalkArgs a = {};
-    for (int i = 0; i < n; i++) a.r[i] = r[i];
-    a.nroles = n;
     a.lanes = p->lanes;
     a.steps = p->steps;
     a.heads = p->heads;
@@ -929,10 +950,19 @@ void launch_roles(const hum_decay_attn_args* p, const Role* r, int n, Cut c, boo
     a.reset_lane = p->reset_lane;
     a.reset_step = p->reset_step;
     a.lengths = p->lengths;
-    const int d = width_of(r[0]);
-    if (p->type == HUM_BF16) launch_walk_t<HUM_BF16>(a, d, s);
-    else if (p->type == HUM_F16) launch_walk_t<HUM_F16>(a, d, s);
-    else launch_walk_t<HUM_F32>(a, d, s);
+    bool done[3] = {};
+    for (int i = 0; i < n; i++) {
+        if (done[i]) continue;
+        a.nroles = 0;
+        for (int j = i; j < n; j++)
+            if (!done[j] && in_32(r[j].dy) == in_32(r[i].dy) && in_32(r[j].dz) == in_32(r[i].dz)) {
+                done[j] = true;
+                a.r[a.nroles++] = r[j];
+            }
+        if (p->type == HUM_BF16) launch_walk_t<HUM_BF16>(a, s);
+        else if (p->type == HUM_F16) launch_walk_t<HUM_F16>(a, s);
+        else launch_walk_t<HUM_F32>(a, s);
+    }
 }
 
 // a state [dv, dk] as the walk's sum over (y channel, z channel): y = keys' side or y = values' side
@@ -951,34 +981,38 @@ uint64_t walk_bytes(const hum_decay_attn_args* p, Cut c) {
     const uint64_t units = (uint64_t)p->lanes * p->heads * c.segs;
     return c.segs > 1 ? round16(4 * units * p->dk * p->dv) + round16(4 * units) : 0;
 }
-// fills the scratch with the segments' entering states: `walk` is a role whose y side is the keys' (or queries')
-void run_segments(const hum_decay_attn_args* p, Role walk, float* scratch, Cut c, hipStream_t s) {
+// fills the scratch of each walk (n of them) with its segments' entering states; a walk is a role whose y side is the keys'
+void run_segments(const hum_decay_attn_args* p, Role* walk, float* const* scratch, int n, Cut c, hipStream_t s) {
     const long units = (long)p->lanes * p->heads, size = (long)p->dk * p->dv;
-    float* through = (float*)((char*)scratch + round16(4 * units * c.segs * size));
-    const float* in = walk.state_in;
-    walk.x = Rows{};
-    walk.out = Rows{};
-    walk.x.shared = walk.out.shared = 1;
-    walk.state_in = nullptr;
-    walk.state_out = scratch;
-    walk.out_unit = size * c.segs;
-    walk.out_seg = size;
-    walk.through = through;
-    walk.s_vec = p->dk % 4 == 0;
-    launch_roles(p, &walk, 1, c, false, s);
-    if (size % 4 == 0 && (uintptr_t)in % 16 == 0)
-        hipLaunchKernelGGL(scan_kernel<4>, dim3((unsigned)((units * size / 4 + 255) / 256)), dim3(256), 0, s, in, scratch, through, c.segs, units, (int)size);
-    else
-        hipLaunchKernelGGL(scan_kernel<1>, dim3((unsigned)((units * size + 255) / 256)), dim3(256), 0, s, in, scratch, through, c.segs, units, (int)size);
+    ScanArgs a = {};
+    a.segs = c.segs;
+    a.size = (int)size;
+    a.units = units;
+    for (int i = 0; i < n; i++) {
+        Role& w = walk[i];
+        float* through = (float*)((char*)scratch[i] + round16(4 * units * c.segs * size));
+        a.w[i].in = w.state_in;
+        a.w[i].seg = scratch[i];
+        a.w[i].through = through;
+        w.x = w.out = Rows{};
+        w.x.shared = w.out.shared = 1;
+        w.state_in = nullptr;
+        w.state_out = scratch[i];
+        w.out_unit = size * c.segs;
+        w.out_seg = size;
+        w.through = through;
+        w.s_vec = p->dk % 4 == 0;
+    }
+    launch_roles(p, walk, n, c, false, s);
+    hipLaunchKernelGGL(scan_kernel, dim3((unsigned)((units * size + 255) / 256), n), dim3(256), 0, s, a);
 }
 void enter_segments(Role& r, const float* scratch, const hum_decay_attn_args* p, Cut c) {
     r.state_in = scratch;
     r.in_unit = (long)p->dk * p->dv * c.segs;
     r.in_seg = (long)p->dk * p->dv;
 }
-int waves_of(const hum_decay_attn_args* p) { return ((p->dk > p->dv ? p->dk : p->dv) + 31) / 32; }
-Cut forward_cut(const hum_decay_attn_args* p) { return cut_of(p, waves_of(p)); }
-Cut backward_cut(const hum_decay_attn_args* p) { return cut_of(p, 3 * waves_of(p)); }
+Cut forward_cut(const hum_decay_attn_args* p) { return cut_of(p, in_32(p->dv)); }
+Cut backward_cut(const hum_decay_attn_args* p) { return cut_of(p, 2 * in_32(p->dk) + in_32(p->dv)); }
 
 int launched(const char* fn) {
     const hipError_t st = hipGetLastError();
@@ -1024,7 +1058,9 @@ int hum_decay_attn(const hum_decay_attn_args* p, const hum_rows* out, void* work
     role_state(r, p->state_in, p->state_out, p, true);
     const Cut c = forward_cut(p);
     if (c.segs > 1) {
-        run_segments(p, r, (float*)workspace, c, (hipStream_t)stream);
+        Role w = r;
+        float* const at = (float*)workspace;
+        run_segments(p, &w, &at, 1, c, (hipStream_t)stream);
         enter_segments(r, (const float*)workspace, p, c);
     }
     launch_roles(p, &r, 1, c, true, (hipStream_t)stream);
@@ -1103,38 +1139,43 @@ int hum_decay_attn_backward(const hum_decay_attn_args* p, const hum_rows* d_out,
         role_state(w, d_state_out, d_state_in, p, true);
     }
     if (c.segs > 1) {
-        Role w = {};
+        Role w[2];
+        float* at[2];
+        int m = 0;
         if (gq.ptr) {
-            w.y = k; w.z = v;
-            w.dy = p->dk; w.dz = p->dv;
-            w.s_add = 1.f;
-            role_state(w, p->state_in, nullptr, p, true);
-            run_segments(p, w, seg_s, c, s);
+            Role& x = w[m] = Role{};
+            at[m++] = seg_s;
+            x.y = k; x.z = v;
+            x.dy = p->dk; x.dz = p->dv;
+            x.s_add = 1.f;
+            role_state(x, p->state_in, nullptr, p, true);
         }
         if (gk.ptr || gv.ptr || d_state_in) {
-            w = Role{};
-            w.y = q; w.z = g;
-            w.dy = p->dk; w.dz = p->dv;
-            w.rev = 1;
-            w.s_add = p->scale;
-            role_state(w, d_state_out, nullptr, p, true);
-            run_segments(p, w, seg_r, c, s);
+            Role& x = w[m] = Role{};
+            at[m++] = seg_r;
+            x.y = q; x.z = g;
+            x.dy = p->dk; x.dz = p->dv;
+            x.rev = 1;
+            x.s_add = p->scale;
+            role_state(x, d_state_out, nullptr, p, true);
         }
+        if (m) run_segments(p, w, at, m, c, s);
         for (int i = 0; i < n; i++) enter_segments(r[i], r[i].rev ? seg_r : seg_s, p, c);
     }
     launch_roles(p, r, n, c, true, s);
-    if (group > 1 && p->steps) {
-        const long rows = (long)p->lanes * p->steps;
-        struct { const hum_rows* o; const float* part; int d; } sums[2] = {{&gk, part_k, p->dk}, {&gv, part_v, p->dv}};
-        for (auto& x : sums) {
-            if (!x.o->ptr) continue;
-            const Rows o = rows_of(*x.o, 1, size, x.d);
-            const long blocks = (rows * p->kv_heads * x.d + 255) / 256;
-            const dim3 grid((unsigned)(blocks < (1 << 16) ? blocks : (1 << 16)));
-            if (p->type == HUM_F32) hipLaunchKernelGGL(share_kernel<HUM_F32>, grid, dim3(256), 0, s, x.part, o, rows, p->steps, p->kv_heads, group, x.d);
-            else if (p->type == HUM_BF16) hipLaunchKernelGGL(share_kernel<HUM_BF16>, grid, dim3(256), 0, s, x.part, o, rows, p->steps, p->kv_heads, group, x.d);
-            else hipLaunchKernelGGL(share_kernel<HUM_F16>, grid, dim3(256), 0, s, x.part, o, rows, p->steps, p->kv_heads, group, x.d);
-        }
+    if (group > 1 && p->steps && (gk.ptr || gv.ptr)) {
+        ShareArgs a = {};
+        a.rows = (long)p->lanes * p->steps;
+        a.steps = p->steps;
+        a.kv = p->kv_heads;
+        a.group = group;
+        a.x[0] = {part_k, rows_of(gk, 1, size, p->dk), p->dk};
+        a.x[1] = {part_v, rows_of(gv, 1, size, p->dv), p->dv};
+        const long blocks = (a.rows * a.kv * (p->dk > p->dv ? p->dk : p->dv) + 255) / 256;
+        const dim3 grid((unsigned)(blocks < (1 << 16) ? blocks : (1 << 16)), 2);
+        if (p->type == HUM_F32) hipLaunchKernelGGL(share_kernel<HUM_F32>, grid, dim3(256), 0, s, a);
+        else if (p->type == HUM_BF16) hipLaunchKernelGGL(share_kernel<HUM_BF16>, grid, dim3(256), 0, s, a);
+        else hipLaunchKernelGGL(share_kernel<HUM_F16>, grid, dim3(256), 0, s, a);
     }
     return launched(fn);
 }
