@@ -189,15 +189,13 @@ __device__ __forceinline__ void put(__bf16* m, int plane, u32x4 raw) {
         }
     }
 }
-// sign bits of the result: whether an element's exponent is all ones
-template <int ST>
-__device__ __forceinline__ unsigned odd_bits(u32x4 u) {
-    constexpr unsigned exponent = ST == HUM_BF16 ? 0x7f807f80u : ST == HUM_F16 ? 0x7c007c00u : 0x7f800000u;
-    constexpr unsigned one = ST == HUM_BF16 ? 0x00800080u : ST == HUM_F16 ? 0x04000400u : 0x00800000u;
+// not 0 where one of 8 values (the first of their parts) is not finite: its exponent is all ones
+__device__ __forceinline__ unsigned odd_bits(bf16x8 v) {
+    const u32x4 u = __builtin_bit_cast(u32x4, v);
     unsigned bad = 0;
 #pragma unroll
-    for (int i = 0; i < 4; i++) bad |= (u[i] & exponent) + one;
-    return bad & (ST == HUM_F32 ? 0x80000000u : 0x80008000u);
+    for (int i = 0; i < 4; i++) bad |= (u[i] & 0x7f807f80u) + 0x00800080u;
+    return bad & 0x80008000u;
 }
 // 8 channels of a row, rounded once; bytes `second` on are the upper half of a float32 row's
 template <int ST>
@@ -325,8 +323,8 @@ __global__ void __launch_bounds__(64 * W, walk_waves(ST, K, W)) walk_kernel(Walk
         return v;
     };
     auto chunk = [&](const View& v, int L) { return buffer(rev ? v.at - (long)(L - 1) * v.step : v.at, (L - 1) * v.step + v.row); };
-    constexpr int PER = D / UNIT, PERZ = 32 / UNIT;   // units of a row, of a wave's part of it
-    constexpr int ROWS = 64 * W / PER, ROWSZ = 64 / PERZ;   // rows of a load
+    constexpr int PER = D / UNIT, PERZ = 32 * W / UNIT;     // units of a row of x and y, of z
+    constexpr int ROWS = 64 * W / PER, ROWSZ = 64 * W / PERZ;   // rows of a load
     constexpr int N = ROWS < CH ? CH / ROWS : 1, NZ = CH / ROWSZ;   // loads of a thread
     View vx = {}, vy = {}, vz = {}, vo = {};
     const int out_size = R.out_f32 ? 4 : SIZE;
@@ -335,7 +333,7 @@ __global__ void __launch_bounds__(64 * W, walk_waves(ST, K, W)) walk_kernel(Walk
     const int mark_step = (int)a.reset_step, mark_off = (rev ? 1 - l : l) * mark_step;
     if constexpr (FAST) {
         vy = view(R.y, SIZE, dy, tid / PER, tid % PER * UNIT);
-        vz = view(R.z, SIZE, dz, l / PERZ, dz0 + l % PERZ * UNIT);
+        vz = view(R.z, SIZE, dz, tid / PERZ, tid % PERZ * UNIT);
         if constexpr (OUTS) {
             vx = view(R.x, SIZE, dy, tid / PER, tid % PER * UNIT);
             vo = view(R.out, out_size, dz, r, dz0 + 8 * g);
@@ -371,7 +369,7 @@ __global__ void __launch_bounds__(64 * W, walk_waves(ST, K, W)) walk_kernel(Walk
         const int L = end - n0 < CH ? end - n0 : CH;
         if constexpr (OUTS) fetch(R.x, vx, ROWS, tid / PER, tid % PER * UNIT, dy, n0, L, rx);
         fetch(R.y, vy, ROWS, tid / PER, tid % PER * UNIT, dy, n0, L, ry);
-        fetch(R.z, vz, ROWSZ, l / PERZ, dz0 + l % PERZ * UNIT, dz, n0, L, rz);
+        fetch(R.z, vz, ROWSZ, tid / PERZ, tid % PERZ * UNIT, dz, n0, L, rz);
         // lane j has the mark that separates the chunk's walk steps j - 1 and j (0: from the entering state, L: from the
         // leaving one).  An episode's first step is cut off from what time puts before it, so the backward walk has it one
         // later.
@@ -443,10 +441,6 @@ __global__ void __launch_bounds__(64 * W, walk_waves(ST, K, W)) walk_kernel(Walk
         const bool more = n0 + CH < end;
         // a mark behind the chunk's last step (lane L's, walking backwards) is this chunk's as well as the next one's first
         const unsigned long long cut = __ballot(mark != 0) & ((2ull << (L - 1 + rev)) - 1) & ~(unsigned long long)rev;
-        unsigned bad = 0;
-#pragma unroll
-        for (int u = 0; u < NZ; u++) bad |= odd_bits<ST>(rz[u]);
-        const bool slow = __any(bad != 0);
         // the last cut at or before step n of the chunk: step n sees the steps from there on, and what entered the chunk only
         // if there is none
         auto cuts_to = [&](int n) { return cut & ((2ull << n) - 1); };
@@ -456,7 +450,8 @@ __global__ void __launch_bounds__(64 * W, walk_waves(ST, K, W)) walk_kernel(Walk
         lds_barrier<W>();   // the chunk before has been read
         if constexpr (OUTS) lay(lx, PITCH, PLANE, ROWS, tid / PER, tid % PER * UNIT, rx);
         lay(ly, PITCH, PLANE, ROWS, tid / PER, tid % PER * UNIT, ry);
-        lay(lz[wave], 32, ZPLANE, ROWSZ, l / PERZ, l % PERZ * UNIT, rz);
+        // (each wave's channels of z have a tile of their own)
+        lay(lz[tid % PERZ * UNIT / 32], 32, ZPLANE, ROWSZ, tid / PERZ, tid % PERZ * UNIT % 32, rz);
         lds_barrier<W>();
         if (more) load_rows(n0 + CH);   // the chunk is in LDS: the registers take the next one's rows
         auto read = [&](const __bf16* m, int row, int k, bf16x8 (&o)[IN]) {
@@ -519,6 +514,7 @@ __global__ void __launch_bounds__(64 * W, walk_waves(ST, K, W)) walk_kernel(Walk
             // z values that are not finite: zeros to the products, and NaN to what sees them.  The steps at which a channel
             // has some go to odd[channel]
             unsigned odd[2] = {0, 0};
+            const bool slow = __any((odd_bits(T[0][0]) | odd_bits(T[1][0])) != 0);
             if (slow) {
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
