@@ -251,38 +251,46 @@ __device__ __forceinline__ f32x4 quad_transpose(f32x4 v) {
 // waves per SIMD that the registers are limited for (the state takes 16 K of them)
 constexpr int walk_waves(int st, int k, int w) {   // (a single wave has all of a chunk's rows in flight)
     const bool alone = k > 1 && w == 1;
-    return st == HUM_BF16 ? (k > 2 || alone ? 2 : 3) : st == HUM_F16 ? (k > 2 && alone ? 1 : 2) : k > 2 || alone ? 1 : 2;
+    return st == HUM_BF16 ? (k > 2 && alone ? 1 : k > 2 || alone ? 2 : 3) : st == HUM_F16 ? (k > 2 && alone ? 1 : 2) : k > 2 || alone ? 1 : 2;
 }
 
-// One workgroup per (lane, head), role and segment; W waves, each with 32 of z's channels and its slice of the state.  The
-// waves share the chunk's x and y rows (K operands of 32 channels) and P.  FAST: every operand may be accessed 16 bytes at a
+// One workgroup per HEADS neighbouring heads of a lane, role and segment; W waves per head, each with 32 of z's channels and
+// its slice of the state.  A head's waves share the chunk's x and y rows (K operands of 32 channels) and P; the heads of a
+// workgroup only share the loading, so that a load meets long pieces of few rows (with one head, 4096 lanes' time-major
+// steps lie 2 MB apart and each load meets 8 pages for 1 KB: forward 177 us, 168 us with the heads together).  FAST: every operand may be accessed 16 bytes at a
 // time through buffers; else element by element, at any alignment and stride.  OUTS: rows come out (else the states of the
 // segments are wanted only).
-template <int ST, int K, int W, bool FAST, bool OUTS>
-__global__ void __launch_bounds__(64 * W, walk_waves(ST, K, W)) walk_kernel(WalkArgs a) {
+template <int ST, int K, int W, int HEADS, bool FAST, bool OUTS>
+__global__ void __launch_bounds__(64 * W * HEADS, walk_waves(ST, K, W)) walk_kernel(WalkArgs a) {
     constexpr int IN = Num<ST>::IN, MID = Num<ST>::MID, SIZE = Num<ST>::SIZE, UNIT = 16 / SIZE;
     constexpr int D = 32 * K;                  // channels of x and y rounded up
     constexpr int PITCH = D + 8;               // of x and y in LDS: 16-byte reads of 16 rows meet no bank twice
     constexpr int PLANE = CH * PITCH, ZPLANE = CH * 32;
-    __shared__ __attribute__((aligned(16))) __bf16 lx[OUTS ? IN * PLANE : 8], ly[IN * PLANE], lz[W][IN * ZPLANE];
-    __shared__ __attribute__((aligned(16))) bf16x8 lp[OUTS ? 2 : 1][MID][64];
+    constexpr int T = 64 * W * HEADS, B = W * HEADS;   // threads, waves
+    __shared__ __attribute__((aligned(16))) __bf16 tx[HEADS][OUTS ? IN * PLANE : 8], ty[HEADS][IN * PLANE], tz[HEADS][W][IN * ZPLANE];
+    __shared__ __attribute__((aligned(16))) bf16x8 tp[HEADS][OUTS ? 2 : 1][MID][64];
     // lambda^d times the scale's part for d = -31 .. 32 steps, zeros for d < 0: between two steps of a chunk, and from a
     // step to the chunk's end
-    __shared__ float pow_pair[2 * CH], pow_add[2 * CH];
-    __shared__ unsigned lodd[W][32];
+    __shared__ float pows_pair[HEADS][2 * CH], pows_add[HEADS][2 * CH];
+    __shared__ unsigned odds[HEADS][W][32];
 
     const int tid = threadIdx.x, l = tid & 63, g = l >> 4, r = l & 15;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int sub = HEADS > 1 ? __builtin_amdgcn_readfirstlane(tid / (64 * W)) : 0;   // the wave's head of the workgroup's
+    const int wave = __builtin_amdgcn_readfirstlane(tid / 64 % W);                     // and its channels of z
+    __bf16 *const lx = tx[sub], *const ly = ty[sub], *const lz = tz[sub][wave];
+    bf16x8(*const lp)[MID][64] = tp[sub];
+    float *const pow_pair = pows_pair[sub], *const pow_add = pows_add[sub];
+    unsigned* const lodd = odds[sub][wave];
     // the roles of one segment read the same rows, and NEAR segments in a row are neighbours in memory (the heads of a lane,
     // lanes of a time-major step): they go to one XCD, one after the other.  Gradient of 4096 lanes x 32 steps: 380 us,
     // 407 with NEAR = 1, 377 with 32 (which leaves XCDs idle at few lanes)
     const int block = blockIdx.x, ri = block / XCDS % a.nroles, turn = block / (XCDS * a.nroles);
     const int item = (turn / NEAR * XCDS + block % XCDS) * NEAR + turn % NEAR;
-    if (item >= a.lanes * a.heads * a.segs) return;
-    const int unit = item / a.segs, seg = item - unit * a.segs;
+    if (item >= a.lanes * a.heads / HEADS * a.segs) return;
+    const int group = item / a.segs, seg = item - group * a.segs;
     const Role& R = a.r[ri];
     const int dz0 = 32 * wave;
-    const int b = unit / a.heads, h = unit - b * a.heads;
+    const int b = group * HEADS / a.heads, h0 = group * HEADS - b * a.heads, h = h0 + sub, unit = b * a.heads + h;
     const int steps = a.steps;
     int len = steps;
     if (a.lengths) {
@@ -292,7 +300,7 @@ __global__ void __launch_bounds__(64 * W, walk_waves(ST, K, W)) walk_kernel(Walk
     const int rev = R.rev, dy = R.dy, dz = R.dz;
     const float lg = a.log_decay[h] * 1.44269504088896340736f;
     auto power = [&](int n) { return n == 0 ? 1.f : __builtin_amdgcn_exp2f(lg * (float)n); };
-    if (tid < 2 * CH) {
+    if (wave == 0) {
         pow_pair[l] = l < CH - 1 ? 0.f : R.s_pair * power(l - (CH - 1));
         pow_add[l] = l < CH - 1 ? 0.f : R.s_add * power(l - (CH - 1));
     }
@@ -300,7 +308,7 @@ __global__ void __launch_bounds__(64 * W, walk_waves(ST, K, W)) walk_kernel(Walk
     const int end = len < seg1 ? len : seg1;
     auto row_of = [&](int tile) { return 8 * (r >> 2) + 4 * tile + (r & 3); };
     auto time = [&](int n) { return rev ? len - 1 - n : n; };   // of walk step n
-    auto head_of = [&](const Rows& m) { return (long)b * m.lane + (long)(h / m.shared) * m.head; };
+    auto head_of = [&](const Rows& m, int head) { return (long)b * m.lane + (long)(head / m.shared) * m.head; };
 
     // ---- rows of a chunk: x and y by all waves, z by each wave its channels, in units of 16 bytes along a row: unit u of
     // thread t is unit t % PER of row u T / PER + t / PER.  FAST: a chunk of L steps is a buffer from its earliest time to its
@@ -313,36 +321,38 @@ __global__ void __launch_bounds__(64 * W, walk_waves(ST, K, W)) walk_kernel(Walk
         int off;        // the thread's byte offset
     };
     const int dir = rev ? -1 : 1;
-    auto view = [&](const Rows& m, int size, int d, int row, int channel) {
+    auto view = [&](const Rows& m, int size, int d, int row, int head, int channel) {   // head: of the workgroup's
+        auto place = [&](int i) { return HEADS > 1 ? ((h0 + i) / m.shared - h0 / m.shared) * (int)m.head * size : 0; };
         View v;
         v.step = (int)m.step * size;
-        v.at = (const char*)m.p + (head_of(m) + (long)time(seg0) * m.step) * size;
+        v.at = (const char*)m.p + (head_of(m, h0) + (long)time(seg0) * m.step) * size;
         v.hop = (long)dir * CH * v.step;
-        v.row = d * size;
-        v.off = channel < d ? dir * row * v.step + channel * size : OUTSIDE;
+        v.row = place(HEADS - 1) + d * size;
+        v.off = channel < d ? dir * row * v.step + place(head) + channel * size : OUTSIDE;
         return v;
     };
     auto chunk = [&](const View& v, int L) { return buffer(rev ? v.at - (long)(L - 1) * v.step : v.at, (L - 1) * v.step + v.row); };
-    constexpr int PER = D / UNIT, PERZ = 32 * W / UNIT;     // units of a row of x and y, of z
-    constexpr int ROWS = 64 * W / PER, ROWSZ = 64 * W / PERZ;   // rows of a load
-    constexpr int N = ROWS < CH ? CH / ROWS : 1, NZ = CH / ROWSZ;   // loads of a thread
+    constexpr int PER = D / UNIT, PERZ = 32 * W / UNIT;               // units of a head's row of x and y, of z
+    constexpr int ROWS = T / (HEADS * PER), ROWSZ = T / (HEADS * PERZ);   // rows of a load
+    constexpr int N = ROWS < CH ? CH / ROWS : 1, NZ = CH / ROWSZ;         // loads of a thread
+    const int in_row = tid % (HEADS * PER), in_rowz = tid % (HEADS * PERZ), row = tid / (HEADS * PER), rowz = tid / (HEADS * PERZ);
     View vx = {}, vy = {}, vz = {}, vo = {};
     const int out_size = R.out_f32 ? 4 : SIZE;
     const unsigned char* marks = a.reset ? a.reset + (long)b * a.reset_lane : nullptr;
     const char* at_mark = nullptr;
     const int mark_step = (int)a.reset_step, mark_off = (rev ? 1 - l : l) * mark_step;
     if constexpr (FAST) {
-        vy = view(R.y, SIZE, dy, tid / PER, tid % PER * UNIT);
-        vz = view(R.z, SIZE, dz, tid / PERZ, tid % PERZ * UNIT);
+        vy = view(R.y, SIZE, dy, row, in_row / PER, in_row % PER * UNIT);
+        vz = view(R.z, SIZE, dz, rowz, in_rowz / PERZ, in_rowz % PERZ * UNIT);
         if constexpr (OUTS) {
-            vx = view(R.x, SIZE, dy, tid / PER, tid % PER * UNIT);
-            vo = view(R.out, out_size, dz, r, dz0 + 8 * g);
+            vx = view(R.x, SIZE, dy, row, in_row / PER, in_row % PER * UNIT);
+            vo = view(R.out, out_size, dz, r, sub, dz0 + 8 * g);
         }
         at_mark = marks ? (const char*)marks + (long)time(seg0) * a.reset_step : nullptr;
     }
     u32x4 rx[OUTS ? N : 1], ry[N], rz[NZ];
     int mark = 0;
-    auto fetch = [&](const Rows& m, View& v, int rows, int row, int channel, int d, int n0, int L, auto& raw) {
+    auto fetch = [&](const Rows& m, View& v, int rows, int row, int channel, int d, int n0, int L, auto& raw) {   // (HEADS 1 if not FAST)
         constexpr int M = sizeof(raw) / 16;
         if constexpr (FAST) {
             const Buf bm = chunk(v, L);
@@ -356,7 +366,7 @@ __global__ void __launch_bounds__(64 * W, walk_waves(ST, K, W)) walk_kernel(Walk
 #pragma unroll
             for (int u = 0; u < M; u++) {
                 const int n = u * rows + row;
-                const E* e = (const E*)m.p + head_of(m) + (long)time(n0 + n) * m.step + channel;
+                const E* e = (const E*)m.p + head_of(m, h) + (long)time(n0 + n) * m.step + channel;
                 EU x = {};
 #pragma unroll
                 for (int j = 0; j < UNIT; j++)
@@ -367,9 +377,9 @@ __global__ void __launch_bounds__(64 * W, walk_waves(ST, K, W)) walk_kernel(Walk
     };
     auto load_rows = [&](int n0) {
         const int L = end - n0 < CH ? end - n0 : CH;
-        if constexpr (OUTS) fetch(R.x, vx, ROWS, tid / PER, tid % PER * UNIT, dy, n0, L, rx);
-        fetch(R.y, vy, ROWS, tid / PER, tid % PER * UNIT, dy, n0, L, ry);
-        fetch(R.z, vz, ROWSZ, tid / PERZ, tid % PERZ * UNIT, dz, n0, L, rz);
+        if constexpr (OUTS) fetch(R.x, vx, ROWS, row, in_row * UNIT, dy, n0, L, rx);
+        fetch(R.y, vy, ROWS, row, in_row * UNIT, dy, n0, L, ry);
+        fetch(R.z, vz, ROWSZ, rowz, in_rowz * UNIT, dz, n0, L, rz);
         // lane j has the mark that separates the chunk's walk steps j - 1 and j (0: from the entering state, L: from the
         // leaving one).  An episode's first step is cut off from what time puts before it, so the backward walk has it one
         // later.
@@ -447,12 +457,12 @@ __global__ void __launch_bounds__(64 * W, walk_waves(ST, K, W)) walk_kernel(Walk
         auto last_cut = [&](unsigned long long m) { return m ? 63 - __builtin_clzll(m) : 0; };
         const int leaving = last_cut(cut);   // what leaves the chunk is of the steps from here on
 
-        lds_barrier<W>();   // the chunk before has been read
-        if constexpr (OUTS) lay(lx, PITCH, PLANE, ROWS, tid / PER, tid % PER * UNIT, rx);
-        lay(ly, PITCH, PLANE, ROWS, tid / PER, tid % PER * UNIT, ry);
+        lds_barrier<B>();   // the chunk before has been read
+        if constexpr (OUTS) lay(tx[in_row / PER], PITCH, PLANE, ROWS, row, in_row % PER * UNIT, rx);
+        lay(ty[in_row / PER], PITCH, PLANE, ROWS, row, in_row % PER * UNIT, ry);
         // (each wave's channels of z have a tile of their own)
-        lay(lz[tid % PERZ * UNIT / 32], 32, ZPLANE, ROWSZ, tid / PERZ, tid % PERZ * UNIT % 32, rz);
-        lds_barrier<W>();
+        lay(tz[in_rowz / PERZ][in_rowz % PERZ * UNIT / 32], 32, ZPLANE, ROWSZ, rowz, in_rowz * UNIT % 32, rz);
+        lds_barrier<B>();
         if (more) load_rows(n0 + CH);   // the chunk is in LDS: the registers take the next one's rows
         auto read = [&](const __bf16* m, int row, int k, bf16x8 (&o)[IN]) {
 #pragma unroll
@@ -494,14 +504,14 @@ __global__ void __launch_bounds__(64 * W, walk_waves(ST, K, W)) walk_kernel(Walk
 #pragma unroll
                 for (int u = 0; u < MID; u++) lp[c][u][l] = parts[u];
             }
-            lds_barrier<W>();
+            lds_barrier<B>();
         }
         if (leaving > 0) {   // z's weights will be zeros for these steps, which a y row that is not finite would not heed
-            for (int e = tid; e < leaving * IN * (D / 8); e += 64 * W) {
+            for (int e = tid % (64 * W); e < leaving * IN * (D / 8); e += 64 * W) {
                 const int row = e / (IN * (D / 8)), at = e % (IN * (D / 8));
                 *(u32x4*)(ly + at / (D / 8) * PLANE + row * PITCH + at % (D / 8) * 8) = u32x4{0, 0, 0, 0};
             }
-            lds_barrier<W>();
+            lds_barrier<B>();
         }
 
         __builtin_amdgcn_sched_barrier(0);   // (what the scheduler would move across costs more registers than there are)
@@ -510,7 +520,7 @@ __global__ void __launch_bounds__(64 * W, walk_waves(ST, K, W)) walk_kernel(Walk
 #pragma unroll
             for (int j = 0; j < 2; j++)
 #pragma unroll
-                for (int i = 0; i < IN; i++) T[j][i] = column(lz[wave] + i * ZPLANE, 32, 8 * g, 4 * j, r);
+                for (int i = 0; i < IN; i++) T[j][i] = column(lz + i * ZPLANE, 32, 8 * g, 4 * j, r);
             // z values that are not finite: zeros to the products, and NaN to what sees them.  The steps at which a channel
             // has some go to odd[channel]
             unsigned odd[2] = {0, 0};
@@ -527,7 +537,7 @@ __global__ void __launch_bounds__(64 * W, walk_waves(ST, K, W)) walk_kernel(Walk
                     }
                     odd[j] |= __shfl_xor(odd[j], 16);
                     odd[j] |= __shfl_xor(odd[j], 32);
-                    if (g == 0) lodd[wave][8 * (r >> 2) + 4 * j + (r & 3)] = odd[j];
+                    if (g == 0) lodd[8 * (r >> 2) + 4 * j + (r & 3)] = odd[j];
                 }
                 lds_barrier<1>();
             }
@@ -571,7 +581,7 @@ __global__ void __launch_bounds__(64 * W, walk_waves(ST, K, W)) walk_kernel(Walk
                         for (int j = 0; j < 2; j++)
 #pragma unroll
                             for (int q = 0; q < 4; q++)
-                                if (lodd[wave][8 * g + 4 * j + q] & sees) o[c][j][q] = __builtin_nanf("");
+                                if (lodd[8 * g + 4 * j + q] & sees) o[c][j][q] = __builtin_nanf("");
                     }
                     const f32x8 v = pair(o[c][0], o[c][1]);
                     if constexpr (FAST) {
@@ -581,7 +591,7 @@ __global__ void __launch_bounds__(64 * W, walk_waves(ST, K, W)) walk_kernel(Walk
                         if (ST == HUM_F32 || R.out_f32) store<HUM_F32>(bo, at, second, v);
                         else store<ST>(bo, at, second, v);
                     } else if (R.out.p && n < L && d < dz) {
-                        const long at = head_of(R.out) + (long)time(n0 + n) * R.out.step + d;
+                        const long at = head_of(R.out, h) + (long)time(n0 + n) * R.out.step + d;
                         if (R.out_f32) store_some<HUM_F32>(R.out.p, at, dz - d, v);
                         else store_some<ST>(R.out.p, at, dz - d, v);
                     }
@@ -639,11 +649,11 @@ __global__ void __launch_bounds__(64 * W, walk_waves(ST, K, W)) walk_kernel(Walk
     if (OUTS && R.out.p && dz0 + 8 * g < dz)
         for (int n = (len > seg0 ? len : seg0) + r; n < seg1; n += 16) {
             const int d = dz0 + 8 * g;
-            const long at = head_of(R.out) + (long)n * R.out.step + d;
+            const long at = head_of(R.out, h) + (long)n * R.out.step + d;
             if (R.out_f32) store_some<HUM_F32>(R.out.p, at, dz - d, f32x8{});
             else store_some<ST>(R.out.p, at, dz - d, f32x8{});
         }
-    if (R.through && tid == 0) R.through[item] = passed;
+    if (R.through && wave == 0 && l == 0) R.through[unit * a.segs + seg] = passed;
     if (R.state_out && (!a.last_only || seg + 1 == a.segs)) {
         float* s = R.state_out + (long)unit * R.out_unit + (long)seg * R.out_seg;
         if constexpr (FAST) {
@@ -887,35 +897,45 @@ int check_args(const char* fn, const hum_decay_attn_args* p) {
 
 int in_32(int d) { return d <= 32 ? 1 : d <= 64 ? 2 : 4; }
 template <int ST, int K, int W, bool OUTS>
-void launch_walk_o(const WalkArgs& a, bool fast, hipStream_t s) {
-    const long units = (long)a.lanes * a.heads * a.segs;
-    const dim3 grid((unsigned)((units + XCDS * NEAR - 1) / (XCDS * NEAR) * (XCDS * NEAR) * a.nroles));
-    if (fast) hipLaunchKernelGGL((walk_kernel<ST, K, W, true, OUTS>), grid, dim3(64 * W), 0, s, a);
-    else if constexpr (K == W) hipLaunchKernelGGL((walk_kernel<ST, K, W, false, OUTS>), grid, dim3(64 * W), 0, s, a);
+void launch_walk_o(const WalkArgs& a, bool fast, bool together, hipStream_t s) {
+    // 4 waves a workgroup from as many heads as that takes, where keys and values are equally wide; a float32 head's rows
+    // fill enough of the LDS by themselves
+    constexpr int H = ST == HUM_F32 || K != W ? 1 : 4 / W;
+    auto grid = [&](int heads) {
+        const long n = (long)a.lanes * a.heads / heads * a.segs;
+        return dim3((unsigned)((n + XCDS * NEAR - 1) / (XCDS * NEAR) * (XCDS * NEAR) * a.nroles));
+    };
+    if (fast && together && a.heads % H == 0) hipLaunchKernelGGL((walk_kernel<ST, K, W, H, true, OUTS>), grid(H), dim3(64 * W * H), 0, s, a);
+    else if (fast) hipLaunchKernelGGL((walk_kernel<ST, K, W, 1, true, OUTS>), grid(1), dim3(64 * W), 0, s, a);
+    else if constexpr (K == W) hipLaunchKernelGGL((walk_kernel<ST, K, W, 1, false, OUTS>), grid(1), dim3(64 * W), 0, s, a);
 }
 template <int ST, int K, int W>
-void launch_walk_w(const WalkArgs& a, bool fast, hipStream_t s) {
-    if (a.r[0].x.p) launch_walk_o<ST, K, W, true>(a, fast, s);
-    else launch_walk_o<ST, K, W, false>(a, fast, s);
+void launch_walk_w(const WalkArgs& a, bool fast, bool together, hipStream_t s) {
+    if (a.r[0].x.p) launch_walk_o<ST, K, W, true>(a, fast, together, s);
+    else launch_walk_o<ST, K, W, false>(a, fast, together, s);
 }
 template <int ST, int K>
-void launch_walk_k(const WalkArgs& a, int w, bool fast, hipStream_t s) {
-    if (w == 1) launch_walk_w<ST, K, 1>(a, fast, s);
-    else if (w == 2) launch_walk_w<ST, K, 2>(a, fast, s);
-    else launch_walk_w<ST, K, 4>(a, fast, s);
+void launch_walk_k(const WalkArgs& a, int w, bool fast, bool together, hipStream_t s) {
+    if (w == 1) launch_walk_w<ST, K, 1>(a, fast, together, s);
+    else if (w == 2) launch_walk_w<ST, K, 2>(a, fast, together, s);
+    else launch_walk_w<ST, K, 4>(a, fast, together, s);
 }
 template <int ST>
 void launch_walk_t(const WalkArgs& a, hipStream_t s) {
-    bool fast = !a.reset || (a.reset_step >= 0 && a.reset_step < (1l << 25));
+    // together: four heads of a step are neighbours and the steps so far apart that a chunk's 32 rows lie in as many pages
+    // (gradient of 4096 x 32 steps, time-major 2 MB apart: 337 us with single heads, 309 us; lane-major 263 and 284 us)
+    bool fast = !a.reset || (a.reset_step >= 0 && a.reset_step < (1l << 25)), together = true;
+    auto within = [](const Rows& m, int d) { return m.head >= 0 && 3 * m.head + d <= m.step && m.step * Num<ST>::SIZE >= 1 << 16; };
     for (int i = 0; i < a.nroles; i++) {
         const Role& r = a.r[i];
         fast = fast && (!r.x.p || r.x.vec) && r.y.vec && r.z.vec && (!r.out.p || r.out.vec) && r.s_vec;
+        together = together && (!r.x.p || within(r.x, r.dy)) && within(r.y, r.dy) && within(r.z, r.dz) && (!r.out.p || within(r.out, r.dz));
     }
     int k = in_32(a.r[0].dy), w = in_32(a.r[0].dz);
     if (!fast) k = w = k > w ? k : w;   // (that form is built for squares only)
-    if (k == 1) launch_walk_k<ST, 1>(a, w, fast, s);
-    else if (k == 2) launch_walk_k<ST, 2>(a, w, fast, s);
-    else launch_walk_k<ST, 4>(a, w, fast, s);
+    if (k == 1) launch_walk_k<ST, 1>(a, w, fast, together, s);
+    else if (k == 2) launch_walk_k<ST, 2>(a, w, fast, together, s);
+    else launch_walk_k<ST, 4>(a, w, fast, together, s);
 }
 
 // Few lanes and many steps: the walks are cut into segments that run side by side, each from the state that a first pass

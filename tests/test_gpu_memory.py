@@ -35,7 +35,8 @@ def close(got, want, size, kind, steps, state=False):
 
 
 class Case:
-    def __init__(self, b, s, h, g, dk, dv, kind="bf16", order="lane", resets=0.0, lengths=None, state=True, seed=0, odd=False):
+    def __init__(self, b, s, h, g, dk, dv, kind="bf16", order="lane", resets=0.0, lengths=None, state=True, seed=0, odd=False,
+                 far=0):
         r = torch.Generator().manual_seed(seed * 7919 + b * 31 + s)
         self.kind, self.scale, self.steps = kind, dk ** -0.5, s
         dt = TYPES[kind]
@@ -44,6 +45,9 @@ class Case:
             extra = 3 if odd else 0   # rows cut out of a wider, unaligned buffer
             shape = (s, b, heads, d + extra) if order == "time" else (b, s, heads, d + extra)
             x = torch.randn(shape, generator=r).to(dt).to(DEV)
+            if far:   # time-major steps `far` elements apart
+                wide = torch.empty(s, far, dtype=dt, device=DEV)
+                x = wide[:, :b * heads * d].copy_(x.reshape(s, -1)).view(s, b, heads, d)
             x = x[..., 1:1 + d] if odd else x
             return x.transpose(0, 1) if order == "time" else x
         self.q, self.k, self.v, self.d_out = rows(h, dk), rows(g, dk), rows(g, dv), rows(h, dv)
@@ -99,6 +103,24 @@ def test_attention_and_gradient(shape, kind):
     c = Case(*shape, kind=kind, resets=0.1, order="time" if sum(shape) % 2 else "lane")
     out, _ = c.check_forward()
     assert out.dtype == c.q.dtype
+    c.check_backward()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp32", "fp16"])
+@pytest.mark.parametrize("dk,dv", [(32, 32), (8, 64), (24, 128), (64, 32), (64, 64), (56, 128), (128, 16), (128, 40), (120, 128)])
+def test_widths_of_keys_and_values(dk, dv, kind):
+    """Every pair of width classes, aligned."""
+    c = Case(2, 75, 2, 1, dk, dv, kind=kind, resets=0.03, lengths=[75, 34])
+    c.check_forward()
+    c.check_backward()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp32", "fp16"])
+@pytest.mark.parametrize("h,g,d", [(4, 4, 64), (4, 1, 64), (4, 2, 32), (8, 8, 32), (3, 3, 64), (6, 3, 32), (2, 2, 128)])
+def test_steps_far_apart(h, g, d, kind):
+    """Time-major steps of a wide batch (64 KB and more from one to the next), where a workgroup takes several heads."""
+    c = Case(3, 70, h, g, d, d, kind=kind, order="time", resets=0.04, lengths=[70, 41, 0], far=32768 + 64)
+    c.check_forward()
     c.check_backward()
 
 
