@@ -343,10 +343,13 @@ Shape shape_of(int c, bool near) {   // near: a wave's rows lie within 2^31 byte
     return {1024, 2};
 }
 int groups_of(Shape s) { return s.tpr >= THREADS ? 1 : THREADS / s.tpr; }
-// workgroups of the backward pass: 4 per CU, each row group with 8 rows at least where there are that many
-long grad_blocks(long rows, Shape s) {
-    const long g = groups_of(s), want = (rows + 8 * g - 1) / (8 * g);
-    return want < 1 ? 1 : want > 1024 ? 1024 : want;
+// workgroups of the backward pass: one per CU at least, up to 4 while their partial rows (16 bytes a channel written and
+// read) stay below an eighth of what the rows themselves take (4099 x 1111 float32: 384 workgroups)
+long grad_blocks(long rows, Shape s, int size) {
+    const long g = groups_of(s), most = (rows + g - 1) / g;
+    long want = 3 * rows * size / 128;
+    want = want < 256 ? 256 : want > 1024 ? 1024 : want;
+    return most < 1 ? 1 : want < most ? want : most;
 }
 
 template <int ST, int TPR, int NV>
@@ -428,7 +431,8 @@ int hum_layer_norm_workspace(const hum_norm_args* p, uint64_t* bytes) {
     const char* fn = "hum_layer_norm_workspace";
     if (const int rc = check_sizes(fn, p)) return rc;
     if (!bytes) return nerr(HUM_ERR_ARG, fn, "null argument");
-    const uint64_t a = grad_blocks(p->rows, shape_of(p->channels, true)), b = grad_blocks(p->rows, shape_of(p->channels, false));
+    const int es = p->type == HUM_F32 ? 4 : 2;
+    const uint64_t a = grad_blocks(p->rows, shape_of(p->channels, true), es), b = grad_blocks(p->rows, shape_of(p->channels, false), es);
     *bytes = (a > b ? a : b) * 2 * p->channels * sizeof(float);
     return HUM_OK;
 }
@@ -454,7 +458,7 @@ int hum_layer_norm_backward(const hum_norm_args* p, const void* dy, int64_t dy_r
     if (!dev.ok) return nerr(HUM_ERR_HIP, fn, "hipSetDevice");
     GradArgs a = {dy, p->x, p->weight, dx, mean, rstd, params ? (float*)workspace : nullptr, (long)p->rows, (long)dy_row, (long)p->x_row, (long)dx_row, p->channels, p->param_type == HUM_F32};
     const bool vec = p->channels % 8 == 0 && aligned(p->x, p->x_row, es) && aligned(dy, dy_row, es) && (!dx || aligned(dx, dx_row, es)) && (uintptr_t)p->weight % 16 == 0;
-    const long blocks = grad_blocks(p->rows, sh);   // no rows: one workgroup writes zero sums
+    const long blocks = grad_blocks(p->rows, sh, es);   // no rows: one workgroup writes zero sums
     launch_norm(p->type, a, sh, vec, blocks, (hipStream_t)stream);
     if (params) {
         const dim3 grid((2 * p->channels + 15) / 16);

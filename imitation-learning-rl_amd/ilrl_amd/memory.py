@@ -117,22 +117,27 @@ def _check(e, q, k, v, log_decay, state, reset, lengths, axes):
                          % ("steps, " if axes == 4 else "", list(qs), list(ks), list(vs)))
     if not q.is_cuda:
         raise ValueError("q must be on a GPU (there is no CPU path)")
-    dev, dt = q.device, q.dtype
+    dev, dt, index = q.device, q.dtype, q.get_device()
     lead, h, dk = qs[:-2], qs[-2], qs[-1]
     g, dv = ks[-2], vs[-1]
-    _on(k, dev, "k", lead + (g, dk), (dt,))
-    _on(v, dev, "v", lead + (g, dv), (dt,))
+    # (one expression for what is nearly always so: the single step's host time is its time)
+    if not (k.dtype == dt == v.dtype and ks == lead + (g, dk) and vs == lead + (g, dv) and k.get_device() == index
+            and v.get_device() == index):
+        _on(k, dev, "k", lead + (g, dk), (dt,))
+        _on(v, dev, "v", lead + (g, dv), (dt,))
     if g < 1 or h % g:
         raise ValueError("%d key / value heads cannot be shared evenly by %d query heads" % (g, h))
     if not (1 <= dk <= MAX_HEAD_CHANNELS and 1 <= dv <= MAX_HEAD_CHANNELS):
         raise ValueError("1 to %d channels a head, got %d (keys) and %d (values)" % (MAX_HEAD_CHANNELS, dk, dv))
-    _on(log_decay, dev, "log_decay", (h,), (f32,))
+    if not (log_decay.dtype == f32 and log_decay.shape == (h,) and log_decay.get_device() == index):
+        _on(log_decay, dev, "log_decay", (h,), (f32,))
     if log_decay.requires_grad:
         raise ValueError("log_decay is a constant schedule and has no gradient: pass log_decay.detach()")
     if not log_decay.is_contiguous():
         log_decay = log_decay.contiguous()
     if state is not None:
-        _on(state, dev, "state", (lead[0], h, dv, dk), (f32,))
+        if not (state.dtype == f32 and state.shape == (lead[0], h, dv, dk) and state.get_device() == index):
+            _on(state, dev, "state", (lead[0], h, dv, dk), (f32,))
         if not state.is_contiguous():
             raise ValueError("state must be contiguous")
     if reset is not None:
@@ -287,7 +292,7 @@ def decay_attention_step(q, k, v, log_decay, state, reset=None, active=None, sca
             raise ValueError("state_out must be contiguous")
     shape = (n, sizes[2], sizes[5])
     if out is None:
-        out = t.empty(shape, dtype=q.dtype, device=dev)
+        out = t.empty_like(v) if v.shape == shape and v.is_contiguous() else t.empty(shape, dtype=q.dtype, device=dev)
     elif _unit(_on(out, dev, "out", shape, (q.dtype,))) is not out:
         raise ValueError("out must have adjacent channels")
     sq, sk, sv, so, index = q.stride(), k.stride(), v.stride(), out.stride(), q.get_device()
@@ -312,11 +317,16 @@ def _norm_args(e, x, weight, bias, param_dtype):
     x2 = _unit(x if x.dim() == 2 else x.reshape(-1, c))
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise ValueError("weight and bias must have one type, got %s and %s" % (weight.dtype, bias.dtype))
+    index, f32 = x.get_device(), e.t.float32
     if weight is not None:
-        weight = _on(weight, x.device, "weight", (c,), (e.t.float32, x.dtype)).contiguous()
+        if not (weight.dtype == f32 and weight.shape == (c,) and weight.get_device() == index):
+            _on(weight, x.device, "weight", (c,), (f32, x.dtype))
+        weight = weight.contiguous()
     if bias is not None:
-        bias = _on(bias, x.device, "bias", (c,), (e.t.float32, x.dtype)).contiguous()
-    a = _NORM.pack(x2.get_device(), code, N.HUM_F32 if param_dtype == e.t.float32 else code, c, x2.shape[0], x2.stride(0),
+        if not (bias.dtype == f32 and bias.shape == (c,) and bias.get_device() == index):
+            _on(bias, x.device, "bias", (c,), (f32, x.dtype))
+        bias = bias.contiguous()
+    a = _NORM.pack(index, code, N.HUM_F32 if param_dtype == f32 else code, c, x2.shape[0], x2.stride(0),
                    x2.data_ptr(), weight.data_ptr() if weight is not None else 0)
     return x2, weight, bias, a
 
@@ -329,7 +339,7 @@ def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, out=None, stats=True
     p = weight if weight is not None else bias
     x2, weight, bias, a = _norm_args(e, x, weight, bias, p.dtype if p is not None else t.float32)
     if out is None:
-        out = t.empty(x.shape, dtype=x.dtype, device=dev)
+        out = t.empty_like(x) if x2 is x and x.is_contiguous() else t.empty(x.shape, dtype=x.dtype, device=dev)
     else:
         _on(out, dev, "out", x.shape, (x.dtype,))
         if not out.is_contiguous():
@@ -351,12 +361,17 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, needs=(True, True, True)
         param_dtype = weight.dtype if weight is not None else None
     x2, weight, _, a = _norm_args(e, x, weight, None, param_dtype if param_dtype is not None else t.float32)
     rows, c = x2.shape
-    dy2 = _unit(_on(dy, dev, "dy", x.shape, (x.dtype,)).reshape(-1, c))
+    if not (dy.dtype == x.dtype and dy.shape == x.shape and dy.get_device() == x.get_device()):
+        _on(dy, dev, "dy", x.shape, (x.dtype,))
+    dy2 = _unit(dy if dy.dim() == 2 else dy.reshape(-1, c))
     mean = _on(mean, dev, "mean", (rows,), (t.float32,)).contiguous()
     rstd = _on(rstd, dev, "rstd", (rows,), (t.float32,)).contiguous()
-    dx = t.empty(x.shape, dtype=x.dtype, device=dev) if needs[0] else None
-    dw = t.empty(c, dtype=param_dtype, device=dev) if needs[1] and param_dtype is not None else None
-    db = t.empty(c, dtype=param_dtype, device=dev) if needs[2] and param_dtype is not None else None
+    dx = dw = db = None
+    if needs[0]:
+        dx = t.empty_like(x) if x2 is x and x.is_contiguous() else t.empty(x.shape, dtype=x.dtype, device=dev)
+    if param_dtype is not None and (needs[1] or needs[2]):
+        dw, db = t.empty((2, c), dtype=param_dtype, device=dev).unbind(0)
+        dw, db = dw if needs[1] else None, db if needs[2] else None
     ws, size = None, 0
     if dw is not None or db is not None:
         need = ctypes.c_uint64(0)
