@@ -59,7 +59,8 @@ struct Rows {               // [lane, step, head, channel] with unit channel str
     void* p;
     long lane, step, head;  // strides in elements
     int shared;             // heads that read one of its heads
-    int vec;                // rows of 16-byte units, aligned; steps do not overlap and lie less than 2^25 bytes apart
+    int near;               // steps lie less than 2^25 bytes apart
+    int vec;                // and do not overlap, and rows are of 16-byte units, aligned
 };
 
 struct Role {
@@ -164,6 +165,12 @@ template <> struct Num<HUM_BF16> { typedef __bf16 T; static constexpr int IN = 1
 template <> struct Num<HUM_F16> { typedef _Float16 T; static constexpr int IN = 2, MID = 2, SIZE = 2; };
 template <> struct Num<HUM_F32> { typedef float T; static constexpr int IN = 3, MID = 3, SIZE = 4; };
 
+// How a walk's rows are accessed.  BUFFER: rows of whole aligned units of 16 bytes, through buffers.  WIDE: 16 bytes at any
+// alignment.  ANY: the same with 64-bit addresses and a branch for heads of fewer channels than 16 bytes hold; also steps
+// 2^25 bytes apart and more, or backwards in memory.  Gradient of 4096 x 32 steps, 4 heads, bf16: 64 channels in BUFFER
+// 304 us; 63 in WIDE 508, in ANY 523, element by element 916; 60 channels 445, 470 and 900
+enum Mode { BUFFER, WIDE, ANY };
+
 // 16 loaded bytes into the planes of an LDS tile
 template <int ST>
 __device__ __forceinline__ void put(__bf16* m, int plane, u32x4 raw) {
@@ -209,12 +216,71 @@ __device__ __forceinline__ void store(Buf b, int at, int second, f32x8 v) {
         buf_store(b, at, __builtin_bit_cast(u32x4, __builtin_convertvector(v, bf16x8)));
     }
 }
-template <int ST>
-__device__ __forceinline__ void store_some(void* p, long at, int n, f32x8 v) {   // n of 8, any alignment
-    typename Num<ST>::T* e = (typename Num<ST>::T*)p + at;
+
+// ---- accesses at element alignment (64-bit addresses; the hardware takes 16 bytes at any of them).  A row's last piece must
+// not pass the row's end, so it is loaded from an earlier place, where it ends with the row, and shifted down
+#define GLOBAL __attribute__((address_space(1)))
+typedef unsigned int any4 __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned int any2 __attribute__((ext_vector_type(2), aligned(2)));
+typedef unsigned int any1 __attribute__((aligned(2)));
+template <typename E> struct Any {
+    static constexpr int UNIT = 16 / sizeof(E);
+    typedef E V __attribute__((ext_vector_type(UNIT)));
+    typedef GLOBAL E* P;
+    // UNIT elements of a row of d, from element c on (c may be behind the end): where to load them, and what is loaded
+    static __device__ __forceinline__ int place(int c, int d) { return d < UNIT || c < d - UNIT ? c : d - UNIT; }
+    static __device__ __forceinline__ u32x4 load(const E* row, int c, int d) {
+        const P p = (P)row;
+        if (d >= UNIT) return *(GLOBAL any4*)(p + place(c, d));
+        V x = {};
 #pragma unroll
-    for (int j = 0; j < 8; j++)
-        if (j < n) e[j] = (typename Num<ST>::T)v[j];
+        for (int j = 0; j < UNIT; j++) x[j] = c + j < d ? p[c + j] : (E)0;   // (a head of few channels)
+        return __builtin_bit_cast(u32x4, x);
+    }
+    // the loaded piece's elements from c - place(c, d) on, zeros behind the row's end
+    static __device__ __forceinline__ u32x4 align(u32x4 v, int by) {
+        if constexpr (sizeof(E) == 2) {
+            const int half = 16 * (by & 1);
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[i] = __builtin_amdgcn_alignbit(i < 3 ? v[i + 1] : 0u, v[i], half);
+        }
+        const int words = by * (int)sizeof(E) / 4;
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = words & 1 ? (i < 3 ? v[i + 1] : 0u) : v[i];
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = words & 2 ? (i < 2 ? v[i + 2] : 0u) : v[i];
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = words & ~3 ? 0u : v[i];
+        return v;
+    }
+    // the first n (of UNIT, or more for all)
+    static __device__ __forceinline__ void store(E* to, int n, u32x4 v) {
+        const P p = (P)to;
+        if (n >= UNIT) {
+            *(GLOBAL any4*)p = v;
+            return;
+        }
+        constexpr int H = UNIT / 2, Q = UNIT / 4;   // elements of 8 bytes, of 4
+        if (n & H) *(GLOBAL any2*)p = u32x2{v[0], v[1]};
+        const unsigned w0 = n & H ? v[2] : v[0], w1 = n & H ? v[3] : v[1];
+        if (n & Q) *(GLOBAL any1*)(p + (n & H)) = w0;
+        if constexpr (sizeof(E) == 2) {
+            const unsigned short e = (unsigned short)(n & Q ? w1 : w0);
+            if (n & 1) p[n & (H + Q)] = __builtin_bit_cast(E, e);
+        }
+    }
+};
+template <int ST>
+__device__ __forceinline__ void store_some(void* p, long at, int n, f32x8 v) {   // n of 8 channels, rounded once
+    typedef typename Num<ST>::T E;
+    E* e = (E*)p + at;
+    if constexpr (ST == HUM_F32) {
+        Any<E>::store(e, n, __builtin_bit_cast(u32x4, __builtin_shufflevector(v, v, 0, 1, 2, 3)));
+        if (n > 4) Any<E>::store(e + 4, n - 4, __builtin_bit_cast(u32x4, __builtin_shufflevector(v, v, 4, 5, 6, 7)));
+    } else {
+        typedef E E8 __attribute__((ext_vector_type(8)));
+        Any<E>::store(e, n, __builtin_bit_cast(u32x4, __builtin_convertvector(v, E8)));
+    }
 }
 
 // what the workgroup's waves wrote to LDS before it, all of them read behind it (loads in flight stay in flight)
@@ -249,19 +315,19 @@ __device__ __forceinline__ f32x4 quad_transpose(f32x4 v) {
 }
 
 // waves per SIMD that the registers are limited for (the state takes 16 K of them)
-constexpr int walk_waves(int st, int k, int w) {   // (a single wave has all of a chunk's rows in flight)
+constexpr int walk_waves(int st, int k, int w, Mode mode) {   // (a single wave has all of a chunk's rows in flight)
     const bool alone = k > 1 && w == 1;
+    if (mode != BUFFER) return st == HUM_BF16 ? (k > 1 ? 2 : 3) : k > 2 ? 1 : 2;
     return st == HUM_BF16 ? (k > 2 && alone ? 1 : k > 2 || alone ? 2 : 3) : st == HUM_F16 ? (k > 2 && alone ? 1 : 2) : k > 2 || alone ? 1 : 2;
 }
 
 // One workgroup per HEADS neighbouring heads of a lane, role and segment; W waves per head, each with 32 of z's channels and
 // its slice of the state.  A head's waves share the chunk's x and y rows (K operands of 32 channels) and P; the heads of a
 // workgroup only share the loading, so that a load meets long pieces of few rows (with one head, 4096 lanes' time-major
-// steps lie 2 MB apart and each load meets 8 pages for 1 KB: forward 177 us, 168 us with the heads together).  FAST: every operand may be accessed 16 bytes at a
-// time through buffers; else element by element, at any alignment and stride.  OUTS: rows come out (else the states of the
+// steps lie 2 MB apart and each load meets 8 pages for 1 KB: forward 177 us, 168 us with the heads together).  OUTS: rows come out (else the states of the
 // segments are wanted only).
-template <int ST, int K, int W, int HEADS, bool FAST, bool OUTS>
-__global__ void __launch_bounds__(64 * W * HEADS, walk_waves(ST, K, W)) walk_kernel(WalkArgs a) {
+template <int ST, int K, int W, int HEADS, Mode MODE, bool OUTS>
+__global__ void __launch_bounds__(64 * W * HEADS, walk_waves(ST, K, W, MODE)) walk_kernel(WalkArgs a) {
     constexpr int IN = Num<ST>::IN, MID = Num<ST>::MID, SIZE = Num<ST>::SIZE, UNIT = 16 / SIZE;
     constexpr int D = 32 * K;                  // channels of x and y rounded up
     constexpr int PITCH = D + 8;               // of x and y in LDS: 16-byte reads of 16 rows meet no bank twice
@@ -311,7 +377,7 @@ __global__ void __launch_bounds__(64 * W * HEADS, walk_waves(ST, K, W)) walk_ker
     auto head_of = [&](const Rows& m, int head) { return (long)b * m.lane + (long)(head / m.shared) * m.head; };
 
     // ---- rows of a chunk: x and y by all waves, z by each wave its channels, in units of 16 bytes along a row: unit u of
-    // thread t is unit t % PER of row u T / PER + t / PER.  FAST: a chunk of L steps is a buffer from its earliest time to its
+    // thread t is unit t % PER of row u T / PER + t / PER.  BUFFER: a chunk of L steps is a buffer from its earliest time to its
     // last row's end, so the steps behind L lie outside (walking backwards: before it, at negative offsets, which are
     // large ones); `at` is the address of the walk's next chunk's first row
     struct View {
@@ -341,7 +407,7 @@ __global__ void __launch_bounds__(64 * W * HEADS, walk_waves(ST, K, W)) walk_ker
     const unsigned char* marks = a.reset ? a.reset + (long)b * a.reset_lane : nullptr;
     const char* at_mark = nullptr;
     const int mark_step = (int)a.reset_step, mark_off = (rev ? 1 - l : l) * mark_step;
-    if constexpr (FAST) {
+    if constexpr (MODE == BUFFER) {
         vy = view(R.y, SIZE, dy, row, in_row / PER, in_row % PER * UNIT);
         vz = view(R.z, SIZE, dz, rowz, in_rowz / PERZ, in_rowz % PERZ * UNIT);
         if constexpr (OUTS) {
@@ -352,26 +418,23 @@ __global__ void __launch_bounds__(64 * W * HEADS, walk_waves(ST, K, W)) walk_ker
     }
     u32x4 rx[OUTS ? N : 1], ry[N], rz[NZ];
     int mark = 0;
-    auto fetch = [&](const Rows& m, View& v, int rows, int row, int channel, int d, int n0, int L, auto& raw) {   // (HEADS 1 if not FAST)
+    auto fetch = [&](const Rows& m, View& v, int rows, int row, int channel, int d, int n0, int L, auto& raw) {   // (HEADS 1 if not BUFFER)
         constexpr int M = sizeof(raw) / 16;
-        if constexpr (FAST) {
+        if constexpr (MODE == BUFFER) {
             const Buf bm = chunk(v, L);
             const int base = rev ? (L - 1) * v.step : 0;
 #pragma unroll
             for (int u = 0; u < M; u++) raw[u] = buf_load(bm, v.off + (base + dir * u * rows * v.step));
             v.at += v.hop;
         } else {
+            // (a row behind the chunk's last step loads the last one's: it is made zeros)
             typedef typename Num<ST>::T E;
-            typedef E EU __attribute__((ext_vector_type(UNIT)));
+            const GLOBAL char* base = (const GLOBAL char*)m.p + (head_of(m, h) + (long)time(n0 + (rev ? L - 1 : 0)) * m.step) * SIZE;
 #pragma unroll
             for (int u = 0; u < M; u++) {
-                const int n = u * rows + row;
-                const E* e = (const E*)m.p + head_of(m, h) + (long)time(n0 + n) * m.step + channel;
-                EU x = {};
-#pragma unroll
-                for (int j = 0; j < UNIT; j++)
-                    if (n < L && channel + j < d) x[j] = e[j];
-                raw[u] = __builtin_bit_cast(u32x4, x);
+                const int n = u * rows + row, k = n < L ? n : L - 1, t = rev ? L - 1 - k : k;
+                if constexpr (MODE == WIDE) raw[u] = *(const GLOBAL any4*)(base + (unsigned)(t * (int)m.step + Any<E>::place(channel, d)) * SIZE);
+                else raw[u] = Any<E>::load((const E*)(const char*)base + t * m.step, channel, d);
             }
         }
     };
@@ -383,20 +446,28 @@ __global__ void __launch_bounds__(64 * W * HEADS, walk_waves(ST, K, W)) walk_ker
         // lane j has the mark that separates the chunk's walk steps j - 1 and j (0: from the entering state, L: from the
         // leaving one).  An episode's first step is cut off from what time puts before it, so the backward walk has it one
         // later.
-        if constexpr (FAST) {
+        if constexpr (MODE == BUFFER) {
             const Buf bm = buffer(rev ? at_mark - (long)(L - 1) * mark_step : at_mark, marks ? (L - 1) * mark_step + 1 : 0);
             mark = __builtin_amdgcn_raw_buffer_load_b8(bm, mark_off + (rev ? (L - 1) * mark_step : 0), 0, 0);
             at_mark += (long)dir * CH * mark_step;
         } else if (marks) {
-            const int n = l - rev;
-            mark = n >= 0 && n < L ? marks[(long)time(n0 + n) * a.reset_step] : 0;
+            const int n = l - rev;   // (lanes outside the chunk's steps are not asked)
+            mark = marks[(long)time(n0 + (n < 0 ? 0 : n < L ? n : L - 1)) * a.reset_step];
         }
     };
-    auto lay = [&](__bf16* m, int pitch, int plane, int rows, int row, int channel, const auto& raw) {
+    auto lay = [&](__bf16* m, int pitch, int plane, int rows, int row, int channel, int d, int L, int at, const auto& raw) {
         constexpr int M = sizeof(raw) / 16;
+        typedef Any<typename Num<ST>::T> A;
 #pragma unroll
         for (int u = 0; u < M; u++)
-            if (u * rows + row < CH) put<ST>(m + (u * rows + row) * pitch + channel, plane, raw[u]);
+            if (u * rows + row < CH) {
+                u32x4 v = raw[u];
+                if constexpr (MODE != BUFFER) {
+                    v = A::align(v, channel - A::place(channel, d));
+                    v = u * rows + row < L ? v : u32x4{0, 0, 0, 0};
+                }
+                put<ST>(m + (u * rows + row) * pitch + at, plane, v);
+            }
     };
     if (seg0 < end) load_rows(seg0);
 
@@ -410,6 +481,14 @@ __global__ void __launch_bounds__(64 * W * HEADS, walk_waves(ST, K, W)) walk_ker
         const int y = 32 * (i >> 1) + 8 * g + 4 * (i & 1) + quad, z = zc(j) - quad;
         return 4 * (__mul24(z, s_z) + __mul24(y, s_y)) | beyond(y, dy) | beyond(z, dz);
     };
+    const int s_d = along_y ? dy : dz;
+    auto state_piece = [&](int i, int j, int& c, bool& in) {   // the element of the row of unit stride it begins at, and which row
+        const int y = 32 * (i >> 1) + 8 * g + 4 * (i & 1) + quad, z = zc(j) - quad;
+        const int row = along_y ? z : y, rows = along_y ? dz : dy;
+        c = along_y ? y : z;
+        in = row < rows;
+        return (in ? row : rows - 1) * s_d;
+    };
     auto turn_state = [&] {
         if (!along_y)
 #pragma unroll
@@ -419,7 +498,7 @@ __global__ void __launch_bounds__(64 * W * HEADS, walk_waves(ST, K, W)) walk_ker
     };
     {
         const float* s = R.state_in ? R.state_in + (long)unit * R.in_unit + (long)seg * R.in_seg : nullptr;
-        if constexpr (FAST) {
+        if constexpr (MODE == BUFFER) {
             const Buf bs = buffer(s, 4 * dy * dz);
 #pragma unroll
             for (int j = 0; j < 2; j++)
@@ -427,15 +506,27 @@ __global__ void __launch_bounds__(64 * W * HEADS, walk_waves(ST, K, W)) walk_ker
                 for (int i = 0; i < 2 * K; i++) S[i][j] = buf_load4(bs, state_at(i, j));
             turn_state();
         } else {
+            typedef Any<float> A;
 #pragma unroll
             for (int j = 0; j < 2; j++)
 #pragma unroll
                 for (int i = 0; i < 2 * K; i++) {
-                    const int y0 = 32 * (i >> 1) + 8 * g + 4 * (i & 1), z = zc(j);
-#pragma unroll
-                    for (int q = 0; q < 4; q++)
-                        S[i][j][q] = s && z < dz && y0 + q < dy ? s[(long)z * R.sz + (long)(y0 + q) * R.sy] : 0.f;
+                    int c;
+                    bool in;
+                    const int at = state_piece(i, j, c, in);
+                    S[i][j] = s ? __builtin_bit_cast(f32x4, A::load(s + at, c, s_d)) : f32x4{0.f, 0.f, 0.f, 0.f};
                 }
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int i = 0; i < 2 * K; i++) {
+                    int c;
+                    bool in;
+                    state_piece(i, j, c, in);
+                    const u32x4 v = A::align(__builtin_bit_cast(u32x4, S[i][j]), c - A::place(c, s_d));
+                    S[i][j] = in ? __builtin_bit_cast(f32x4, v) : f32x4{0.f, 0.f, 0.f, 0.f};
+                }
+            turn_state();
         }
     }
     float w_in[2];
@@ -458,10 +549,10 @@ __global__ void __launch_bounds__(64 * W * HEADS, walk_waves(ST, K, W)) walk_ker
         const int leaving = last_cut(cut);   // what leaves the chunk is of the steps from here on
 
         lds_barrier<B>();   // the chunk before has been read
-        if constexpr (OUTS) lay(tx[in_row / PER], PITCH, PLANE, ROWS, row, in_row % PER * UNIT, rx);
-        lay(ty[in_row / PER], PITCH, PLANE, ROWS, row, in_row % PER * UNIT, ry);
+        if constexpr (OUTS) lay(tx[in_row / PER], PITCH, PLANE, ROWS, row, in_row * UNIT, dy, L, in_row % PER * UNIT, rx);
+        lay(ty[in_row / PER], PITCH, PLANE, ROWS, row, in_row * UNIT, dy, L, in_row % PER * UNIT, ry);
         // (each wave's channels of z have a tile of their own)
-        lay(tz[in_rowz / PERZ][in_rowz % PERZ * UNIT / 32], 32, ZPLANE, ROWSZ, rowz, in_rowz * UNIT % 32, rz);
+        lay(tz[in_rowz / PERZ][in_rowz % PERZ * UNIT / 32], 32, ZPLANE, ROWSZ, rowz, in_rowz * UNIT, dz, L, in_rowz * UNIT % 32, rz);
         lds_barrier<B>();
         if (more) load_rows(n0 + CH);   // the chunk is in LDS: the registers take the next one's rows
         auto read = [&](const __bf16* m, int row, int k, bf16x8 (&o)[IN]) {
@@ -584,7 +675,7 @@ __global__ void __launch_bounds__(64 * W * HEADS, walk_waves(ST, K, W)) walk_ker
                                 if (lodd[8 * g + 4 * j + q] & sees) o[c][j][q] = __builtin_nanf("");
                     }
                     const f32x8 v = pair(o[c][0], o[c][1]);
-                    if constexpr (FAST) {
+                    if constexpr (MODE == BUFFER) {
                         const Buf bo = buffer(R.out.p ? (rev ? vo.at - (long)(L - 1) * vo.step : vo.at) : nullptr, (L - 1) * vo.step + vo.row);
                         int at = vo.off + ((rev ? (L - 1) * vo.step : 0) + dir * 16 * c * vo.step);
                         const int second = (at + 16) | beyond(d + 4, dz);
@@ -642,7 +733,7 @@ __global__ void __launch_bounds__(64 * W * HEADS, walk_waves(ST, K, W)) walk_ker
                 }
             }
         }
-        if constexpr (FAST && OUTS) vo.at += vo.hop;
+        if constexpr (MODE == BUFFER && OUTS) vo.at += vo.hop;
     }
 
     // ---- the steps behind the lane's length
@@ -656,7 +747,7 @@ __global__ void __launch_bounds__(64 * W * HEADS, walk_waves(ST, K, W)) walk_ker
     if (R.through && wave == 0 && l == 0) R.through[unit * a.segs + seg] = passed;
     if (R.state_out && (!a.last_only || seg + 1 == a.segs)) {
         float* s = R.state_out + (long)unit * R.out_unit + (long)seg * R.out_seg;
-        if constexpr (FAST) {
+        if constexpr (MODE == BUFFER) {
             const Buf bs = buffer(s, 4 * dy * dz);
             turn_state();
 #pragma unroll
@@ -664,14 +755,15 @@ __global__ void __launch_bounds__(64 * W * HEADS, walk_waves(ST, K, W)) walk_ker
 #pragma unroll
                 for (int i = 0; i < 2 * K; i++) buf_store4(bs, state_at(i, j), S[i][j]);
         } else {
+            turn_state();
 #pragma unroll
             for (int j = 0; j < 2; j++)
 #pragma unroll
                 for (int i = 0; i < 2 * K; i++) {
-                    const int y0 = 32 * (i >> 1) + 8 * g + 4 * (i & 1), z = zc(j);
-#pragma unroll
-                    for (int q = 0; q < 4; q++)
-                        if (z < dz && y0 + q < dy) s[(long)z * R.sz + (long)(y0 + q) * R.sy] = S[i][j][q];
+                    int c;
+                    bool in;
+                    const int at = state_piece(i, j, c, in);
+                    if (in && c < s_d) Any<float>::store(s + at + c, s_d - c, __builtin_bit_cast(u32x4, S[i][j]));
                 }
         }
     }
@@ -773,35 +865,37 @@ __device__ __forceinline__ float row_sum(float v) {   // over LPR neighbouring l
     return v;
 }
 
-// VEC: rows of S are 16-byte aligned multiples of 4 channels
-template <int ST, int LPR, bool VEC>
+// A row's last piece of 4 channels is the row's last 4: the lane does what its neighbour does to the channels before its own
+// (both store the same) and leaves them out of its sum.  Buffers take 16 bytes at any multiple of 4.  (One lane per row:
+// single channels, as there may be fewer than 4.)
+template <int ST, int LPR>
 __global__ void __launch_bounds__(256) step_kernel(StepArgs a) {
     constexpr int U = 4, ROWS = 64 / LPR;
     const int unit = blockIdx.x / a.blocks, blk = blockIdx.x - unit * a.blocks;
     const int b = unit / a.heads, h = unit - b * a.heads;
     const int wave = threadIdx.x >> 6, l = threadIdx.x & 63;
-    const int c0 = 4 * (l % LPR), row0 = (blk * 4 + wave) * U * ROWS + l / LPR;
+    const int own = 4 * (l % LPR), c0 = LPR == 1 || own + 4 <= a.dk ? own : a.dk - 4, row0 = (blk * 4 + wave) * U * ROWS + l / LPR;
     const long size = (long)a.dv * a.dk;
     const Buf si = buffer(a.state_in ? a.state_in + unit * size : nullptr, 4 * (int)size), so = buffer(a.state_out + unit * size, 4 * (int)size);
-    int at[U];   // byte offsets of a lane's 4 channels (VEC), else of the first
+    int at[U];   // byte offsets of a lane's first channel
     f32x4 s[U];
 #pragma unroll
     for (int u = 0; u < U; u++) {
         const int row = row0 + u * ROWS;
-        at[u] = 4 * (__mul24(row, a.dk) + c0) | beyond(row, a.dv) | beyond(c0, a.dk);
-        if constexpr (VEC) {
+        at[u] = 4 * (__mul24(row, a.dk) + c0) | beyond(row, a.dv) | beyond(own, a.dk);
+        if constexpr (LPR > 1) {
             s[u] = buf_load4(si, at[u]);
         } else {
 #pragma unroll
             for (int j = 0; j < 4; j++)
-                s[u][j] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(si, (at[u] + 4 * j) | beyond(c0 + j, a.dk), 0, 0));
+                s[u][j] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(si, (at[u] + 4 * j) | beyond(j, a.dk), 0, 0));
         }
     }
     const long qo = (long)b * a.q.lane + (long)(h / a.q.shared) * a.q.head, ko = (long)b * a.k.lane + (long)(h / a.k.shared) * a.k.head;
     const long vo = (long)b * a.v.lane + (long)(h / a.v.shared) * a.v.head, oo = (long)b * a.out.lane + (long)h * a.out.head;
     float q[4], k[4], v[U];
 #pragma unroll
-    for (int j = 0; j < 4; j++) {   // (a channel behind the last reads the last: its k is made 0)
+    for (int j = 0; j < 4; j++) {   // (a channel behind the last reads the last: it is not stored)
         const int c = c0 + j < a.dk ? c0 + j : a.dk - 1;
         q[j] = elem<ST>(a.q.p, qo + c);
         k[j] = elem<ST>(a.k.p, ko + c);
@@ -822,19 +916,19 @@ __global__ void __launch_bounds__(256) step_kernel(StepArgs a) {
         if (on) {
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const bool in = c0 + j < a.dk;
-                s[u][j] = in ? (fresh ? 0.f : s[u][j] * lambda) + v[u] * k[j] : 0.f;
+                const bool in = LPR > 1 ? c0 + j >= own : j < a.dk;
+                s[u][j] = (fresh ? 0.f : s[u][j] * lambda) + v[u] * k[j];
                 o[u] += in ? s[u][j] * q[j] : 0.f;
             }
             o[u] = row_sum<LPR>(o[u]) * a.scale;
         }
         if (!keep) {
-            if constexpr (VEC) {
+            if constexpr (LPR > 1) {
                 buf_store4(so, at[u], s[u]);
             } else {
 #pragma unroll
                 for (int j = 0; j < 4; j++)
-                    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, (float)s[u][j]), so, (at[u] + 4 * j) | beyond(c0 + j, a.dk), 0, 0);
+                    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, (float)s[u][j]), so, (at[u] + 4 * j) | beyond(j, a.dk), 0, 0);
             }
         }
     }
@@ -871,9 +965,10 @@ struct OnDevice {   // the caller's current device stays what it was
 int elem_size(int type) { return type == HUM_F32 ? 4 : 2; }
 
 Rows rows_of(const hum_rows& r, int shared, int size, int d) {
+    const bool near = r.step >= 0 && r.step < (1l << 25) / size;
     const bool vec = ((uintptr_t)r.ptr | (uintptr_t)(r.lane * size) | (uintptr_t)(r.step * size) | (uintptr_t)(r.head * size)) % 16 == 0 &&
-                     d * size % 16 == 0 && r.step >= d && r.step < (1l << 25) / size;
-    return Rows{r.ptr, (long)r.lane, (long)r.step, (long)r.head, shared, vec};
+                     d * size % 16 == 0 && r.step >= d && near;
+    return Rows{r.ptr, (long)r.lane, (long)r.step, (long)r.head, shared, near, vec};
 }
 
 int check_args(const char* fn, const hum_decay_attn_args* p) {
@@ -897,7 +992,7 @@ int check_args(const char* fn, const hum_decay_attn_args* p) {
 
 int in_32(int d) { return d <= 32 ? 1 : d <= 64 ? 2 : 4; }
 template <int ST, int K, int W, bool OUTS>
-void launch_walk_o(const WalkArgs& a, bool fast, bool together, hipStream_t s) {
+void launch_walk_o(const WalkArgs& a, Mode mode, bool together, hipStream_t s) {
     // 4 waves a workgroup from as many heads as that takes, where keys and values are equally wide; a float32 head's rows
     // fill enough of the LDS by themselves
     constexpr int H = ST == HUM_F32 || K != W ? 1 : 4 / W;
@@ -905,37 +1000,43 @@ void launch_walk_o(const WalkArgs& a, bool fast, bool together, hipStream_t s) {
         const long n = (long)a.lanes * a.heads / heads * a.segs;
         return dim3((unsigned)((n + XCDS * NEAR - 1) / (XCDS * NEAR) * (XCDS * NEAR) * a.nroles));
     };
-    if (fast && together && a.heads % H == 0) hipLaunchKernelGGL((walk_kernel<ST, K, W, H, true, OUTS>), grid(H), dim3(64 * W * H), 0, s, a);
-    else if (fast) hipLaunchKernelGGL((walk_kernel<ST, K, W, 1, true, OUTS>), grid(1), dim3(64 * W), 0, s, a);
-    else if constexpr (K == W) hipLaunchKernelGGL((walk_kernel<ST, K, W, 1, false, OUTS>), grid(1), dim3(64 * W), 0, s, a);
+    if (mode == BUFFER && together && a.heads % H == 0) hipLaunchKernelGGL((walk_kernel<ST, K, W, H, BUFFER, OUTS>), grid(H), dim3(64 * W * H), 0, s, a);
+    else if (mode == BUFFER) hipLaunchKernelGGL((walk_kernel<ST, K, W, 1, BUFFER, OUTS>), grid(1), dim3(64 * W), 0, s, a);
+    else if constexpr (K == W) {
+        if (mode == WIDE) hipLaunchKernelGGL((walk_kernel<ST, K, W, 1, WIDE, OUTS>), grid(1), dim3(64 * W), 0, s, a);
+        else hipLaunchKernelGGL((walk_kernel<ST, K, W, 1, ANY, OUTS>), grid(1), dim3(64 * W), 0, s, a);
+    }
 }
 template <int ST, int K, int W>
-void launch_walk_w(const WalkArgs& a, bool fast, bool together, hipStream_t s) {
-    if (a.r[0].x.p) launch_walk_o<ST, K, W, true>(a, fast, together, s);
-    else launch_walk_o<ST, K, W, false>(a, fast, together, s);
+void launch_walk_w(const WalkArgs& a, Mode mode, bool together, hipStream_t s) {
+    if (a.r[0].x.p) launch_walk_o<ST, K, W, true>(a, mode, together, s);
+    else launch_walk_o<ST, K, W, false>(a, mode, together, s);
 }
 template <int ST, int K>
-void launch_walk_k(const WalkArgs& a, int w, bool fast, bool together, hipStream_t s) {
-    if (w == 1) launch_walk_w<ST, K, 1>(a, fast, together, s);
-    else if (w == 2) launch_walk_w<ST, K, 2>(a, fast, together, s);
-    else launch_walk_w<ST, K, 4>(a, fast, together, s);
+void launch_walk_k(const WalkArgs& a, int w, Mode mode, bool together, hipStream_t s) {
+    if (w == 1) launch_walk_w<ST, K, 1>(a, mode, together, s);
+    else if (w == 2) launch_walk_w<ST, K, 2>(a, mode, together, s);
+    else launch_walk_w<ST, K, 4>(a, mode, together, s);
 }
 template <int ST>
 void launch_walk_t(const WalkArgs& a, hipStream_t s) {
     // together: four heads of a step are neighbours and the steps so far apart that a chunk's 32 rows lie in as many pages
     // (gradient of 4096 x 32 steps, time-major 2 MB apart: 337 us with single heads, 309 us; lane-major 263 and 284 us)
-    bool fast = !a.reset || (a.reset_step >= 0 && a.reset_step < (1l << 25)), together = true;
+    bool buffers = !a.reset || (a.reset_step >= 0 && a.reset_step < (1l << 25)), wide = true, together = true;
+    auto near = [](const Rows& m, int d) { return m.near && d * Num<ST>::SIZE >= 16; };
     auto within = [](const Rows& m, int d) { return m.head >= 0 && 3 * m.head + d <= m.step && m.step * Num<ST>::SIZE >= 1 << 16; };
     for (int i = 0; i < a.nroles; i++) {
         const Role& r = a.r[i];
-        fast = fast && (!r.x.p || r.x.vec) && r.y.vec && r.z.vec && (!r.out.p || r.out.vec) && r.s_vec;
+        buffers = buffers && (!r.x.p || r.x.vec) && r.y.vec && r.z.vec && (!r.out.p || r.out.vec) && r.s_vec;
+        wide = wide && (!r.x.p || near(r.x, r.dy)) && near(r.y, r.dy) && near(r.z, r.dz);
         together = together && (!r.x.p || within(r.x, r.dy)) && within(r.y, r.dy) && within(r.z, r.dz) && (!r.out.p || within(r.out, r.dz));
     }
     int k = in_32(a.r[0].dy), w = in_32(a.r[0].dz);
-    if (!fast) k = w = k > w ? k : w;   // (that form is built for squares only)
-    if (k == 1) launch_walk_k<ST, 1>(a, w, fast, together, s);
-    else if (k == 2) launch_walk_k<ST, 2>(a, w, fast, together, s);
-    else launch_walk_k<ST, 4>(a, w, fast, together, s);
+    const Mode mode = buffers ? BUFFER : wide ? WIDE : ANY;
+    if (mode != BUFFER) k = w = k > w ? k : w;   // (those are built for squares only)
+    if (k == 1) launch_walk_k<ST, 1>(a, w, mode, together, s);
+    else if (k == 2) launch_walk_k<ST, 2>(a, w, mode, together, s);
+    else launch_walk_k<ST, 4>(a, w, mode, together, s);
 }
 
 // Few lanes and many steps: the walks are cut into segments that run side by side, each from the state that a first pass
@@ -1199,20 +1300,15 @@ int hum_decay_attn_backward(const hum_decay_attn_args* p, const hum_rows* d_out,
 }  // extern "C"
 
 namespace {
-template <int ST, int LPR>
-void launch_step_v(const StepArgs& a, bool vec, dim3 grid, hipStream_t s) {
-    if (vec) hipLaunchKernelGGL((step_kernel<ST, LPR, true>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((step_kernel<ST, LPR, false>), grid, dim3(256), 0, s, a);
-}
 template <int ST>
-void launch_step(const StepArgs& a, int lpr, bool vec, dim3 grid, hipStream_t s) {
+void launch_step(const StepArgs& a, int lpr, dim3 grid, hipStream_t s) {
     switch (lpr) {
-        case 1: launch_step_v<ST, 1>(a, vec, grid, s); break;
-        case 2: launch_step_v<ST, 2>(a, vec, grid, s); break;
-        case 4: launch_step_v<ST, 4>(a, vec, grid, s); break;
-        case 8: launch_step_v<ST, 8>(a, vec, grid, s); break;
-        case 16: launch_step_v<ST, 16>(a, vec, grid, s); break;
-        default: launch_step_v<ST, 32>(a, vec, grid, s); break;
+        case 1: hipLaunchKernelGGL((step_kernel<ST, 1>), grid, dim3(256), 0, s, a); break;
+        case 2: hipLaunchKernelGGL((step_kernel<ST, 2>), grid, dim3(256), 0, s, a); break;
+        case 4: hipLaunchKernelGGL((step_kernel<ST, 4>), grid, dim3(256), 0, s, a); break;
+        case 8: hipLaunchKernelGGL((step_kernel<ST, 8>), grid, dim3(256), 0, s, a); break;
+        case 16: hipLaunchKernelGGL((step_kernel<ST, 16>), grid, dim3(256), 0, s, a); break;
+        default: hipLaunchKernelGGL((step_kernel<ST, 32>), grid, dim3(256), 0, s, a); break;
     }
 }
 }  // namespace
@@ -1242,14 +1338,13 @@ extern "C" int hum_decay_attn_step(const hum_decay_attn_args* p, const uint8_t* 
     a.dk = p->dk;
     a.dv = p->dv;
     a.scale = p->scale;
-    const bool vec = p->dk % 4 == 0 && ((uintptr_t)p->state_in | (uintptr_t)p->state_out) % 16 == 0;
     int lpr = 1;
     while (4 * lpr < p->dk) lpr *= 2;
     const int rows = 4 * 4 * (64 / lpr);
     a.blocks = (p->dv + rows - 1) / rows;
     const dim3 grid((unsigned)(p->lanes * p->heads * a.blocks));
-    if (p->type == HUM_BF16) launch_step<HUM_BF16>(a, lpr, vec, grid, (hipStream_t)stream);
-    else if (p->type == HUM_F16) launch_step<HUM_F16>(a, lpr, vec, grid, (hipStream_t)stream);
-    else launch_step<HUM_F32>(a, lpr, vec, grid, (hipStream_t)stream);
+    if (p->type == HUM_BF16) launch_step<HUM_BF16>(a, lpr, grid, (hipStream_t)stream);
+    else if (p->type == HUM_F16) launch_step<HUM_F16>(a, lpr, grid, (hipStream_t)stream);
+    else launch_step<HUM_F32>(a, lpr, grid, (hipStream_t)stream);
     return launched(fn);
 }

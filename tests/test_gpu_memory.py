@@ -116,6 +116,30 @@ def test_widths_of_keys_and_values(dk, dv, kind):
 
 
 @pytest.mark.parametrize("kind", ["bf16", "fp32", "fp16"])
+@pytest.mark.parametrize("dk", [1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 13, 14, 15, 17, 23, 31, 33, 34, 61, 66, 99, 127])
+def test_rows_that_end_inside_a_load(dk, kind):
+    """Rows of any width at any alignment, cut out of a buffer of NaN: nothing beside a row is read into it, and a result's
+    row is written beside others that keep theirs."""
+    dv = dk * 37 % 128 + 1
+    c = Case(2, 37, 2, 1, dk, dv, kind=kind, order="time" if dk % 2 else "lane", resets=0.05, lengths=[37, 20], odd=True)
+    for name in ("q", "k", "v", "d_out"):
+        x = getattr(c, name)
+        wide = torch.full((*x.shape[:3], x.shape[3] + 3), float("nan"), dtype=x.dtype, device=DEV)
+        wide[..., 1:1 + x.shape[3]] = x
+        setattr(c, name, wide[..., 1:1 + x.shape[3]])
+    c.check_forward()
+    c.check_backward()
+
+
+@pytest.mark.parametrize("kind,d", [("bf16", 64), ("bf16", 63), ("fp32", 5), ("fp16", 6)])
+def test_steps_very_far_apart(kind, d):
+    """32 MB and more from one step to the next."""
+    c = Case(2, 36, 2, 1, d, d, kind=kind, order="time", resets=0.04, lengths=[36, 33], far=(2 ** 25 + 64) // TYPES[kind].itemsize)
+    c.check_forward()
+    c.check_backward()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp32", "fp16"])
 @pytest.mark.parametrize("h,g,d", [(4, 4, 64), (4, 1, 64), (4, 2, 32), (8, 8, 32), (3, 3, 64), (6, 3, 32), (2, 2, 128)])
 def test_steps_far_apart(h, g, d, kind):
     """Time-major steps of a wide batch (64 KB and more from one to the next), where a workgroup takes several heads."""
@@ -282,6 +306,19 @@ def test_step_is_one_step_of_the_walk(n, h, g, dk, dv, kind):
     here = old.clone()
     out2 = M.decay_attention_step(c.q[:, 0], c.k[:, 0], c.v[:, 0], c.log_decay, here, reset=c.reset[:, 0], active=active, scale=c.scale)
     assert torch.equal(out, out2) and torch.equal(here, into)
+
+
+@pytest.mark.parametrize("dk", [2, 3, 5, 6, 7, 9, 11, 15, 18, 29, 31, 33, 62, 63, 65, 95, 126, 127])
+def test_step_of_rows_that_end_inside_a_load(dk):
+    """Also of states that begin 4 bytes behind a multiple of 16, and what lies beside a state stays as it was."""
+    n, h, dv = 3, 2, 21
+    c = Case(n, 1, h, h, dk, dv, kind="fp32", resets=0.3)
+    size = n * h * dv * dk
+    flat = torch.full((size + 2,), 7.0, device=DEV)
+    state = flat[1:-1].view(n, h, dv, dk).copy_(c.state)
+    out = M.decay_attention_step(c.q[:, 0], c.k[:, 0], c.v[:, 0], c.log_decay, state, reset=c.reset[:, 0], scale=c.scale)
+    c.check_forward((out[:, None], state))
+    assert flat[0] == 7 and flat[-1] == 7
 
 
 def test_step_forgets_a_state_that_is_not_finite():
