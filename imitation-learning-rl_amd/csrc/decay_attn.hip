@@ -13,18 +13,26 @@
 // so one kernel, the walk out = walk(x, y, z) with the state sum y z^T, computes all four (struct Role).
 //
 // The walk goes over chunks of 32 steps.  Inside a chunk it is products of small matrices on the matrix cores:
-// P = (Y X^T) masked and weighted by D, O^T = Z^T P + S^T X^T, S = lambda^32 S + (w Y)^T Z.  One wave owns one (lane,
-// head, slice of z's channels) and keeps that slice of S in its accumulators for the whole walk; P and S never leave
-// registers, because the rows of every A operand are taken in the order
+// P = (Y X^T) masked and weighted by D, O^T = Z^T P + S^T X^T, S = lambda^32 S + (w Y)^T Z.  A workgroup owns one (lane,
+// head); each of its waves owns 32 of z's channels and keeps its slice of S in registers for the whole walk.  The chunk's
+// rows come into registers while the chunk before is worked on, and from there into LDS, where all waves read them; P is
+// formed by one wave for each half of its columns and shared through LDS.  The rows of every A operand are taken in the order
 //     matrix row m of tile a  <->  index 8 (m >> 2) + 4 a + (m & 3)   (of 32)
 // under which the accumulators of a pair of tiles (lane group g holds rows 4 g .. 4 g + 3 of each) are exactly the 8
-// consecutive contraction indexes 8 g .. 8 g + 7 that lane group needs as an operand of the next product.  Only Y^T and
-// Z^T (contraction over the steps) go through LDS, read back transposed.
+// consecutive contraction indexes 8 g .. 8 g + 7 that lane group needs as an operand of the next product: S feeds O, and P
+// goes to the other waves, without a change of layout.  Contractions over the steps read Y and Z back transposed.
 //
-// Rounding.  Products of bf16 inputs are exact in the float32 accumulators.  Computed operands are split into bf16
-// parts that sum to them: P and the state read by O into two (2^-18 of the value, under the output's own 2^-9), the
-// weighted Y that enters the state into three (2^-26, below float32's 2^-24: the state is held in 32 bits).  float32 and
-// float16 inputs use the float32 matrix instruction (16 times slower, 153 TFLOP/s on this card) and are not split.
+// What bounds it (bf16, time-major rows).  Many lanes: HBM.  Forward of 4096 lanes x 32 steps, 4 heads x 64 x 64: 0.80 GB
+// in 152 us, 5.3 TB/s where a large copy reaches 5.1; gradient 1.28 GB in 297 us.  Few lanes: the latency of a chunk (LDS
+// round trips and dependent matrix instructions), 2 to 4 us of it, since a walk is serial: so walks are cut into segments
+// (cut_of), whose states cost traffic of their own.  Forward of 1 x 8192 steps, 8 heads x 128 x 128: segments' states 19,
+// scan 13, outputs 30 us.
+//
+// Rounding.  Every element type goes through the bf16 matrix cores: bf16 inputs as they are, float16 as two bf16 parts and
+// float32 as three, exactly but for 2^-27; products of parts are exact in the float32 accumulators.  Computed operands are
+// split likewise: P and the state read by O into two parts (2^-18 of the value, under the output's own 2^-9 or 2^-12; three
+// for float32), the weighted Z that enters the state into three (2^-27, below float32's 2^-24: the state is held in 32
+// bits).  An output is rounded once.
 //
 // Non-finite values.  A row of Z multiplies zeros of P for the steps that must not see it (earlier steps, other
 // episodes), and 0 x inf is NaN: such values of z enter the products as zeros and make NaN of the channels of exactly the
@@ -314,7 +322,8 @@ __device__ __forceinline__ f32x4 quad_transpose(f32x4 v) {
     return v;
 }
 
-// waves per SIMD that the registers are limited for (the state takes 16 K of them)
+// waves per SIMD that the registers are limited for (the state takes 16 K of them): the most that fit without scratch memory,
+// a few bytes of which cost more than a wave gives (forward of 4096 x 32 steps: 162 us, 180 with 12 bytes, 186 with two waves)
 constexpr int walk_waves(int st, int k, int w, Mode mode) {   // (a single wave has all of a chunk's rows in flight)
     const bool alone = k > 1 && w == 1;
     if (mode != BUFFER) return st == HUM_BF16 ? (k > 1 ? 2 : 3) : k > 2 ? 1 : 2;
@@ -324,8 +333,8 @@ constexpr int walk_waves(int st, int k, int w, Mode mode) {   // (a single wave 
 // One workgroup per HEADS neighbouring heads of a lane, role and segment; W waves per head, each with 32 of z's channels and
 // its slice of the state.  A head's waves share the chunk's x and y rows (K operands of 32 channels) and P; the heads of a
 // workgroup only share the loading, so that a load meets long pieces of few rows (with one head, 4096 lanes' time-major
-// steps lie 2 MB apart and each load meets 8 pages for 1 KB: forward 177 us, 168 us with the heads together).  OUTS: rows come out (else the states of the
-// segments are wanted only).
+// steps lie 2 MB apart and each load meets 8 pages for 1 KB: forward 177 us, 168 us with the heads together).  OUTS: rows
+// come out (else the states of the segments are wanted only).
 template <int ST, int K, int W, int HEADS, Mode MODE, bool OUTS>
 __global__ void __launch_bounds__(64 * W * HEADS, walk_waves(ST, K, W, MODE)) walk_kernel(WalkArgs a) {
     constexpr int IN = Num<ST>::IN, MID = Num<ST>::MID, SIZE = Num<ST>::SIZE, UNIT = 16 / SIZE;
@@ -771,7 +780,7 @@ __global__ void __launch_bounds__(64 * W * HEADS, walk_waves(ST, K, W, MODE)) wa
 
 // the segments' entering states from what each of them adds: seg[g] <- state before segment g, one thread per element of
 // walk blockIdx.y.  A recurrence over the segments that only their loads' latency bounds: AHEAD of them are in flight
-// (64 segments of 8 heads x 128 x 128: 22 us with 8 of 16 bytes each)
+// (64 segments of 8 heads x 128 x 128: 13 us, 22 us with 8 in flight of 16 bytes each)
 struct ScanArgs {
     struct { const float* in; float* seg; const float* through; } w[2];
     int segs, size;
@@ -805,7 +814,8 @@ __global__ void __launch_bounds__(256) scan_kernel(ScanArgs a) {
 }
 
 // gradients of keys (blockIdx.y 0) and values (1) that `group` heads share: the sum of the heads' float32 partial results
-// part [lanes, steps, heads, d] -> out [lanes, steps, heads / group, d]; one thread per output channel
+// part [lanes, steps, heads, d] -> out [lanes, steps, heads / group, d]; one thread per output channel, the heads in order
+// (21 lanes x 131 steps, 4 heads to 1: 4 us, a launch's latency)
 struct ShareArgs {
     struct { const float* part; Rows out; int d; } x[2];
     long rows;
@@ -828,7 +838,8 @@ __global__ void __launch_bounds__(256) share_kernel(ShareArgs a) {
 
 // ---- single step: S = a S + v k^T, o = scale S q, all in float32 on the vector units - the state is read and written
 // once (8 bytes for 4 operations), so HBM bounds it.  LPR lanes of 4 key channels hold one row of S; a wave has
-// 64 / LPR rows in one load and U loads in flight, issued before anything that decides whether they are used.
+// 64 / LPR rows in one load and U loads in flight, issued before anything that decides whether they are used.  4096 lanes,
+// 4 heads x 64 x 64: 0.55 GB in 93 us, 5.8 TB/s; one lane: 10 us, the host's.
 struct StepArgs {
     Rows q, k, v, out;
     const float* log_decay;

@@ -468,9 +468,11 @@ typedef struct {
  *     S_t = a_t S_{t-1} + v_t k_t^T,  o_t = scale S_t q_t,  a_t = 0 where reset[lane, t] != 0 (an episode starts at step
  *     t: nothing before it is seen), else exp(log_decay[head]).
  * q [lanes, steps, heads, dk], k [lanes, steps, kv_heads, dk], v [lanes, steps, kv_heads, dv] of element type `type`;
- * query head h reads key / value head h / (heads / kv_heads).  Products of bf16 rows are summed in float32; the state is
- * float32.  Steps behind a lane's length are not read; their outputs and gradients are zeros.  log_decay is a constant
- * schedule (<= 0; -inf: no memory), not a trained parameter: it has no gradient. */
+ * query head h reads key / value head h / (heads / kv_heads).  Rows may have any alignment to their elements and any
+ * strides (rows of whole 16-byte units are the fast ones).  All sums and the state are float32; an output is rounded once.
+ * A value that is not finite makes NaN or an infinity of what the formula lets it reach, and of nothing else: not of
+ * earlier steps, other lanes or other episodes.  Steps behind a lane's length are not read; their outputs and gradients
+ * are zeros.  log_decay is a constant schedule (<= 0; -inf: no memory), not a trained parameter: it has no gradient. */
 typedef struct {
     int32_t device, type;
     int32_t lanes, steps, heads, kv_heads, dk, dv;   /* dk, dv in [1, 128]; lanes x heads <= 2^21 */
