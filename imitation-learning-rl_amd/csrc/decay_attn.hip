@@ -133,6 +133,21 @@ __device__ __forceinline__ void split(f32x8 v, bf16x8 (&o)[N]) {
     }
 }
 template <int N>
+__device__ __forceinline__ void split(f32x4 v, bf16x4 (&o)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        o[i] = __builtin_convertvector(v, bf16x4);
+        if (i + 1 < N) {
+            const u32x2 u = __builtin_bit_cast(u32x2, o[i]);
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                v[2 * j] -= __builtin_bit_cast(float, u[j] << 16);
+                v[2 * j + 1] -= __builtin_bit_cast(float, u[j] & 0xffff0000u);
+            }
+        }
+    }
+}
+template <int N>
 __device__ __forceinline__ f32x8 whole(const bf16x8 (&o)[N]) {
     f32x8 v = {};
 #pragma unroll
@@ -156,10 +171,11 @@ __device__ __forceinline__ void mma(f32x4& c, const bf16x8 (&a)[NA], const bf16x
         for (int j = 0; j < NB; j++)
             if (i + j < 3) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[j], c, 0, 0, 0);
 }
-// rows s0 .. s0 + 7 of 16 columns, 4 neighbours per quarter of 16 lanes: the transposing LDS load
+// rows s0 .. s0 + 7 of 16 columns, 4 neighbours per quarter of 16 lanes, quarters APART: the transposing LDS load
+template <int APART>
 __device__ __forceinline__ bf16x8 column(const __bf16* m, int pitch, int s0, int c0, int r) {
     typedef __attribute__((address_space(3))) bf16x4 L4;
-    const __bf16* p = m + (s0 + (r >> 2)) * pitch + c0 + 8 * (r & 3);
+    const __bf16* p = m + (s0 + (r >> 2)) * pitch + c0 + APART * (r & 3);
     const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((L4*)p);
     const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((L4*)(p + 4 * pitch));
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
@@ -176,7 +192,7 @@ template <> struct Num<HUM_F32> { typedef float T; static constexpr int IN = 3, 
 // How a walk's rows are accessed.  BUFFER: rows of whole aligned units of 16 bytes, through buffers.  WIDE: 16 bytes at any
 // alignment.  ANY: the same with 64-bit addresses and a branch for heads of fewer channels than 16 bytes hold; also steps
 // 2^25 bytes apart and more, or backwards in memory.  Gradient of 4096 x 32 steps, 4 heads, bf16: 64 channels in BUFFER
-// 304 us; 63 in WIDE 508, in ANY 523, element by element 916; 60 channels 445, 470 and 900
+// 301 us, 63 in WIDE 442 (60: 381), element by element 916 (900); WIDE saves 3 % against ANY
 enum Mode { BUFFER, WIDE, ANY };
 
 // 16 loaded bytes into the planes of an LDS tile
@@ -190,18 +206,10 @@ __device__ __forceinline__ void put(__bf16* m, int plane, u32x4 raw) {
         *(bf16x8*)m = o[0];
         *(bf16x8*)(m + plane) = o[1];
     } else {
-        f32x4 v = __builtin_bit_cast(f32x4, raw);
+        bf16x4 o[3];
+        split<3>(__builtin_bit_cast(f32x4, raw), o);
 #pragma unroll
-        for (int i = 0; i < 3; i++) {
-            const bf16x4 o = __builtin_convertvector(v, bf16x4);
-            *(bf16x4*)(m + i * plane) = o;
-            const u32x2 u = __builtin_bit_cast(u32x2, o);
-#pragma unroll
-            for (int j = 0; j < 2; j++) {
-                v[2 * j] -= __builtin_bit_cast(float, u[j] << 16);
-                v[2 * j + 1] -= __builtin_bit_cast(float, u[j] & 0xffff0000u);
-            }
-        }
+        for (int i = 0; i < 3; i++) *(bf16x4*)(m + i * plane) = o[i];
     }
 }
 // not 0 where one of 8 values (the first of their parts) is not finite: its exponent is all ones
@@ -222,6 +230,16 @@ __device__ __forceinline__ void store(Buf b, int at, int second, f32x8 v) {
         buf_store(b, at, __builtin_bit_cast(u32x4, __builtin_convertvector(v, f16x8)));
     } else {
         buf_store(b, at, __builtin_bit_cast(u32x4, __builtin_convertvector(v, bf16x8)));
+    }
+}
+
+template <int ST>
+__device__ __forceinline__ void store(Buf b, int at, int, f32x4 v) {
+    if constexpr (ST == HUM_F32) {
+        buf_store4(b, at, v);
+    } else {
+        typedef typename Num<ST>::T E4 __attribute__((ext_vector_type(4)));
+        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, __builtin_convertvector(v, E4)), b, at, 0, 0);
     }
 }
 
@@ -279,6 +297,18 @@ template <typename E> struct Any {
     }
 };
 template <int ST>
+__device__ __forceinline__ void store_some(void* p, long at, int n, f32x4 v) {   // n of 4
+    typedef typename Num<ST>::T E;
+    E* e = (E*)p + at;
+    if constexpr (ST == HUM_F32) {
+        Any<E>::store(e, n, __builtin_bit_cast(u32x4, v));
+    } else {
+        typedef E E4 __attribute__((ext_vector_type(4)));
+        const u32x2 u = __builtin_bit_cast(u32x2, __builtin_convertvector(v, E4));
+        Any<E>::store(e, n < 4 ? n : 4, u32x4{u[0], u[1], 0, 0});
+    }
+}
+template <int ST>
 __device__ __forceinline__ void store_some(void* p, long at, int n, f32x8 v) {   // n of 8 channels, rounded once
     typedef typename Num<ST>::T E;
     E* e = (E*)p + at;
@@ -335,19 +365,20 @@ constexpr int walk_waves(int st, int k, int w, Mode mode) {   // (a single wave 
 // workgroup only share the loading, so that a load meets long pieces of few rows (with one head, 4096 lanes' time-major
 // steps lie 2 MB apart and each load meets 8 pages for 1 KB: forward 177 us, 168 us with the heads together).  OUTS: rows
 // come out (else the states of the segments are wanted only).
-template <int ST, int K, int W, int HEADS, Mode MODE, bool OUTS>
+template <int ST, int K, int W, int J, int HEADS, Mode MODE, bool OUTS>
 __global__ void __launch_bounds__(64 * W * HEADS, walk_waves(ST, K, W, MODE)) walk_kernel(WalkArgs a) {
     constexpr int IN = Num<ST>::IN, MID = Num<ST>::MID, SIZE = Num<ST>::SIZE, UNIT = 16 / SIZE;
     constexpr int D = 32 * K;                  // channels of x and y rounded up
     constexpr int PITCH = D + 8;               // of x and y in LDS: 16-byte reads of 16 rows meet no bank twice
-    constexpr int PLANE = CH * PITCH, ZPLANE = CH * 32;
+    constexpr int Z = 16 * J;                  // channels of z of a wave
+    constexpr int PLANE = CH * PITCH, ZPLANE = CH * Z;
     constexpr int T = 64 * W * HEADS, B = W * HEADS;   // threads, waves
     __shared__ __attribute__((aligned(16))) __bf16 tx[HEADS][OUTS ? IN * PLANE : 8], ty[HEADS][IN * PLANE], tz[HEADS][W][IN * ZPLANE];
     __shared__ __attribute__((aligned(16))) bf16x8 tp[HEADS][OUTS ? 2 : 1][MID][64];
     // lambda^d times the scale's part for d = -31 .. 32 steps, zeros for d < 0: between two steps of a chunk, and from a
     // step to the chunk's end
     __shared__ float pows_pair[HEADS][2 * CH], pows_add[HEADS][2 * CH];
-    __shared__ unsigned odds[HEADS][W][32];
+    __shared__ unsigned odds[HEADS][W][Z];
 
     const int tid = threadIdx.x, l = tid & 63, g = l >> 4, r = l & 15;
     const int sub = HEADS > 1 ? __builtin_amdgcn_readfirstlane(tid / (64 * W)) : 0;   // the wave's head of the workgroup's
@@ -364,7 +395,7 @@ __global__ void __launch_bounds__(64 * W * HEADS, walk_waves(ST, K, W, MODE)) wa
     if (item >= a.lanes * a.heads / HEADS * a.segs) return;
     const int group = item / a.segs, seg = item - group * a.segs;
     const Role& R = a.r[ri];
-    const int dz0 = 32 * wave;
+    const int dz0 = Z * wave;
     const int b = group * HEADS / a.heads, h0 = group * HEADS - b * a.heads, h = h0 + sub, unit = b * a.heads + h;
     const int steps = a.steps;
     int len = steps;
@@ -407,7 +438,7 @@ __global__ void __launch_bounds__(64 * W * HEADS, walk_waves(ST, K, W, MODE)) wa
         return v;
     };
     auto chunk = [&](const View& v, int L) { return buffer(rev ? v.at - (long)(L - 1) * v.step : v.at, (L - 1) * v.step + v.row); };
-    constexpr int PER = D / UNIT, PERZ = 32 * W / UNIT;               // units of a head's row of x and y, of z
+    constexpr int PER = D / UNIT, PERZ = Z * W / UNIT;               // units of a head's row of x and y, of z
     constexpr int ROWS = T / (HEADS * PER), ROWSZ = T / (HEADS * PERZ);   // rows of a load
     constexpr int N = ROWS < CH ? CH / ROWS : 1, NZ = CH / ROWSZ;         // loads of a thread
     const int in_row = tid % (HEADS * PER), in_rowz = tid % (HEADS * PERZ), row = tid / (HEADS * PER), rowz = tid / (HEADS * PERZ);
@@ -421,7 +452,7 @@ __global__ void __launch_bounds__(64 * W * HEADS, walk_waves(ST, K, W, MODE)) wa
         vz = view(R.z, SIZE, dz, rowz, in_rowz / PERZ, in_rowz % PERZ * UNIT);
         if constexpr (OUTS) {
             vx = view(R.x, SIZE, dy, row, in_row / PER, in_row % PER * UNIT);
-            vo = view(R.out, out_size, dz, r, sub, dz0 + 8 * g);
+            vo = view(R.out, out_size, dz, r, sub, dz0 + 4 * J * g);
         }
         at_mark = marks ? (const char*)marks + (long)time(seg0) * a.reset_step : nullptr;
     }
@@ -481,8 +512,8 @@ __global__ void __launch_bounds__(64 * W * HEADS, walk_waves(ST, K, W, MODE)) wa
     if (seg0 < end) load_rows(seg0);
 
     // ---- the entering state: tile (i, j) holds y channels 32 (i / 2) + 8 g + 4 (i & 1) + 0..3 of z channel zc(j)
-    f32x4 S[2 * K][2];
-    auto zc = [&](int j) { return dz0 + 8 * (r >> 2) + 4 * j + (r & 3); };
+    f32x4 S[2 * K][J];
+    auto zc = [&](int j) { return dz0 + 4 * J * (r >> 2) + 4 * j + (r & 3); };
     // rows of unit stride are read 16 bytes at a time: along y directly, along z by one row a quad lane and a transpose
     const bool along_y = R.sy == 1;
     const int quad = along_y ? 0 : r & 3, s_y = along_y ? 1 : dz, s_z = along_y ? dy : 1;
@@ -501,7 +532,7 @@ __global__ void __launch_bounds__(64 * W * HEADS, walk_waves(ST, K, W, MODE)) wa
     auto turn_state = [&] {
         if (!along_y)
 #pragma unroll
-            for (int j = 0; j < 2; j++)
+            for (int j = 0; j < J; j++)
 #pragma unroll
                 for (int i = 0; i < 2 * K; i++) S[i][j] = quad_transpose(S[i][j]);
     };
@@ -510,14 +541,14 @@ __global__ void __launch_bounds__(64 * W * HEADS, walk_waves(ST, K, W, MODE)) wa
         if constexpr (MODE == BUFFER) {
             const Buf bs = buffer(s, 4 * dy * dz);
 #pragma unroll
-            for (int j = 0; j < 2; j++)
+            for (int j = 0; j < J; j++)
 #pragma unroll
                 for (int i = 0; i < 2 * K; i++) S[i][j] = buf_load4(bs, state_at(i, j));
             turn_state();
         } else {
             typedef Any<float> A;
 #pragma unroll
-            for (int j = 0; j < 2; j++)
+            for (int j = 0; j < J; j++)
 #pragma unroll
                 for (int i = 0; i < 2 * K; i++) {
                     int c;
@@ -526,7 +557,7 @@ __global__ void __launch_bounds__(64 * W * HEADS, walk_waves(ST, K, W, MODE)) wa
                     S[i][j] = s ? __builtin_bit_cast(f32x4, A::load(s + at, c, s_d)) : f32x4{0.f, 0.f, 0.f, 0.f};
                 }
 #pragma unroll
-            for (int j = 0; j < 2; j++)
+            for (int j = 0; j < J; j++)
 #pragma unroll
                 for (int i = 0; i < 2 * K; i++) {
                     int c;
@@ -561,7 +592,7 @@ __global__ void __launch_bounds__(64 * W * HEADS, walk_waves(ST, K, W, MODE)) wa
         if constexpr (OUTS) lay(tx[in_row / PER], PITCH, PLANE, ROWS, row, in_row * UNIT, dy, L, in_row % PER * UNIT, rx);
         lay(ty[in_row / PER], PITCH, PLANE, ROWS, row, in_row * UNIT, dy, L, in_row % PER * UNIT, ry);
         // (each wave's channels of z have a tile of their own)
-        lay(tz[in_rowz / PERZ][in_rowz % PERZ * UNIT / 32], 32, ZPLANE, ROWSZ, rowz, in_rowz * UNIT, dz, L, in_rowz * UNIT % 32, rz);
+        lay(tz[in_rowz / PERZ][in_rowz % PERZ * UNIT / Z], Z, ZPLANE, ROWSZ, rowz, in_rowz * UNIT, dz, L, in_rowz * UNIT % Z, rz);
         lds_barrier<B>();
         if (more) load_rows(n0 + CH);   // the chunk is in LDS: the registers take the next one's rows
         auto read = [&](const __bf16* m, int row, int k, bf16x8 (&o)[IN]) {
@@ -569,40 +600,51 @@ __global__ void __launch_bounds__(64 * W * HEADS, walk_waves(ST, K, W, MODE)) wa
             for (int i = 0; i < IN; i++) o[i] = *(const bf16x8*)(m + i * PLANE + row * PITCH + 32 * k + 8 * g);
         };
 
-        // ---- P^T: rows s (step row_of(t)), columns t (walk step 16 c + r).  Columns 16 c .. are formed by wave c (by the only
-        // one) for all
+        // ---- P^T: rows s (step row_of(t)), columns t (walk step 16 c + r).  Tile (t, c) is formed by wave 2 c + t for all
+        // where slices are thin and there are as many, else both of a column by wave c (or the only one)
         if constexpr (OUTS) {
+            constexpr bool QUARTERS = J == 1 && W >= 4;
+            constexpr int NT = QUARTERS ? 1 : 2;
 #pragma unroll
             for (int c = 0; c < 2; c++) {
-                if (W > 1 && wave != c) continue;
-                f32x4 p[2];
+                if (W > 1 && (QUARTERS ? wave >> 1 : wave) != c) continue;
+                const int t0 = QUARTERS ? wave & 1 : 0;
+                f32x4 p[NT];
 #pragma unroll
-                for (int t = 0; t < 2; t++) p[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+                for (int t = 0; t < NT; t++) p[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int k = 0; k < K; k++) {
                     bf16x8 x[IN], y[IN];
                     read(lx, 16 * c + r, k, x);
 #pragma unroll
-                    for (int t = 0; t < 2; t++) {
-                        read(ly, row_of(t), k, y);
+                    for (int t = 0; t < NT; t++) {
+                        read(ly, row_of(t0 + t), k, y);
                         mma(p[t], y, x);
                     }
                 }
-                f32x8 v = pair(p[0], p[1]);
-                float w[8];
+                float w[4 * NT];
 #pragma unroll
-                for (int j = 0; j < 8; j++) w[j] = pow_pair[CH - 1 + 16 * c + r - 8 * g - j];
+                for (int j = 0; j < 4 * NT; j++) w[j] = pow_pair[CH - 1 + 16 * c + r - 8 * g - 4 * t0 - j];
                 if (cut) {
-                    const int seen = last_cut(cuts_to(16 * c + r)) - 8 * g;
+                    const int seen = last_cut(cuts_to(16 * c + r)) - 8 * g - 4 * t0;
 #pragma unroll
-                    for (int j = 0; j < 8; j++) w[j] = j >= seen ? w[j] : 0.f;
+                    for (int j = 0; j < 4 * NT; j++) w[j] = j >= seen ? w[j] : 0.f;
                 }
 #pragma unroll
-                for (int j = 0; j < 8; j++) v[j] = mul0(v[j], w[j]);
-                bf16x8 parts[MID];
-                split(v, parts);
+                for (int t = 0; t < NT; t++)
 #pragma unroll
-                for (int u = 0; u < MID; u++) lp[c][u][l] = parts[u];
+                    for (int j = 0; j < 4; j++) p[t][j] = mul0(p[t][j], w[4 * t + j]);
+                if constexpr (QUARTERS) {
+                    bf16x4 parts[MID];
+                    split(p[0], parts);
+#pragma unroll
+                    for (int u = 0; u < MID; u++) ((bf16x4*)&lp[c][u][l])[t0] = parts[u];
+                } else {
+                    bf16x8 parts[MID];
+                    split(pair(p[0], p[1]), parts);
+#pragma unroll
+                    for (int u = 0; u < MID; u++) lp[c][u][l] = parts[u];
+                }
             }
             lds_barrier<B>();
         }
@@ -616,18 +658,18 @@ __global__ void __launch_bounds__(64 * W * HEADS, walk_waves(ST, K, W, MODE)) wa
 
         __builtin_amdgcn_sched_barrier(0);   // (what the scheduler would move across costs more registers than there are)
         if (dz0 < dz) {   // a wave behind z's channels only helps to load
-            bf16x8 T[2][IN];   // Z^T
+            bf16x8 T[J][IN];   // Z^T
 #pragma unroll
-            for (int j = 0; j < 2; j++)
+            for (int j = 0; j < J; j++)
 #pragma unroll
-                for (int i = 0; i < IN; i++) T[j][i] = column(lz + i * ZPLANE, 32, 8 * g, 4 * j, r);
+                for (int i = 0; i < IN; i++) T[j][i] = column<4 * J>(lz + i * ZPLANE, Z, 8 * g, 4 * j, r);
             // z values that are not finite: zeros to the products, and NaN to what sees them.  The steps at which a channel
             // has some go to odd[channel]
-            unsigned odd[2] = {0, 0};
-            const bool slow = __any((odd_bits(T[0][0]) | odd_bits(T[1][0])) != 0);
+            unsigned odd[J] = {};
+            const bool slow = __any((odd_bits(T[0][0]) | odd_bits(T[J - 1][0])) != 0);
             if (slow) {
 #pragma unroll
-                for (int j = 0; j < 2; j++) {
+                for (int j = 0; j < J; j++) {
 #pragma unroll
                     for (int e = 0; e < 8; e++) {
                         const bool is = (__builtin_bit_cast(unsigned short, (__bf16)T[j][0][e]) & 0x7f80) == 0x7f80;
@@ -637,24 +679,24 @@ __global__ void __launch_bounds__(64 * W * HEADS, walk_waves(ST, K, W, MODE)) wa
                     }
                     odd[j] |= __shfl_xor(odd[j], 16);
                     odd[j] |= __shfl_xor(odd[j], 32);
-                    if (g == 0) lodd[8 * (r >> 2) + 4 * j + (r & 3)] = odd[j];
+                    if (g == 0) lodd[4 * J * (r >> 2) + 4 * j + (r & 3)] = odd[j];
                 }
                 lds_barrier<1>();
             }
             // O^T: rows z channels, columns t
             if constexpr (OUTS) {
-                f32x4 o[2][2];
+                f32x4 o[2][J];
 #pragma unroll
                 for (int c = 0; c < 2; c++)
 #pragma unroll
-                    for (int j = 0; j < 2; j++) o[c][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+                    for (int j = 0; j < J; j++) o[c][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int k = 0; k < K; k++) {
                     bf16x8 x[2][IN];
                     read(lx, r, k, x[0]);
                     read(lx, 16 + r, k, x[1]);
 #pragma unroll
-                    for (int j = 0; j < 2; j++) {
+                    for (int j = 0; j < J; j++) {
                         bf16x8 sp[MID];
                         split(pair(S[2 * k][j], S[2 * k + 1][j]), sp);
 #pragma unroll
@@ -663,14 +705,14 @@ __global__ void __launch_bounds__(64 * W * HEADS, walk_waves(ST, K, W, MODE)) wa
                 }
 #pragma unroll
                 for (int c = 0; c < 2; c++) {
-                    const int n = 16 * c + r, d = dz0 + 8 * g;
+                    const int n = 16 * c + r, d = dz0 + 4 * J * g;
                     float wi = w_in[c];
                     if (cut) wi = cuts_to(n) ? 0.f : wi;
                     bf16x8 P[MID];
 #pragma unroll
                     for (int u = 0; u < MID; u++) P[u] = lp[c][u][l];
 #pragma unroll
-                    for (int j = 0; j < 2; j++) {
+                    for (int j = 0; j < J; j++) {
 #pragma unroll
                         for (int q = 0; q < 4; q++) o[c][j][q] = mul0(o[c][j][q], wi);
                         mma(o[c][j], T[j], P);
@@ -678,12 +720,16 @@ __global__ void __launch_bounds__(64 * W * HEADS, walk_waves(ST, K, W, MODE)) wa
                     if (slow) {
                         const unsigned sees = ((2u << n) - 1) & ~((1u << last_cut(cuts_to(n))) - 1);
 #pragma unroll
-                        for (int j = 0; j < 2; j++)
+                        for (int j = 0; j < J; j++)
 #pragma unroll
                             for (int q = 0; q < 4; q++)
-                                if (lodd[8 * g + 4 * j + q] & sees) o[c][j][q] = __builtin_nanf("");
+                                if (lodd[4 * J * g + 4 * j + q] & sees) o[c][j][q] = __builtin_nanf("");
                     }
-                    const f32x8 v = pair(o[c][0], o[c][1]);
+                    auto joined = [&] {
+                        if constexpr (J == 1) return o[c][0];
+                        else return pair(o[c][0], o[c][1]);
+                    };
+                    const auto v = joined();
                     if constexpr (MODE == BUFFER) {
                         const Buf bo = buffer(R.out.p ? (rev ? vo.at - (long)(L - 1) * vo.step : vo.at) : nullptr, (L - 1) * vo.step + vo.row);
                         int at = vo.off + ((rev ? (L - 1) * vo.step : 0) + dir * 16 * c * vo.step);
@@ -705,7 +751,7 @@ __global__ void __launch_bounds__(64 * W * HEADS, walk_waves(ST, K, W, MODE)) wa
 #pragma unroll
                 for (int i = 0; i < 2 * K; i++)
 #pragma unroll
-                    for (int j = 0; j < 2; j++)
+                    for (int j = 0; j < J; j++)
 #pragma unroll
                         for (int q = 0; q < 4; q++) S[i][j][q] = mul0(S[i][j][q], through);
                 float w[8];
@@ -714,9 +760,9 @@ __global__ void __launch_bounds__(64 * W * HEADS, walk_waves(ST, K, W, MODE)) wa
                 if (cut)
 #pragma unroll
                     for (int j = 0; j < 8; j++) w[j] = 8 * g + j >= leaving ? w[j] : 0.f;
-                bf16x8 zp[2][3];
+                bf16x8 zp[J][3];
 #pragma unroll
-                for (int j = 0; j < 2; j++) {
+                for (int j = 0; j < J; j++) {
                     f32x8 v = whole(T[j]);
 #pragma unroll
                     for (int q = 0; q < 8; q++) v[q] = mul0(v[q], w[q]);
@@ -726,14 +772,14 @@ __global__ void __launch_bounds__(64 * W * HEADS, walk_waves(ST, K, W, MODE)) wa
                 for (int i = 0; i < 2 * K; i++) {
                     bf16x8 y[IN];
 #pragma unroll
-                    for (int u = 0; u < IN; u++) y[u] = column(ly + u * PLANE, PITCH, 8 * g, 32 * (i >> 1) + 4 * (i & 1), r);
+                    for (int u = 0; u < IN; u++) y[u] = column<8>(ly + u * PLANE, PITCH, 8 * g, 32 * (i >> 1) + 4 * (i & 1), r);
 #pragma unroll
-                    for (int j = 0; j < 2; j++) mma(S[i][j], y, zp[j]);
+                    for (int j = 0; j < J; j++) mma(S[i][j], y, zp[j]);
                 }
                 if (slow) {
                     const unsigned sees = (unsigned)((1ull << L) - 1) & ~(unsigned)((1ull << leaving) - 1);
 #pragma unroll
-                    for (int j = 0; j < 2; j++)
+                    for (int j = 0; j < J; j++)
                         if (odd[j] & sees)
 #pragma unroll
                             for (int i = 0; i < 2 * K; i++)
@@ -746,12 +792,13 @@ __global__ void __launch_bounds__(64 * W * HEADS, walk_waves(ST, K, W, MODE)) wa
     }
 
     // ---- the steps behind the lane's length
-    if (OUTS && R.out.p && dz0 + 8 * g < dz)
+    typedef typename std::conditional<J == 1, f32x4, f32x8>::type Zero;
+    if (OUTS && R.out.p && dz0 + 4 * J * g < dz)
         for (int n = (len > seg0 ? len : seg0) + r; n < seg1; n += 16) {
-            const int d = dz0 + 8 * g;
+            const int d = dz0 + 4 * J * g;
             const long at = head_of(R.out, h) + (long)n * R.out.step + d;
-            if (R.out_f32) store_some<HUM_F32>(R.out.p, at, dz - d, f32x8{});
-            else store_some<ST>(R.out.p, at, dz - d, f32x8{});
+            if (R.out_f32) store_some<HUM_F32>(R.out.p, at, dz - d, Zero{});
+            else store_some<ST>(R.out.p, at, dz - d, Zero{});
         }
     if (R.through && wave == 0 && l == 0) R.through[unit * a.segs + seg] = passed;
     if (R.state_out && (!a.last_only || seg + 1 == a.segs)) {
@@ -760,13 +807,13 @@ __global__ void __launch_bounds__(64 * W * HEADS, walk_waves(ST, K, W, MODE)) wa
             const Buf bs = buffer(s, 4 * dy * dz);
             turn_state();
 #pragma unroll
-            for (int j = 0; j < 2; j++)
+            for (int j = 0; j < J; j++)
 #pragma unroll
                 for (int i = 0; i < 2 * K; i++) buf_store4(bs, state_at(i, j), S[i][j]);
         } else {
             turn_state();
 #pragma unroll
-            for (int j = 0; j < 2; j++)
+            for (int j = 0; j < J; j++)
 #pragma unroll
                 for (int i = 0; i < 2 * K; i++) {
                     int c;
@@ -1002,32 +1049,45 @@ int check_args(const char* fn, const hum_decay_attn_args* p) {
 }
 
 int in_32(int d) { return d <= 32 ? 1 : d <= 64 ? 2 : 4; }
+template <int ST, int K, int W, int J, int HEADS, Mode MODE, bool OUTS>
+void launch_walk_j(const WalkArgs& a, hipStream_t s) {
+    const long n = (long)a.lanes * a.heads / HEADS * a.segs;
+    const dim3 grid((unsigned)((n + XCDS * NEAR - 1) / (XCDS * NEAR) * (XCDS * NEAR) * a.nroles));
+    hipLaunchKernelGGL((walk_kernel<ST, K, W, J, HEADS, MODE, OUTS>), grid, dim3(64 * W * HEADS), 0, s, a);
+}
+// W waves of 32 of z's channels, or 2 W of 16: half of a wave's part of a chunk, while a head's rows are read from LDS twice
+// as often.  Thin slices are faster while a wave of 32 channels has a SIMD of its own (thin: bf16, 4 heads x 64 x 64, 200 steps,
+// 64 lanes: 21.4 us with wide slices, 18.5; 128 lanes 25.7 and 22.8, 512 lanes 62 and 64), and always for types of several
+// parts (float32, 512 lanes: 146 and 125 us) and where the registers of wide slices leave a SIMD two waves or one (float16,
+// 1024 lanes x 100 steps x 127 channels: 609 and 428 us; bf16 63 channels 121 and 116, gradient 272 and 257).
 template <int ST, int K, int W, bool OUTS>
-void launch_walk_o(const WalkArgs& a, Mode mode, bool together, hipStream_t s) {
-    // 4 waves a workgroup from as many heads as that takes, where keys and values are equally wide; a float32 head's rows
-    // fill enough of the LDS by themselves
-    constexpr int H = ST == HUM_F32 || K != W ? 1 : 4 / W;
-    auto grid = [&](int heads) {
-        const long n = (long)a.lanes * a.heads / heads * a.segs;
-        return dim3((unsigned)((n + XCDS * NEAR - 1) / (XCDS * NEAR) * (XCDS * NEAR) * a.nroles));
-    };
-    if (mode == BUFFER && together && a.heads % H == 0) hipLaunchKernelGGL((walk_kernel<ST, K, W, H, BUFFER, OUTS>), grid(H), dim3(64 * W * H), 0, s, a);
-    else if (mode == BUFFER) hipLaunchKernelGGL((walk_kernel<ST, K, W, 1, BUFFER, OUTS>), grid(1), dim3(64 * W), 0, s, a);
-    else if constexpr (K == W) {
-        if (mode == WIDE) hipLaunchKernelGGL((walk_kernel<ST, K, W, 1, WIDE, OUTS>), grid(1), dim3(64 * W), 0, s, a);
-        else hipLaunchKernelGGL((walk_kernel<ST, K, W, 1, ANY, OUTS>), grid(1), dim3(64 * W), 0, s, a);
+void launch_walk_o(const WalkArgs& a, Mode mode, bool together, bool thin, hipStream_t s) {
+    if (mode == BUFFER) {
+        if constexpr (ST == HUM_BF16 || (ST == HUM_F16 && K > 2))
+            if (!thin) {
+                // 4 waves a workgroup from as many heads as that takes, where keys and values are equally wide
+                constexpr int H = ST != HUM_BF16 || K != W ? 1 : 4 / W;
+                if (together && a.heads % H == 0) return launch_walk_j<ST, K, W, 2, H, BUFFER, OUTS>(a, s);
+                return launch_walk_j<ST, K, W, 2, 1, BUFFER, OUTS>(a, s);
+            }
+        launch_walk_j<ST, K, 2 * W, 1, 1, BUFFER, OUTS>(a, s);
+    } else if constexpr (K == W) {
+        if constexpr (ST == HUM_BF16 && K > 2)
+            if (mode == WIDE && !thin) return launch_walk_j<ST, K, W, 2, 1, WIDE, OUTS>(a, s);
+        if (mode == WIDE) launch_walk_j<ST, K, 2 * W, 1, 1, WIDE, OUTS>(a, s);
+        else launch_walk_j<ST, K, 2 * W, 1, 1, ANY, OUTS>(a, s);
     }
 }
 template <int ST, int K, int W>
-void launch_walk_w(const WalkArgs& a, Mode mode, bool together, hipStream_t s) {
-    if (a.r[0].x.p) launch_walk_o<ST, K, W, true>(a, mode, together, s);
-    else launch_walk_o<ST, K, W, false>(a, mode, together, s);
+void launch_walk_w(const WalkArgs& a, Mode mode, bool together, bool thin, hipStream_t s) {
+    if (a.r[0].x.p) launch_walk_o<ST, K, W, true>(a, mode, together, thin, s);
+    else launch_walk_o<ST, K, W, false>(a, mode, together, thin, s);
 }
 template <int ST, int K>
-void launch_walk_k(const WalkArgs& a, int w, Mode mode, bool together, hipStream_t s) {
-    if (w == 1) launch_walk_w<ST, K, 1>(a, mode, together, s);
-    else if (w == 2) launch_walk_w<ST, K, 2>(a, mode, together, s);
-    else launch_walk_w<ST, K, 4>(a, mode, together, s);
+void launch_walk_k(const WalkArgs& a, int w, Mode mode, bool together, bool thin, hipStream_t s) {
+    if (w == 1) launch_walk_w<ST, K, 1>(a, mode, together, thin, s);
+    else if (w == 2) launch_walk_w<ST, K, 2>(a, mode, together, thin, s);
+    else launch_walk_w<ST, K, 4>(a, mode, together, thin, s);
 }
 template <int ST>
 void launch_walk_t(const WalkArgs& a, hipStream_t s) {
@@ -1045,9 +1105,10 @@ void launch_walk_t(const WalkArgs& a, hipStream_t s) {
     int k = in_32(a.r[0].dy), w = in_32(a.r[0].dz);
     const Mode mode = buffers ? BUFFER : wide ? WIDE : ANY;
     if (mode != BUFFER) k = w = k > w ? k : w;   // (those are built for squares only)
-    if (k == 1) launch_walk_k<ST, 1>(a, w, mode, together, s);
-    else if (k == 2) launch_walk_k<ST, 2>(a, w, mode, together, s);
-    else launch_walk_k<ST, 4>(a, w, mode, together, s);
+    const bool thin = (long)a.lanes * a.heads * a.segs * a.nroles * w <= 1024;
+    if (k == 1) launch_walk_k<ST, 1>(a, w, mode, together, thin, s);
+    else if (k == 2) launch_walk_k<ST, 2>(a, w, mode, together, thin, s);
+    else launch_walk_k<ST, 4>(a, w, mode, together, thin, s);
 }
 
 // Few lanes and many steps: the walks are cut into segments that run side by side, each from the state that a first pass

@@ -7,6 +7,8 @@ sums over the steps, the decays' powers (one exp2 of a product, at most 32 steps
 `size`; at most C = 128 + steps + 64 of them lie on one path.  bf16 operands formed from float32 values are split in two
 parts, whose remainder is 2^-18 of the value; three such operands meet on a path at most.  The result's own rounding is
 half a step, eps / 2 of its value (fp16: at least half its smallest number, 2^-25)."""
+import copy
+
 import pytest
 
 pytestmark = pytest.mark.gpu
@@ -146,6 +148,58 @@ def test_steps_far_apart(h, g, d, kind):
     c = Case(3, 70, h, g, d, d, kind=kind, order="time", resets=0.04, lengths=[70, 41, 0], far=32768 + 64)
     c.check_forward()
     c.check_backward()
+
+
+def check_many(c, n):
+    """The case's lanes n times over: every copy is the first, and the first is right."""
+    def many(x):
+        if x is None:
+            return None
+        if x.dim() == 4 and x.stride(0) < x.stride(1):   # time-major
+            return x.transpose(0, 1).repeat(1, n, 1, 1).transpose(0, 1)
+        return x.repeat(n, *[1] * (x.dim() - 1))
+    big = copy.copy(c)
+    for name in ("q", "k", "v", "d_out", "state", "d_state", "reset", "lengths"):
+        setattr(big, name, many(getattr(c, name)))
+    b = c.q.shape[0]
+    got, grads = big.forward(), big.backward()
+    for x in got + grads:
+        copies = x.reshape(n, b, *x.shape[1:])
+        assert torch.equal(copies, copies[:1].expand_as(copies))
+    c.check_forward(tuple(x[:b] for x in got))
+    c.check_backward(tuple(x[:b] for x in grads))
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp32", "fp16"])
+@pytest.mark.parametrize("dk,dv", [(32, 32), (32, 64), (16, 128), (64, 24), (64, 64), (48, 128), (128, 32), (128, 64), (120, 128), (99, 127), (31, 63)])
+def test_more_walks_than_the_card_has_waves(dk, dv, kind):
+    """Batches of thousands of walks (each wave has wider slices there, for some types and widths)."""
+    check_many(Case(3, 43, 2, 1, dk, dv, kind=kind, resets=0.05, lengths=[43, 0, 34]), 240)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp16"])
+@pytest.mark.parametrize("h,g,d", [(4, 4, 64), (4, 1, 64), (4, 2, 32), (8, 8, 32), (3, 3, 64), (2, 2, 128)])
+def test_many_walks_of_steps_far_apart(h, g, d, kind):
+    """The same time-major, 64 KB and more from a step to the next (a workgroup takes several heads)."""
+    check_many(Case(4, 37, h, g, d, d, kind=kind, order="time", resets=0.04, lengths=[37, 20, 0, 33]), 130)
+
+
+@pytest.mark.parametrize("kind,dk,dv", [("bf16", 64, 64), ("bf16", 128, 128), ("fp16", 128, 128), ("bf16", 127, 99)])
+def test_many_walks_meet_values_that_are_not_finite(kind, dk, dv):
+    c = Case(2, 50, 2, 2, dk, dv, kind=kind, state=False)
+    c.reset = torch.zeros(2, 50, dtype=torch.uint8, device=DEV)
+    c.reset[:, 40] = 1
+    c.v[1, 36, :, 3] = float("inf")
+    q, k, v = (x.repeat(300, 1, 1, 1) for x in (c.q, c.k, c.v))
+    got, state = M.decay_attention(q, k, v, c.log_decay, reset=c.reset.repeat(300, 1), scale=c.scale)
+    few, few_state = M.decay_attention(c.q, c.k, c.v, c.log_decay, reset=c.reset, scale=c.scale)
+    for x, y in ((got, few), (state, few_state)):
+        bad = ~x.reshape(300, *y.shape).isfinite()
+        assert torch.equal(bad, (~y.isfinite()).expand_as(bad))
+    bad = ~got.isfinite()
+    want = torch.zeros_like(bad)
+    want[1::2, 36:40, :, 3] = True
+    assert torch.equal(bad, want) and state.isfinite().all()
 
 
 @pytest.mark.parametrize("steps", [700, 1500])
