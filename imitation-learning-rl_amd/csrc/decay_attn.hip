@@ -1060,8 +1060,11 @@ void launch_walk_j(const WalkArgs& a, hipStream_t s) {
 // 64 lanes: 21.4 us with wide slices, 18.5; 128 lanes 25.7 and 22.8, 512 lanes 62 and 64), and always for types of several
 // parts (float32, 512 lanes: 146 and 125 us) and where the registers of wide slices leave a SIMD two waves or one (float16,
 // 1024 lanes x 100 steps x 127 channels: 609 and 428 us; bf16 63 channels 121 and 116, gradient 272 and 257).
+// Rows of more than 64 channels are work for four waves to load and to form P of, also where z has fewer channels than they
+// could hold (float32, 128 x 32 channels, 64 lanes x 100 steps: 28.9 us with two waves, 24.8 with four).
 template <int ST, int K, int W, bool OUTS>
 void launch_walk_o(const WalkArgs& a, Mode mode, bool together, bool thin, hipStream_t s) {
+    constexpr int THIN = K > 2 && W == 1 ? 4 : 2 * W;
     if (mode == BUFFER) {
         if constexpr (ST == HUM_BF16 || (ST == HUM_F16 && K > 2))
             if (!thin) {
@@ -1070,12 +1073,13 @@ void launch_walk_o(const WalkArgs& a, Mode mode, bool together, bool thin, hipSt
                 if (together && a.heads % H == 0) return launch_walk_j<ST, K, W, 2, H, BUFFER, OUTS>(a, s);
                 return launch_walk_j<ST, K, W, 2, 1, BUFFER, OUTS>(a, s);
             }
-        launch_walk_j<ST, K, 2 * W, 1, 1, BUFFER, OUTS>(a, s);
+        launch_walk_j<ST, K, THIN, 1, 1, BUFFER, OUTS>(a, s);
+    } else if (mode == WIDE) {
+        if constexpr (ST == HUM_BF16 && K > 2 && W > 2)
+            if (!thin) return launch_walk_j<ST, K, W, 2, 1, WIDE, OUTS>(a, s);
+        launch_walk_j<ST, K, THIN, 1, 1, WIDE, OUTS>(a, s);
     } else if constexpr (K == W) {
-        if constexpr (ST == HUM_BF16 && K > 2)
-            if (mode == WIDE && !thin) return launch_walk_j<ST, K, W, 2, 1, WIDE, OUTS>(a, s);
-        if (mode == WIDE) launch_walk_j<ST, K, 2 * W, 1, 1, WIDE, OUTS>(a, s);
-        else launch_walk_j<ST, K, 2 * W, 1, 1, ANY, OUTS>(a, s);
+        launch_walk_j<ST, K, THIN, 1, 1, ANY, OUTS>(a, s);
     }
 }
 template <int ST, int K, int W>
@@ -1104,7 +1108,7 @@ void launch_walk_t(const WalkArgs& a, hipStream_t s) {
     }
     int k = in_32(a.r[0].dy), w = in_32(a.r[0].dz);
     const Mode mode = buffers ? BUFFER : wide ? WIDE : ANY;
-    if (mode != BUFFER) k = w = k > w ? k : w;   // (those are built for squares only)
+    if (mode == ANY) k = w = k > w ? k : w;   // (that is built for squares only)
     const bool thin = (long)a.lanes * a.heads * a.segs * a.nroles * w <= 1024;
     if (k == 1) launch_walk_k<ST, 1>(a, w, mode, together, thin, s);
     else if (k == 2) launch_walk_k<ST, 2>(a, w, mode, together, thin, s);
@@ -1112,15 +1116,25 @@ void launch_walk_t(const WalkArgs& a, hipStream_t s) {
 }
 
 // Few lanes and many steps: the walks are cut into segments that run side by side, each from the state that a first pass
-// over the segments before it and a scan have left for it (segments without outputs: half the work of a walk).
+// over the segments before it and a scan have left for it (segments without outputs: half the work of a walk).  Longer
+// walks have longer segments (each has a state in memory and a turn in the scan) and more of them side by side; walks
+// that would be cut into few, or are short, do not gain what the first pass and two launches cost.  Averages over types,
+// widths of 32 to 128 and both directions, against the best cut of each case:
+//     12 to 24 chunks,  8 waves: uncut 2.34, segments of 1 chunk 1.00, of 4 1.67;  256 waves: uncut 1.02, up to 2048 waves 1.29
+//     32 chunks, 256 waves: uncut 1.09, 2048 waves 1.11;  63 chunks, 256 waves: uncut 1.25, 2048 1.09, 4096 1.06
+//     125 chunks, 512 waves: uncut 1.06, 4096 1.02;  250 chunks, 16 waves: segments of 1 chunk 1.13, 2 1.10, 3 1.00, 4 1.09
 struct Cut { int segs, steps; };
-constexpr int WAVES = 4096, MIN_CHUNKS = 4;   // four waves per SIMD; segments of 4 chunks at least
-Cut cut_of(const hum_decay_attn_args* p, int each) {   // waves of a (lane, head)
-    const long waves = (long)p->lanes * p->heads * each;
-    const int chunks = (p->steps + CH - 1) / CH;
-    if (waves == 0 || 2 * waves > WAVES || chunks < 2 * MIN_CHUNKS) return {1, p->steps};
-    long segs = WAVES / waves;
-    if (segs > chunks / MIN_CHUNKS) segs = chunks / MIN_CHUNKS;
+Cut cut_of(const hum_decay_attn_args* p, int walks) {   // of a (lane, head)
+    // in waves of 32 x 32 channels; uneven widths (10 lanes x 7 heads x 907 steps of 117 and 22 channels, float16 gradient:
+    // 206 us uncut, 154 cut) take the mean of theirs
+    const double waves = (double)p->lanes * p->heads * walks * std::sqrt((double)(in_32(p->dk) * in_32(p->dv)));
+    const int chunks = (p->steps + CH - 1) / CH, least = chunks < 32 ? 1 : chunks < 128 ? 2 : 3;
+    const int most = chunks < 48 ? 2048 : 4096;
+    const bool parts = p->type != HUM_BF16;   // chunks take longer: 29 of them are cut into 5 segments too
+    if (waves == 0 || chunks < (parts ? 8 : 12) || waves * (chunks >= 96 ? 4 : parts && chunks >= 20 && chunks < 48 ? 4.5 : 8) > most)
+        return {1, p->steps};
+    long segs = (long)(most / waves);
+    if (segs > chunks / least) segs = chunks / least;
     const int per = (int)((chunks + segs - 1) / segs);
     return {(chunks + per - 1) / per, per * CH};
 }
@@ -1200,8 +1214,8 @@ void enter_segments(Role& r, const float* scratch, const hum_decay_attn_args* p,
     r.in_unit = (long)p->dk * p->dv * c.segs;
     r.in_seg = (long)p->dk * p->dv;
 }
-Cut forward_cut(const hum_decay_attn_args* p) { return cut_of(p, in_32(p->dv)); }
-Cut backward_cut(const hum_decay_attn_args* p) { return cut_of(p, 2 * in_32(p->dk) + in_32(p->dv)); }
+Cut forward_cut(const hum_decay_attn_args* p) { return cut_of(p, 1); }
+Cut backward_cut(const hum_decay_attn_args* p) { return cut_of(p, 3); }
 
 int launched(const char* fn) {
     const hipError_t st = hipGetLastError();
