@@ -434,7 +434,7 @@ __global__ void __launch_bounds__(64 * W * HEADS, walk_waves(ST, K, W, MODE)) wa
         v.at = (const char*)m.p + (head_of(m, h0) + (long)time(seg0) * m.step) * size;
         v.hop = (long)dir * CH * v.step;
         v.row = place(HEADS - 1) + d * size;
-        v.off = channel < d ? dir * row * v.step + place(head) + channel * size : OUTSIDE;
+        v.off = channel < d && row < CH ? dir * row * v.step + place(head) + channel * size : OUTSIDE;   // (8 waves load 64 rows)
         return v;
     };
     auto chunk = [&](const View& v, int L) { return buffer(rev ? v.at - (long)(L - 1) * v.step : v.at, (L - 1) * v.step + v.row); };
@@ -1048,6 +1048,12 @@ int check_args(const char* fn, const hum_decay_attn_args* p) {
     return HUM_OK;
 }
 
+// two states share memory
+bool meet(const hum_decay_attn_args* p, const float* a, const float* b) {
+    const uint64_t size = 4ull * p->lanes * p->heads * p->dk * p->dv;
+    return a && b && (uintptr_t)a < (uintptr_t)b + size && (uintptr_t)b < (uintptr_t)a + size;
+}
+
 int in_32(int d) { return d <= 32 ? 1 : d <= 64 ? 2 : 4; }
 template <int ST, int K, int W, int J, int HEADS, Mode MODE, bool OUTS>
 void launch_walk_j(const WalkArgs& a, hipStream_t s) {
@@ -1241,6 +1247,8 @@ int hum_decay_attn(const hum_decay_attn_args* p, const hum_rows* out, void* work
     if (const int rc = check_args(fn, p)) return rc;
     if (!out || (p->lanes && p->steps && !out->ptr) || ((uintptr_t)out->ptr) % elem_size(p->type))
         return derr(HUM_ERR_ARG, fn, "out is required, aligned to its elements");
+    if (p->state_in != p->state_out && meet(p, p->state_in, p->state_out))
+        return derr(HUM_ERR_ARG, fn, "state_out must be state_in or not overlap it");
     uint64_t need = 0;
     if (const int rc = hum_decay_attn_workspace(p, 0, &need)) return rc;
     if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
@@ -1288,11 +1296,7 @@ int hum_decay_attn_backward(const hum_decay_attn_args* p, const hum_rows* d_out,
     if (const int rc = hum_decay_attn_workspace(p, 1, &need)) return rc;
     if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
         return derr(HUM_ERR_ARG, fn, "the workspace is too small (hum_decay_attn_workspace) or not aligned to 16 bytes");
-    const uint64_t state = 4ull * p->lanes * p->heads * p->dk * p->dv;
-    auto meets = [&](const float* a, const float* b) {
-        return a && b && (uintptr_t)a < (uintptr_t)b + state && (uintptr_t)b < (uintptr_t)a + state;
-    };
-    if (meets(d_state_in, d_state_out) || meets(d_state_in, p->state_in))
+    if (meet(p, d_state_in, d_state_out) || meet(p, d_state_in, p->state_in))
         return derr(HUM_ERR_ARG, fn, "d_state_in must not overlap state_in or d_state_out");
     if (!p->lanes) return HUM_OK;
     const OnDevice dev(p->device);
@@ -1405,6 +1409,8 @@ extern "C" int hum_decay_attn_step(const hum_decay_attn_args* p, const uint8_t* 
     if (p->steps != 1 || p->lengths) return derr(HUM_ERR_ARG, fn, "steps must be 1 and lengths NULL (active says which lanes step)");
     if (!out || (p->lanes && (!out->ptr || !p->state_out)) || ((uintptr_t)out->ptr) % elem_size(p->type))
         return derr(HUM_ERR_ARG, fn, "out (aligned to its elements) and state_out are required");
+    if (p->state_in != p->state_out && meet(p, p->state_in, p->state_out))
+        return derr(HUM_ERR_ARG, fn, "state_out must be state_in or not overlap it");
     if (!p->lanes) return HUM_OK;
     const OnDevice dev(p->device);
     if (!dev.ok) return derr(HUM_ERR_HIP, fn, "hipSetDevice");

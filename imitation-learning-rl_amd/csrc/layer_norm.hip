@@ -401,6 +401,14 @@ int check_sizes(const char* fn, const hum_norm_args* p) {
 bool near(int64_t row, int size) { return row >= 0 && row < (1l << 28) / size; }
 bool aligned(const void* p, int64_t row, int size) { return ((uintptr_t)p | (uintptr_t)(row * size)) % 16 == 0; }
 
+// rows that are written must lie apart, and over the rows they replace if they begin with them
+bool apart(const hum_norm_args* p, const void* out, int64_t row) {
+    return p->rows < 2 || !out || row >= p->channels || row <= -(int64_t)p->channels;
+}
+bool replaces(const hum_norm_args* p, const void* out, int64_t row, const void* in, int64_t in_row) {
+    return p->rows < 2 || !out || out != in || row == in_row;
+}
+
 int launched(const char* fn) {
     const hipError_t st = hipGetLastError();
     return st == hipSuccess ? HUM_OK : nerr(HUM_ERR_HIP, fn, hipGetErrorString(st));
@@ -416,6 +424,8 @@ int hum_layer_norm(const hum_norm_args* p, const void* bias, float eps, void* y,
     if (const int rc = check_sizes(fn, p)) return rc;
     const int es = p->type == HUM_F32 ? 4 : 2, ps = p->param_type == HUM_F32 ? 4 : 2;
     if ((p->rows && !y) || (uintptr_t)y % es || (uintptr_t)bias % ps) return nerr(HUM_ERR_ARG, fn, "y is required; rows and parameters must be aligned to their elements");
+    if (!apart(p, y, y_row) || !replaces(p, y, y_row, p->x, p->x_row))
+        return nerr(HUM_ERR_ARG, fn, "rows of y must not overlap, and have x's stride if y is x");
     if (!mean != !rstd) return nerr(HUM_ERR_ARG, fn, "mean and rstd are wanted together");
     if (((uintptr_t)mean | (uintptr_t)rstd) % 4) return nerr(HUM_ERR_ARG, fn, "mean and rstd must be aligned to 4 bytes");
     if (!(eps >= 0.f) || !std::isfinite(eps)) return nerr(HUM_ERR_ARG, fn, "eps must be finite and >= 0");
@@ -449,6 +459,8 @@ int hum_layer_norm_backward(const hum_norm_args* p, const void* dy, int64_t dy_r
     if (p->rows && (!dy || !mean || !rstd)) return nerr(HUM_ERR_ARG, fn, "dy, mean and rstd are required");
     if (((uintptr_t)dy | (uintptr_t)dx) % es || ((uintptr_t)d_weight | (uintptr_t)d_bias) % ps || ((uintptr_t)mean | (uintptr_t)rstd) % 4)
         return nerr(HUM_ERR_ARG, fn, "rows, statistics and parameters must be aligned to their elements");
+    if (!apart(p, dx, dx_row) || !replaces(p, dx, dx_row, p->x, p->x_row) || !replaces(p, dx, dx_row, dy, dy_row))
+        return nerr(HUM_ERR_ARG, fn, "rows of dx must not overlap, and have x's or dy's stride if dx is one of them");
     const Shape sh = shape_of(p->channels, near(p->x_row, es) && near(dy_row, es) && near(dx_row, es));
     const bool params = d_weight || d_bias;
     uint64_t need = 0;

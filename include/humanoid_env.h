@@ -480,7 +480,7 @@ typedef struct {
     const float* log_decay;      /* [heads] */
     hum_rows q, k, v;
     const float* state_in;       /* [lanes, heads, dv, dk], contiguous; NULL = zeros */
-    float* state_out;            /* the same, may be state_in; NULL = not wanted */
+    float* state_out;            /* the same, may be state_in (else they must not overlap); NULL = not wanted */
     const uint8_t* reset;        /* element [lane, step] at lane * reset_lane + step * reset_step; NULL = none */
     int64_t reset_lane, reset_step;
     const int32_t* lengths;      /* [lanes], clamped to [0, steps]; NULL = all steps */
@@ -503,7 +503,7 @@ int hum_decay_attn_step(const hum_decay_attn_args* args, const uint8_t* active, 
 /* Layer norm over the channels of each row: y = (x - mean) rstd weight + bias, rstd = 1 / sqrt(var + eps), sums in
  * float32.  x [rows, channels] of element type `type`, x_row elements from one row to the next, channels adjacent (the
  * same holds for y, dy and dx with their own); weight, bias [channels] of param_type (HUM_F32 or `type`); NULL weight =
- * ones, NULL bias = zeros.  y may be x. */
+ * ones, NULL bias = zeros.  y may be x, row for row. */
 typedef struct {
     int32_t device, type, param_type, channels;   /* channels in [1, 16384] */
     int64_t rows, x_row;
@@ -515,7 +515,7 @@ int hum_layer_norm(const hum_norm_args* args, const void* bias, float eps, void*
                    float* rstd, void* stream);
 /* bytes of scratch hum_layer_norm_backward needs when d_weight or d_bias is wanted */
 int hum_layer_norm_workspace(const hum_norm_args* args, uint64_t* bytes);
-/* dx [rows, channels], d_weight and d_bias [channels] of param_type, each may be NULL; dx may be dy or x.  The
+/* dx [rows, channels], d_weight and d_bias [channels] of param_type, each may be NULL; dx may be dy or x, row for row.  The
  * parameter gradients are summed in a fixed order: the same inputs give the same bits. */
 int hum_layer_norm_backward(const hum_norm_args* args, const void* dy, int64_t dy_row, const float* mean,
                             const float* rstd, void* dx, int64_t dx_row, void* d_weight, void* d_bias, void* workspace,

@@ -147,6 +147,22 @@ def test_norm_entry_points_refuse():
     assert L.hum_layer_norm(r(_norm(rows=0, x=None)), None, 1e-5, None, 64, None, None, None) == 0
 
 
+def test_outputs_that_overlap_what_is_still_read():
+    L, r, out = N.lib(), ctypes.byref, N.HumRows(0x1000, 64, 64, 8)
+
+    def refused(rc, text):
+        assert rc == N.HUM_ERR_ARG and text in L.hum_last_error(), L.hum_last_error()
+    size = 4 * 2 * 4 * 8 * 8
+    for at in (0x100004, 0x100000 + size - 4, 0x100000 - size + 4):
+        refused(L.hum_decay_attn(r(_attn(state_in=0x100000, state_out=at)), r(out), None, 0, None), b"overlap")
+        refused(L.hum_decay_attn_step(r(_attn(steps=1, state_in=0x100000, state_out=at)), None, r(out), None), b"overlap")
+    a = _norm(x_row=80)
+    for y, row in ((0x1000, 64), (0x1000, 96), (0x9000, 63), (0x9000, 0), (0x9000, -63)):
+        refused(L.hum_layer_norm(r(a), None, 1e-5, y, row, None, None, None), b"overlap")
+        refused(L.hum_layer_norm_backward(r(a), 0x5000, 64, 0x4000, 0x4000, y, row, None, None, None, 0, None), b"overlap")
+    refused(L.hum_layer_norm_backward(r(a), 0x5000, 64, 0x4000, 0x4000, 0x5000, 80, None, None, None, 0, None), b"overlap")
+
+
 def test_front_refuses_cpu_tensors():
     from ilrl_amd import memory as M
     x = torch.zeros(2, 3, 4, 8)
