@@ -495,6 +495,34 @@ def test_norm_and_gradient(rows, c, kind):
         assert all(torch.equal(p, q) for p, q in zip((dx, dw, db), again))
 
 
+@pytest.mark.parametrize("kind", ["bf16", "fp32", "fp16"])
+@pytest.mark.parametrize("rows,c", [(5, 1), (7, 3), (70, 4), (9, 6), (13, 9), (40, 15), (21, 63), (300, 65), (11, 250), (37, 511), (6, 1030),
+                                    (5, 1537), (3, 3001), (3, 6003), (2, 12001)])
+def test_norm_rows_that_end_inside_a_load(rows, c, kind):
+    """Rows of any width at any alignment, cut out of a buffer of NaN, and parameters that begin anywhere: the results are
+    those of the same rows by themselves, to the rounding of another order of the sums; nothing beside a row is read or
+    written."""
+    r = torch.Generator().manual_seed(rows * 31 + c)
+    dt = TYPES[kind]
+
+    def cut(*shape, type=dt):
+        x = torch.randn(shape, generator=r).to(type).to(DEV)
+        wide = torch.full((*shape[:-1], c + 3), float("nan"), dtype=type, device=DEV)
+        wide[..., 1:1 + c] = x
+        return wide[..., 1:1 + c]
+    x, dy = cut(rows, c), cut(rows, c)
+    for pd in (torch.float32, dt):
+        w, b = cut(c, type=pd), cut(c, type=pd)
+        y, mean, rstd = M.layer_norm_forward(x, w, b)
+        want = R.norm(x, w, b, 1e-5)
+        assert ((y.double().cpu() - want).abs() <= norm_bounds(x, w, b, want, kind)).all()
+        dx, dw, db = M.layer_norm_backward(dy, x, mean, rstd, w)
+        for got in (dx, dw, db):
+            assert got.isfinite().all()
+        one = M.layer_norm_backward(dy[:1].clone(), x[:1].clone(), mean[:1].clone(), rstd[:1].clone(), w.clone())[0]
+        torch.testing.assert_close(dx[:1], one, atol=0.0, rtol=0.0)
+
+
 def test_norm_without_parameters_empty_and_in_place():
     x = torch.randn(4, 3, 48, device=DEV)
     y = M.layer_norm(x)
