@@ -16,7 +16,7 @@
 // P = (Y X^T) masked and weighted by D, O^T = Z^T P + S^T X^T, S = lambda^32 S + (w Y)^T Z.  A workgroup owns one (lane,
 // head); each of its waves owns 32 of z's channels and keeps its slice of S in registers for the whole walk.  The chunk's
 // rows come into registers while the chunk before is worked on, and from there into LDS, where all waves read them; P is
-// formed by one wave for each half of its columns and shared through LDS.  The rows of every A operand are taken in the order
+// formed by two or four of the waves and shared through LDS.  The rows of every A operand are taken in the order
 //     matrix row m of tile a  <->  index 8 (m >> 2) + 4 a + (m & 3)   (of 32)
 // under which the accumulators of a pair of tiles (lane group g holds rows 4 g .. 4 g + 3 of each) are exactly the 8
 // consecutive contraction indexes 8 g .. 8 g + 7 that lane group needs as an operand of the next product: S feeds O, and P

@@ -463,6 +463,36 @@ def norm_bounds(x, w, b, y, kind):
     return HALF[kind] * y.abs() * 1.01 + wa * dh + 4 * U * (wa * h.abs() + ba) + (2.0 ** -25 if kind == "fp16" else 0)
 
 
+def test_captured_gradients_follow_their_inputs():
+    """Forward and gradient through autograd, captured together: every replay is the eager result for the inputs of then."""
+    c = Case(4, 70, 4, 2, 32, 64, kind="bf16", resets=0.05, order="time")
+    x, w = torch.randn(90, 64, device=DEV), torch.randn(64, device=DEV)
+    leaves = [t.detach().clone().requires_grad_(True) for t in (c.q, c.k, c.v, c.state, x, w)]
+
+    def step():
+        q, k, v, s, x, w = leaves
+        out, state = M.decay_attention(q, k, v, c.log_decay, state=s, reset=c.reset, scale=c.scale)
+        y = M.layer_norm(x, w)
+        return torch.autograd.grad((out, state, y), leaves, (c.d_out, c.d_state, y.detach()))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()   # (its graph is gone with its results)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        grads = step()
+    for turn in range(3):
+        with torch.no_grad():
+            for i, t in enumerate(leaves):
+                t.copy_(torch.randn(t.shape, generator=torch.Generator().manual_seed(10 * turn + i)).to(t.dtype))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [g.clone() for g in grads]
+        for a, e in zip(got, step()):
+            assert torch.equal(a, e)
+
+
 NORMS = [(1, 70), (3, 1), (5, 7), (1000, 64), (17, 44), (33, 128), (257, 256), (9, 257), (40, 512), (6, 1000), (5, 2048), (3, 4096), (2, 5000),
          (3, 8192), (2, 16384), (4, 9001), (2500, 32)]
 
