@@ -54,6 +54,7 @@ class _Entry:
         self.norm_workspace = bind("hum_layer_norm_workspace", b, need)
         self.norm_backward = bind("hum_layer_norm_backward", b, vp, i64, vp, vp, vp, i64, vp, vp, vp, u64, vp)
         self.raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        self.written = torch.autograd.graph.increment_version   # for tensors of the caller's that a kernel wrote into
 
     def stream(self, index):
         if self.raw_stream is not None:
@@ -296,8 +297,8 @@ def decay_attention_step(q, k, v, log_decay, state, reset=None, active=None, sca
         _on(state_out, dev, "state_out", state.shape, (t.float32,))
         if not state_out.is_contiguous():
             raise ValueError("state_out must be contiguous")
-    shape = (n, sizes[2], sizes[5])
-    if out is None:
+    shape, made = (n, sizes[2], sizes[5]), out is None
+    if made:
         out = t.empty_like(v) if v.shape == shape and v.is_contiguous() else t.empty(shape, dtype=q.dtype, device=dev)
     elif _unit(_on(out, dev, "out", shape, (q.dtype,))) is not out:
         raise ValueError("out must have adjacent channels")
@@ -308,6 +309,9 @@ def decay_attention_step(q, k, v, log_decay, state, reset=None, active=None, sca
                    reset.stride(0) if reset is not None else 0, 0, 0)
     N.check(e.step(a, active.data_ptr() if active is not None else None, _ROWS.pack(out.data_ptr(), so[0], 0, so[1]),
                    e.stream(index)), "hum_decay_attn_step")
+    e.written(state_out)   # (a gradient that has saved them raises)
+    if not made:
+        e.written(out)
     return out
 
 
@@ -344,7 +348,8 @@ def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, out=None, stats=True
     t, dev = e.t, x.device
     p = weight if weight is not None else bias
     x2, weight, bias, a = _norm_args(e, x, weight, bias, p.dtype if p is not None else t.float32)
-    if out is None:
+    made = out is None
+    if made:
         out = t.empty_like(x) if x2 is x and x.is_contiguous() else t.empty(x.shape, dtype=x.dtype, device=dev)
     else:
         _on(out, dev, "out", x.shape, (x.dtype,))
@@ -354,6 +359,8 @@ def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, out=None, stats=True
     mean = t.empty(rows, dtype=t.float32, device=dev) if stats else None
     rstd = t.empty(rows, dtype=t.float32, device=dev) if stats else None
     N.check(e.norm(a, _p(bias), eps, out.data_ptr(), c, _p(mean), _p(rstd), e.stream(x.get_device())), "hum_layer_norm")
+    if not made:
+        e.written(out)
     return out, mean, rstd
 
 
