@@ -74,6 +74,7 @@ class HierVecEnv(HumanoidVecEnv):
                                       _ptr(self.obs), _ptr(self.reward_high), _ptr(self.reward), _ptr(self.done),
                                       _ptr(self.frame), flags, _ptr(self.obs_high_reset), self._stream()),
                 "hum_hier_step")
+        self._advanced()
         return self.agents, self.obs_high, self.obs, self.reward_high, self.reward, self.done, self.frame
 
     def step_k(self, high_actions, low_actions, agent=None, autoreset=False, skip_physics=False, out=None):
@@ -95,6 +96,7 @@ class HierVecEnv(HumanoidVecEnv):
         N.check(N.lib().hum_hier_step_k(self.h, _ptr(ah), _ptr(al), _ptr(ag), _ptr(agents), _ptr(oh), _ptr(ol),
                                         _ptr(rh), _ptr(rl), _ptr(done), _ptr(frame), flags, _ptr(ohr), k,
                                         self._stream()), "hum_hier_step_k")
+        self._advanced()
         return out
 
     def step_k_out(self, k):

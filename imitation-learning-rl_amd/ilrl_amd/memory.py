@@ -457,7 +457,8 @@ class PolicyMemory:
 
     def step(self, obs, state, reset=None, active=None):
         """Features [n, n_in] for the lanes' observations obs [n, n_in]; `state` moves on in place.  reset [n]: this step
-        starts an episode (the previous step's done flags); active [n]: lanes that step."""
+        starts an episode (HumanoidVecEnv.episode_start(); behind a step with auto-reset its done flags); active [n]:
+        lanes that step."""
         with _e().t.no_grad():
             q, k, v = self._project(obs)
             return self._join(obs, decay_attention_step(q, k, v, self.log_decay, state, reset=reset, active=active))

@@ -222,9 +222,10 @@ class DevicePolicy:
         sample_batch_columns(..., mean=...).
         memory: a PolicyMemory (ilrl_amd/memory.py) between the observations and the network; per step it advances the
         lanes' memory `state` (memory.begin(n), moved on in place from call to call) and the network reads its features.
-        An episode that ended at the previous step is forgotten.  The trajectory then also holds resets [k,n] (the rows
-        at which an episode started), what sample_batch_columns(..., memory=) and memory.forward need with a copy of
-        `state` from before the call.  Not with fused."""
+        An episode that ended at the previous step, or that venv.reset() has left since, is forgotten.  The trajectory
+        then also holds resets [k,n] (the rows at which another episode starts, venv.episode_start()), what
+        sample_batch_columns(..., memory=) and memory.forward need with a copy of `state` from before the call.  Not
+        with fused."""
         t = self.torch
         n = venv.n
         if memory is not None:
@@ -258,6 +259,7 @@ class DevicePolicy:
         else:
             fn = N.lib().hum_rollout_fused if fused else N.lib().hum_rollout
             N.check(fn(*args, venv._stream()), "hum_rollout_fused" if fused else "hum_rollout")
+        venv._advanced()
         return tr
 
 
@@ -285,10 +287,11 @@ class DevicePolicy:
         for i in range(k):
             # lanes that finished an episode in the previous step act on their reset observation, with nothing remembered
             obs = t.where(venv.done.bool()[:, None], venv.obs_reset, venv.obs)
-            feat = memory.step(obs, state, reset=venv.done)
+            starts = venv.done if i else venv.episode_start()   # (a reset() before the call has cleared its lanes' done)
+            feat = memory.step(obs, state, reset=starts)
             if tr:
                 tr["obs"][i].copy_(obs)
-                tr["resets"][i].copy_(venv.done)
+                tr["resets"][i].copy_(starts)
             self.act(feat, explore=explore, step=step0 + i, out=act, raw_out=tr["actions"][i] if tr else None)
             venv.step(act, autoreset=True)
             if tr:
@@ -360,6 +363,7 @@ def hier_rollout(venv, high, low, k, explore=True, step0=0, trajectories=True, f
     else:
         fn = "hum_hier_rollout_fused" if fused else "hum_hier_rollout"
         N.check(getattr(N.lib(), fn)(*args, venv._stream()), fn)
+    venv._advanced()
     return tr
 
 

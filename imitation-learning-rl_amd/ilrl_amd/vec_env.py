@@ -96,6 +96,8 @@ class HumanoidVecEnv:
         self.obs_reset = torch.zeros(self.n, N.HUM_NOBS, dtype=f32, device=self.device)
         self.reward = torch.zeros(self.n, dtype=f32, device=self.device)
         self.done = torch.zeros(self.n, dtype=torch.uint8, device=self.device)
+        self.begun = torch.zeros(self.n, dtype=torch.uint8, device=self.device)   # lanes that reset() cut off (episode_start)
+        self._stepped = self._begun = self._begun_captured = False
         self.frame = torch.zeros(self.n, dtype=torch.int32, device=self.device)
         self.aux = torch.zeros(self.n, N.HUM_NAUX, dtype=f32, device=self.device)
 
@@ -168,6 +170,27 @@ class HumanoidVecEnv:
             self.done.zero_()
         else:
             self.done.masked_fill_(m.bool(), 0)
+        if self._stepped:   # (before the first step there is no episode to leave)
+            self._begun = True
+            self._begun_captured = self._begun_captured or self.torch.cuda.is_current_stream_capturing()
+            if m is None:
+                self.begun.fill_(1)
+            else:
+                self.begun.masked_fill_(m.bool(), 1)
+
+    def _advanced(self):
+        """Every call that has stepped the lanes comes here: the marks reset() left are over.  No launch where there are
+        none; a captured step clears them on every replay, since a replay cannot ask."""
+        self._stepped = True
+        capturing = self.torch.cuda.is_current_stream_capturing()
+        if self._begun or capturing:
+            self.begun.zero_()
+            self._begun = self._begun and (capturing or self._begun_captured)
+
+    def episode_start(self):
+        """uint8 [n]: lanes whose current observation starts another episode than their last step's - it ended there
+        (done), or reset() has left it since.  What a policy's memory must not carry over (PolicyMemory.step's `reset`)."""
+        return (self.done != 0).logical_or(self.begun).to(self.torch.uint8)
 
     def step(self, actions, autoreset=False, skip_physics=False):
         """One env step for all lanes. actions: float32 [n,17] (device tensor or array)."""
@@ -178,6 +201,7 @@ class HumanoidVecEnv:
         flags = (N.HUM_STEP_AUTORESET if autoreset else 0) | (N.HUM_STEP_SKIP_PHYSICS if skip_physics else 0)
         N.check(N.lib().hum_step(self.h, _ptr(a), _ptr(self.obs), _ptr(self.reward), _ptr(self.done),
                                  _ptr(self.frame), flags, _ptr(self.obs_reset), self._stream()), "hum_step")
+        self._advanced()
         return self.obs, self.reward, self.done, self.frame
 
     def step_k(self, actions, autoreset=False, skip_physics=False, out=None):
@@ -195,6 +219,7 @@ class HumanoidVecEnv:
         flags = (N.HUM_STEP_AUTORESET if autoreset else 0) | (N.HUM_STEP_SKIP_PHYSICS if skip_physics else 0)
         N.check(N.lib().hum_step_k(self.h, _ptr(a), _ptr(obs), _ptr(rew), _ptr(done), _ptr(frame), flags,
                                    _ptr(obs_reset), k, self._stream()), "hum_step_k")
+        self._advanced()
         return out
 
     def step_k_out(self, k):

@@ -75,3 +75,81 @@ def test_a_step_elsewhere_leaves_the_gradient():
         assert s.any()
         y = torch.zeros(3, 8, device="cuda")
         M.layer_norm_forward(y, out=y)
+
+
+@pytest.mark.parametrize("between", ["masked", "all", "masked, stepped", "twice"])
+def test_reset_between_rollouts_starts_an_episode(between):
+    """Lanes that venv.reset() takes to a new episode forget the old one, and the trajectory says so to the learner."""
+    n = 12
+    pol, mem, env = DevicePolicy.random_init(seed=1), M.PolicyMemory(heads=2, channels=16, seed=3), HumanoidVecEnv(n, seed=2)
+    with torch.no_grad():
+        mem.w_out += 0.1 * rows(32, 70, seed=8)
+    mask = torch.arange(n).remainder(3).eq(0).to(torch.uint8).cuda()
+    env.reset()
+    assert not env.episode_start().any()   # no episode came before
+    state = mem.begin(n)
+    first = pol.rollout(env, 3, memory=mem, state=state)
+    assert not first["resets"][0].any() and state.flatten(1).any(1).all()
+    starts = env.done.bool()
+    env.reset(None if between == "all" else mask)
+    starts = torch.ones_like(starts) if between == "all" else starts | mask.bool()
+    if between == "twice":
+        env.reset(1 - mask)
+        starts.fill_(True)
+    assert torch.equal(env.episode_start().bool(), starts)
+    if between == "masked, stepped":   # the marked step is not the rollout's
+        env.step(torch.zeros(n, 17), autoreset=True)
+        starts = env.done.bool()
+    before, want = state.clone(), state.clone()
+    obs = torch.where(env.done.bool()[:, None], env.obs_reset, env.obs)
+    tr = pol.rollout(env, 2, memory=mem, state=state)
+    assert torch.equal(tr["resets"][0].bool(), starts) and torch.equal(tr["resets"][1], tr["dones"][0])
+    assert torch.equal(tr["obs"][0], obs)
+    mem.step(obs, want, reset=starts)
+    mem.step(tr["obs"][1], want, reset=tr["resets"][1])
+    assert torch.equal(state, want)
+    if starts.any():
+        blank = mem.begin(n)
+        mem.step(obs, blank)
+        mem.step(tr["obs"][1], blank, reset=tr["resets"][1])
+        assert torch.equal(state[starts], blank[starts])   # nothing of the old episode is left
+    # the learner's pass over the fragment does not see it either
+    _, last = mem.forward(tr["obs"], state=before, reset=tr["resets"])
+    torch.testing.assert_close(last.detach(), state, rtol=1e-4, atol=1e-5)
+    assert not (env.episode_start().bool() & ~env.done.bool()).any()
+    env.close()
+    pol.close()
+
+
+def test_other_rollouts_end_the_start_of_an_episode():
+    """Every call that steps the lanes ends what reset() marked."""
+    n, pol, env = 8, DevicePolicy.random_init(seed=1), HumanoidVecEnv(8, seed=2)
+    env.reset()
+    env.step(torch.zeros(n, 17))
+    for advance in (lambda: pol.rollout(env, 1), lambda: env.step_k(torch.zeros(2, n, 17), autoreset=True),
+                    lambda: env.step(torch.zeros(n, 17))):
+        env.reset()
+        assert env.episode_start().all()
+        advance()
+        assert not env.begun.any()
+    env.close()
+    pol.close()
+
+
+def test_a_replayed_step_ends_the_start_of_an_episode():
+    """A step captured into a graph clears the marks on every replay, also of resets that came after the capture."""
+    n, env = 8, HumanoidVecEnv(8, seed=2)
+    act = torch.zeros(n, 17, device="cuda")
+    env.reset()
+    env.step(act)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        env.step(act, autoreset=True)
+    for _ in range(3):
+        env.reset()
+        assert env.episode_start().all()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert not env.begun.any()
+    env.close()
