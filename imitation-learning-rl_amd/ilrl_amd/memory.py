@@ -366,12 +366,15 @@ def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, out=None, stats=True
 
 def layer_norm_backward(dy, x, mean, rstd, weight=None, needs=(True, True, True), param_dtype=None):
     """(dx, d_weight, d_bias) for the gradient dy of layer_norm's output, from its input x and the statistics
-    layer_norm_forward returned.  needs: which of the three to compute (the others are None).  Without a weight the
-    parameter gradients are computed only if param_dtype names their type."""
+    layer_norm_forward returned.  needs: which of the three to compute (the others are None).  The parameter gradients are
+    of the weight's type; without a weight they are computed only if param_dtype names their type, float32 or x's."""
     e = _e()
     t, dev = e.t, x.device
     if param_dtype is None:
         param_dtype = weight.dtype if weight is not None else None
+    elif param_dtype not in (t.float32, x.dtype) or (weight is not None and param_dtype != weight.dtype):
+        # (the kernel has one type for the weight and both gradients)
+        raise ValueError("param_dtype must be the weight's type, without one float32 or x's, got %s" % param_dtype)
     x2, weight, _, a = _norm_args(e, x, weight, None, param_dtype if param_dtype is not None else t.float32)
     rows, c = x2.shape
     if not (dy.dtype == x.dtype and dy.shape == x.shape and dy.get_device() == x.get_device()):
