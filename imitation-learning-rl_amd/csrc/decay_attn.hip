@@ -45,6 +45,7 @@
 #include <type_traits>
 
 #include "../../include/humanoid_env.h"
+#include "overlap.h"
 
 void hum_internal_set_error(const char* msg);
 
@@ -1048,11 +1049,19 @@ int check_args(const char* fn, const hum_decay_attn_args* p) {
     return HUM_OK;
 }
 
-// two states share memory
-bool meet(const hum_decay_attn_args* p, const float* a, const float* b) {
-    const uint64_t size = 4ull * p->lanes * p->heads * p->dk * p->dv;
-    return a && b && (uintptr_t)a < (uintptr_t)b + size && (uintptr_t)b < (uintptr_t)a + size;
+// the memory that arguments stand for (overlap.h)
+typedef overlap::Bytes Bytes;
+Bytes bytes_of(const hum_decay_attn_args* p, const hum_rows& r, int heads, int d, int size) {
+    return Bytes(r.ptr, (int64_t)d * size).by(p->lanes, r.lane * size).by(p->steps, r.step * size).by(heads, r.head * size);
 }
+Bytes bytes_of(const hum_decay_attn_args* p, const float* state) {
+    return Bytes(state, 4ll * p->lanes * p->heads * p->dk * p->dv);
+}
+Bytes bytes_of_reset(const hum_decay_attn_args* p) { return Bytes(p->reset, 1).by(p->lanes, p->reset_lane).by(p->steps, p->reset_step); }
+Bytes bytes_of_decay(const hum_decay_attn_args* p) { return Bytes(p->log_decay, 4ll * p->heads); }
+Bytes bytes_of_lengths(const hum_decay_attn_args* p) { return Bytes(p->lengths, 4ll * p->lanes); }
+// a call's state_in, out of the question where state_out is the same
+Bytes bytes_of_entering(const hum_decay_attn_args* p) { return p->state_in == p->state_out ? Bytes() : bytes_of(p, p->state_in); }
 
 int in_32(int d) { return d <= 32 ? 1 : d <= 64 ? 2 : 4; }
 template <int ST, int K, int W, int J, int HEADS, Mode MODE, bool OUTS>
@@ -1247,16 +1256,20 @@ int hum_decay_attn(const hum_decay_attn_args* p, const hum_rows* out, void* work
     if (const int rc = check_args(fn, p)) return rc;
     if (!out || (p->lanes && p->steps && !out->ptr) || ((uintptr_t)out->ptr) % elem_size(p->type))
         return derr(HUM_ERR_ARG, fn, "out is required, aligned to its elements");
-    if (p->state_in != p->state_out && meet(p, p->state_in, p->state_out))
-        return derr(HUM_ERR_ARG, fn, "state_out must be state_in or not overlap it");
     uint64_t need = 0;
     if (const int rc = hum_decay_attn_workspace(p, 0, &need)) return rc;
     if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
         return derr(HUM_ERR_ARG, fn, "the workspace is too small (hum_decay_attn_workspace) or not aligned to 16 bytes");
     if (!p->lanes) return HUM_OK;
+    const int size = elem_size(p->type), group = p->heads / p->kv_heads;
+    const Bytes writes[] = {bytes_of(p, *out, p->heads, p->dv, size), bytes_of(p, p->state_out), Bytes(workspace, need)};
+    const Bytes reads[] = {bytes_of(p, p->q, p->heads, p->dk, size), bytes_of(p, p->k, p->kv_heads, p->dk, size),
+                           bytes_of(p, p->v, p->kv_heads, p->dv, size), bytes_of_entering(p), bytes_of_decay(p), bytes_of_reset(p),
+                           bytes_of_lengths(p)};
+    if (overlap::clash(writes, reads))
+        return derr(HUM_ERR_ARG, fn, "out, state_out and the workspace must overlap neither each other nor an input (state_out may be state_in)");
     const OnDevice dev(p->device);
     if (!dev.ok) return derr(HUM_ERR_HIP, fn, "hipSetDevice");
-    const int size = elem_size(p->type), group = p->heads / p->kv_heads;
     Role r = {};
     r.x = rows_of(p->q, 1, size, p->dk);
     r.y = rows_of(p->k, group, size, p->dk);
@@ -1296,9 +1309,15 @@ int hum_decay_attn_backward(const hum_decay_attn_args* p, const hum_rows* d_out,
     if (const int rc = hum_decay_attn_workspace(p, 1, &need)) return rc;
     if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
         return derr(HUM_ERR_ARG, fn, "the workspace is too small (hum_decay_attn_workspace) or not aligned to 16 bytes");
-    if (meet(p, d_state_in, d_state_out) || meet(p, d_state_in, p->state_in))
-        return derr(HUM_ERR_ARG, fn, "d_state_in must not overlap state_in or d_state_out");
     if (!p->lanes) return HUM_OK;
+    const Bytes writes[] = {bytes_of(p, gq, p->heads, p->dk, size), bytes_of(p, gk, p->kv_heads, p->dk, size),
+                            bytes_of(p, gv, p->kv_heads, p->dv, size), bytes_of(p, d_state_in), Bytes(workspace, need)};
+    const Bytes reads[] = {bytes_of(p, p->q, p->heads, p->dk, size), bytes_of(p, p->k, p->kv_heads, p->dk, size),
+                           bytes_of(p, p->v, p->kv_heads, p->dv, size), bytes_of(p, *d_out, p->heads, p->dv, size),
+                           bytes_of(p, p->state_in), bytes_of(p, d_state_out), bytes_of_decay(p), bytes_of_reset(p),
+                           bytes_of_lengths(p)};
+    if (overlap::clash(writes, reads))
+        return derr(HUM_ERR_ARG, fn, "gradients and the workspace must overlap neither each other nor an input");
     const OnDevice dev(p->device);
     if (!dev.ok) return derr(HUM_ERR_HIP, fn, "hipSetDevice");
     const Rows q = rows_of(p->q, 1, size, p->dk), k = rows_of(p->k, group, size, p->dk);
@@ -1409,12 +1428,17 @@ extern "C" int hum_decay_attn_step(const hum_decay_attn_args* p, const uint8_t* 
     if (p->steps != 1 || p->lengths) return derr(HUM_ERR_ARG, fn, "steps must be 1 and lengths NULL (active says which lanes step)");
     if (!out || (p->lanes && (!out->ptr || !p->state_out)) || ((uintptr_t)out->ptr) % elem_size(p->type))
         return derr(HUM_ERR_ARG, fn, "out (aligned to its elements) and state_out are required");
-    if (p->state_in != p->state_out && meet(p, p->state_in, p->state_out))
-        return derr(HUM_ERR_ARG, fn, "state_out must be state_in or not overlap it");
     if (!p->lanes) return HUM_OK;
+    const int size = elem_size(p->type), group = p->heads / p->kv_heads;
+    // (a head's workgroups and waves read all of q and k, and store their rows of out and of the state at once)
+    const Bytes writes[] = {bytes_of(p, *out, p->heads, p->dv, size), bytes_of(p, p->state_out)};
+    const Bytes reads[] = {bytes_of(p, p->q, p->heads, p->dk, size), bytes_of(p, p->k, p->kv_heads, p->dk, size),
+                           bytes_of(p, p->v, p->kv_heads, p->dv, size), bytes_of_entering(p), bytes_of_decay(p), bytes_of_reset(p),
+                           Bytes(active, p->lanes)};
+    if (overlap::clash(writes, reads))
+        return derr(HUM_ERR_ARG, fn, "out and state_out must overlap neither each other nor an input (state_out may be state_in)");
     const OnDevice dev(p->device);
     if (!dev.ok) return derr(HUM_ERR_HIP, fn, "hipSetDevice");
-    const int size = elem_size(p->type), group = p->heads / p->kv_heads;
     StepArgs a = {};
     a.q = rows_of(p->q, 1, size, p->dk);
     a.k = rows_of(p->k, group, size, p->dk);

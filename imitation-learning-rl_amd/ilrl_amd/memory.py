@@ -279,8 +279,9 @@ def decay_attention_step(q, k, v, log_decay, state, reset=None, active=None, sca
     """One step of every lane: q [lanes, heads, dk], k [lanes, kv_heads, dk], v [lanes, kv_heads, dv], state
     [lanes, heads, dv, dk] float32 -> out [lanes, heads, dv].  The new state goes to state_out, by default into `state`
     itself.  reset [lanes] uint8 or bool: this step starts an episode; active [lanes] uint8 or bool: lanes that step
-    (None = all), the others keep their state and give zeros.  Not differentiable (the learner's pass over the recorded
-    fragment is): inputs that require a gradient are refused while gradients are recorded."""
+    (None = all), the others keep their state and give zeros.  out and state_out may be slices of a buffer that holds the
+    inputs too, but must not overlap them (state_out may be state).  Not differentiable (the learner's pass over the
+    recorded fragment is): inputs that require a gradient are refused while gradients are recorded."""
     e = _e()
     t = e.t
     if t.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (state is not None and state.requires_grad)):

@@ -487,17 +487,19 @@ typedef struct {
 } hum_decay_attn_args;
 /* bytes of scratch that hum_decay_attn (backward = 0) or hum_decay_attn_backward (1) needs for these sizes (0: none) */
 int hum_decay_attn_workspace(const hum_decay_attn_args* args, int32_t backward, uint64_t* bytes);
-/* out [lanes, steps, heads, dv] must not overlap an input. */
+/* out [lanes, steps, heads, dv], state_out and the workspace must overlap neither each other nor an input (state_out may be
+ * state_in).  Slices of one packed buffer that lie between each other's rows do not overlap. */
 int hum_decay_attn(const hum_decay_attn_args* args, const hum_rows* out, void* workspace, uint64_t workspace_bytes,
                    void* stream);
 /* Gradients for d_out [lanes, steps, heads, dv] and d_state_out (gradient of state_out; NULL = zeros), from the forward
  * call's inputs (args->state_out is not used): dq, dk, dv shaped like q, k, v (dk, dv summed over the heads that share
- * one) and d_state_in; each may be NULL.  Outputs must not overlap inputs or each other. */
+ * one) and d_state_in; each may be NULL.  Outputs and the workspace must not overlap inputs or each other. */
 int hum_decay_attn_backward(const hum_decay_attn_args* args, const hum_rows* d_out, const float* d_state_out,
                             const hum_rows* dq, const hum_rows* dk, const hum_rows* dv, float* d_state_in,
                             void* workspace, uint64_t workspace_bytes, void* stream);
 /* One step (args->steps = 1, lengths NULL) of every lane with active[lane] != 0 (NULL = all): the sampler's form.  An
- * idle lane keeps its state and gives zeros.  state_out is required and may be state_in.  The step strides are unused. */
+ * idle lane keeps its state and gives zeros.  state_out is required and may be state_in; out and state_out must overlap
+ * nothing else of the call.  The step strides are unused. */
 int hum_decay_attn_step(const hum_decay_attn_args* args, const uint8_t* active, const hum_rows* out, void* stream);
 
 /* Layer norm over the channels of each row: y = (x - mean) rstd weight + bias, rstd = 1 / sqrt(var + eps), sums in

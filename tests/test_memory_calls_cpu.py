@@ -1,9 +1,14 @@
 """Calls of the policy memory's operators that are refused before anything reaches a GPU."""
+import ctypes
+
 import pytest
 
 torch = pytest.importorskip("torch")
 
+from ilrl_amd import _native as N  # noqa: E402
 from ilrl_amd import memory as M  # noqa: E402
+
+r = ctypes.byref
 
 
 @pytest.mark.parametrize("x,weight,param", [
@@ -18,3 +23,79 @@ def test_norm_gradient_refuses_a_parameter_type_that_is_not_the_weights(x, weigh
     w = torch.zeros(8, dtype=weight) if weight is not None else None
     with pytest.raises(ValueError, match="param_dtype"):
         M.layer_norm_backward(a, a, torch.zeros(3), torch.ones(3), w, param_dtype=param)
+
+
+# ---------------------------------------------------------------------------------------------- outputs over inputs
+# (addresses that nothing is at: every call here is refused)
+LANES, STEPS, HEADS, D = 2, 3, 4, 8
+Q, K, V, OUT, STATE, NEXT, RESET, DECAY, GRAD, SPACE = (0x1000000 * i for i in range(1, 11))
+
+
+def rows(at, step=HEADS * D, head=D, lane=None):
+    return N.HumRows(at, STEPS * step if lane is None else lane, step, head)
+
+
+def attn(**kw):
+    d = dict(device=0, type=N.HUM_F32, lanes=LANES, steps=STEPS, heads=HEADS, kv_heads=HEADS, dk=D, dv=D, scale=1.0,
+             log_decay=DECAY, q=rows(Q), k=rows(K), v=rows(V), state_in=STATE, state_out=NEXT, reset=RESET, reset_lane=STEPS,
+             reset_step=1)
+    d.update(kw)
+    return N.HumDecayAttnArgs(**d)
+
+
+def refused(rc):
+    assert rc == N.HUM_ERR_ARG and b"overlap" in N.lib().hum_last_error(), (rc, N.lib().hum_last_error())
+
+
+SIZE, ALL = 4 * STEPS * HEADS * D * LANES, 4 * LANES * HEADS * D * D
+
+
+@pytest.mark.parametrize("at", [Q, K, V, Q + SIZE - 4, V - SIZE + 4, STATE + ALL - 4, NEXT, DECAY, RESET + 4])
+def test_out_that_overlaps_is_refused(at):
+    """Waves that store out beside others that still read: the whole of q and k by every wave of a head."""
+    L = N.lib()
+    refused(L.hum_decay_attn(r(attn()), r(rows(at)), None, 0, None))
+    one = dict(steps=1, q=rows(Q, lane=HEADS * D), k=rows(K, lane=HEADS * D), v=rows(V, lane=HEADS * D), reset_lane=STEPS)
+    small = SIZE // STEPS
+    at = {Q + SIZE - 4: Q + small - 4, V - SIZE + 4: V - small + 4, RESET + 4: RESET}.get(at, at)
+    refused(L.hum_decay_attn_step(r(attn(**one)), None, r(rows(at, lane=HEADS * D)), None))
+    refused(L.hum_decay_attn_step(r(attn(**one)), GRAD, r(rows(GRAD, lane=HEADS * D)), None))   # active
+
+
+@pytest.mark.parametrize("at", [Q, K, V, DECAY, STATE + 4, STATE - ALL + 4])
+def test_state_out_that_overlaps_is_refused(at):
+    L = N.lib()
+    refused(L.hum_decay_attn(r(attn(state_out=at)), r(rows(OUT)), None, 0, None))
+    refused(L.hum_decay_attn_step(r(attn(steps=1, state_out=at)), None, r(rows(OUT)), None))
+
+
+def test_rows_of_out_that_lie_on_each_other_are_refused():
+    L = N.lib()
+    for bad in (rows(OUT, head=0), rows(OUT, head=D - 1), rows(OUT, lane=0), rows(OUT, step=(HEADS - 1) * D)):
+        refused(L.hum_decay_attn(r(attn()), r(bad), None, 0, None))
+        refused(L.hum_decay_attn_backward(r(attn()), r(rows(GRAD)), None, r(bad), None, None, None, None, 0, None))
+    refused(L.hum_decay_attn_step(r(attn(steps=1)), None, r(rows(OUT, lane=0)), None))
+
+
+@pytest.mark.parametrize("at", [Q, K, V, GRAD, DECAY, STATE, NEXT])
+def test_gradients_that_overlap_are_refused(at):
+    L = N.lib()
+    own = [rows(OUT), rows(OUT + 0x10000), rows(OUT + 0x20000)]
+    for i in range(3):
+        g = [rows(at) if j == i else own[j] for j in range(3)]
+        refused(L.hum_decay_attn_backward(r(attn()), r(rows(GRAD)), NEXT, *map(r, g), None, None, 0, None))
+        g[i] = own[i - 1]
+        refused(L.hum_decay_attn_backward(r(attn()), r(rows(GRAD)), NEXT, *map(r, g), None, None, 0, None))
+    refused(L.hum_decay_attn_backward(r(attn()), r(rows(GRAD)), NEXT, *map(r, own), at, None, 0, None))
+
+
+def test_workspaces_that_overlap_are_refused():
+    L, need = N.lib(), ctypes.c_uint64(0)
+    shared = attn(kv_heads=2)
+    assert L.hum_decay_attn_workspace(r(shared), 1, r(need)) == 0 and need.value
+    for at in (Q, K + 16, V, GRAD, OUT, STATE, NEXT):
+        refused(L.hum_decay_attn_backward(r(shared), r(rows(GRAD)), NEXT, r(rows(OUT)), None, None, None, at, need.value, None))
+    long = dict(steps=1000, lanes=1)
+    assert L.hum_decay_attn_workspace(r(attn(**long)), 0, r(need)) == 0 and need.value
+    for at in (Q, V, STATE, NEXT, OUT):
+        refused(L.hum_decay_attn(r(attn(**long)), r(rows(OUT)), at, need.value, None))
