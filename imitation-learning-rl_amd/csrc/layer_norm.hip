@@ -20,6 +20,7 @@
 #include <cstdio>
 
 #include "../../include/humanoid_env.h"
+#include "overlap.h"
 
 void hum_internal_set_error(const char* msg);
 
@@ -430,12 +431,16 @@ int check_sizes(const char* fn, const hum_norm_args* p) {
 bool near(int64_t row, int size) { return row >= 0 && row < (1l << 28) / size; }
 bool aligned(const void* p, int64_t row, int size) { return ((uintptr_t)p | (uintptr_t)(row * size)) % 16 == 0; }
 
-// rows that are written must lie apart, and over the rows they replace if they begin with them
-bool apart(const hum_norm_args* p, const void* out, int64_t row) {
-    return p->rows < 2 || !out || row >= p->channels || row <= -(int64_t)p->channels;
+// the memory that arguments stand for (overlap.h)
+typedef overlap::Bytes Bytes;
+Bytes rows_of(const hum_norm_args* p, const void* at, int64_t row, int size) {
+    return Bytes(at, (int64_t)p->channels * size).by(p->rows, row * size);
 }
-bool replaces(const hum_norm_args* p, const void* out, int64_t row, const void* in, int64_t in_row) {
-    return p->rows < 2 || !out || out != in || row == in_row;
+Bytes stats_of(const hum_norm_args* p, const float* at) { return Bytes(at, 4 * p->rows); }
+Bytes params_of(const hum_norm_args* p, const void* at, int size) { return Bytes(at, (int64_t)p->channels * size); }
+// rows that are read, out of the question where `out` replaces them row for row (a row is in registers before it is written)
+Bytes rows_read(const hum_norm_args* p, const void* at, int64_t row, int size, const void* out, int64_t out_row) {
+    return at == out && (row == out_row || p->rows < 2) ? Bytes() : rows_of(p, at, row, size);
 }
 
 int launched(const char* fn) {
@@ -453,12 +458,14 @@ int hum_layer_norm(const hum_norm_args* p, const void* bias, float eps, void* y,
     if (const int rc = check_sizes(fn, p)) return rc;
     const int es = p->type == HUM_F32 ? 4 : 2, ps = p->param_type == HUM_F32 ? 4 : 2;
     if ((p->rows && !y) || (uintptr_t)y % es || (uintptr_t)bias % ps) return nerr(HUM_ERR_ARG, fn, "y is required; rows and parameters must be aligned to their elements");
-    if (!apart(p, y, y_row) || !replaces(p, y, y_row, p->x, p->x_row))
-        return nerr(HUM_ERR_ARG, fn, "rows of y must not overlap, and have x's stride if y is x");
     if (!mean != !rstd) return nerr(HUM_ERR_ARG, fn, "mean and rstd are wanted together");
     if (((uintptr_t)mean | (uintptr_t)rstd) % 4) return nerr(HUM_ERR_ARG, fn, "mean and rstd must be aligned to 4 bytes");
     if (!(eps >= 0.f) || !std::isfinite(eps)) return nerr(HUM_ERR_ARG, fn, "eps must be finite and >= 0");
     if (!p->rows) return HUM_OK;
+    const Bytes writes[] = {rows_of(p, y, y_row, es), stats_of(p, mean), stats_of(p, rstd)};
+    const Bytes reads[] = {rows_read(p, p->x, p->x_row, es, y, y_row), params_of(p, p->weight, ps), params_of(p, bias, ps)};
+    if (overlap::clash(writes, reads))
+        return nerr(HUM_ERR_ARG, fn, "y and the statistics must overlap neither themselves, each other nor an input (y may be x, row for row)");
     const OnDevice dev(p->device);
     if (!dev.ok) return nerr(HUM_ERR_HIP, fn, "hipSetDevice");
     NormArgs a = {p->x, p->weight, bias, y, mean, rstd, (long)p->rows, (long)p->x_row, (long)y_row, p->channels, p->param_type == HUM_F32, eps};
@@ -488,8 +495,6 @@ int hum_layer_norm_backward(const hum_norm_args* p, const void* dy, int64_t dy_r
     if (p->rows && (!dy || !mean || !rstd)) return nerr(HUM_ERR_ARG, fn, "dy, mean and rstd are required");
     if (((uintptr_t)dy | (uintptr_t)dx) % es || ((uintptr_t)d_weight | (uintptr_t)d_bias) % ps || ((uintptr_t)mean | (uintptr_t)rstd) % 4)
         return nerr(HUM_ERR_ARG, fn, "rows, statistics and parameters must be aligned to their elements");
-    if (!apart(p, dx, dx_row) || !replaces(p, dx, dx_row, p->x, p->x_row) || !replaces(p, dx, dx_row, dy, dy_row))
-        return nerr(HUM_ERR_ARG, fn, "rows of dx must not overlap, and have x's or dy's stride if dx is one of them");
     const Shape sh = shape_of(p->channels, near(p->x_row, es) && near(dy_row, es) && near(dx_row, es));
     const bool params = d_weight || d_bias;
     uint64_t need = 0;
@@ -498,6 +503,13 @@ int hum_layer_norm_backward(const hum_norm_args* p, const void* dy, int64_t dy_r
     if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
         return nerr(HUM_ERR_ARG, fn, "the workspace is too small (hum_layer_norm_workspace) or not aligned to 16 bytes");
     if (!params && (!p->rows || !dx)) return HUM_OK;
+    const Bytes writes[] = {rows_of(p, dx, dx_row, es), Bytes(params ? workspace : nullptr, need)};
+    const Bytes reads[] = {rows_read(p, p->x, p->x_row, es, dx, dx_row), rows_read(p, dy, dy_row, es, dx, dx_row),
+                           params_of(p, p->weight, ps), stats_of(p, mean), stats_of(p, rstd)};
+    // (the second launch writes these: the inputs have been read, the workspace has not)
+    const Bytes sums[] = {params_of(p, d_weight, ps), params_of(p, d_bias, ps)};
+    if (overlap::clash(writes, reads) || overlap::clash(sums, writes))
+        return nerr(HUM_ERR_ARG, fn, "gradients and the workspace must overlap neither themselves, each other nor an input (dx may be x or dy, row for row)");
     const OnDevice dev(p->device);
     if (!dev.ok) return nerr(HUM_ERR_HIP, fn, "hipSetDevice");
     GradArgs a = {dy, p->x, p->weight, dx, mean, rstd, params ? (float*)workspace : nullptr, (long)p->rows, (long)dy_row, (long)p->x_row, (long)dx_row, p->channels, p->param_type == HUM_F32};

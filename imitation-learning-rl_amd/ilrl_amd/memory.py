@@ -344,7 +344,7 @@ def _norm_args(e, x, weight, bias, param_dtype):
 
 def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, out=None, stats=True):
     """(y, mean, rstd): layer_norm without autograd and what its backward pass needs (mean, rstd [rows] float32, None
-    without stats)."""
+    without stats).  out: a contiguous tensor for y, x itself or one that does not overlap an input."""
     e = _e()
     t, dev = e.t, x.device
     p = weight if weight is not None else bias

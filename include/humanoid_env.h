@@ -505,7 +505,7 @@ int hum_decay_attn_step(const hum_decay_attn_args* args, const uint8_t* active, 
 /* Layer norm over the channels of each row: y = (x - mean) rstd weight + bias, rstd = 1 / sqrt(var + eps), sums in
  * float32.  x [rows, channels] of element type `type`, x_row elements from one row to the next, channels adjacent (the
  * same holds for y, dy and dx with their own); weight, bias [channels] of param_type (HUM_F32 or `type`); NULL weight =
- * ones, NULL bias = zeros.  y may be x, row for row. */
+ * ones, NULL bias = zeros.  y may be x, row for row; else outputs must overlap neither each other nor an input. */
 typedef struct {
     int32_t device, type, param_type, channels;   /* channels in [1, 16384] */
     int64_t rows, x_row;
@@ -517,8 +517,9 @@ int hum_layer_norm(const hum_norm_args* args, const void* bias, float eps, void*
                    float* rstd, void* stream);
 /* bytes of scratch hum_layer_norm_backward needs when d_weight or d_bias is wanted */
 int hum_layer_norm_workspace(const hum_norm_args* args, uint64_t* bytes);
-/* dx [rows, channels], d_weight and d_bias [channels] of param_type, each may be NULL; dx may be dy or x, row for row.  The
- * parameter gradients are summed in a fixed order: the same inputs give the same bits. */
+/* dx [rows, channels], d_weight and d_bias [channels] of param_type, each may be NULL; dx may be dy or x, row for row, else
+ * dx and the workspace must overlap neither each other, a gradient nor an input.  The parameter gradients are summed in a
+ * fixed order: the same inputs give the same bits. */
 int hum_layer_norm_backward(const hum_norm_args* args, const void* dy, int64_t dy_row, const float* mean,
                             const float* rstd, void* dx, int64_t dx_row, void* d_weight, void* d_bias, void* workspace,
                             uint64_t workspace_bytes, void* stream);

@@ -69,3 +69,22 @@ def shifted(state):
     flat = torch.cat([state.flatten(), state.new_zeros(1)])
     state.set_(flat.untyped_storage(), 0, state.shape, state.stride())
     return flat[1:].view(state.shape)
+
+
+def test_norm_into_its_input_or_beside_it():
+    """Row for row over the input, or apart from it: another place inside the input's rows is refused."""
+    rows, c = 300, 64
+    flat = torch.randn(rows * c + 2 * c, generator=torch.Generator().manual_seed(1)).cuda()
+    x = flat[:rows * c].view(rows, c)
+    want = M.layer_norm(x)
+    for shift in (1, 4, c, 2 * c):
+        with pytest.raises(N.NativeError, match="overlap"):
+            M.layer_norm_forward(x, out=flat[shift:shift + rows * c].view(rows, c))
+    with pytest.raises(N.NativeError, match="overlap"):
+        M.layer_norm_forward(x, x[7], out=x)   # a weight among the rows it replaces
+    assert torch.equal(M.layer_norm(x), want)
+    half = flat[:rows * c].view(2, rows // 2, c)
+    y, _, _ = M.layer_norm_forward(half[0], out=half[1])   # the buffer's other half
+    assert torch.equal(y, want[:rows // 2])
+    M.layer_norm_forward(half[0], out=half[0])
+    assert torch.equal(half[0], half[1])

@@ -99,3 +99,36 @@ def test_workspaces_that_overlap_are_refused():
     assert L.hum_decay_attn_workspace(r(attn(**long)), 0, r(need)) == 0 and need.value
     for at in (Q, V, STATE, NEXT, OUT):
         refused(L.hum_decay_attn(r(attn(**long)), r(rows(OUT)), at, need.value, None))
+
+
+C, ROWS = 64, 5
+
+
+def norm(**kw):
+    d = dict(device=0, type=N.HUM_F32, param_type=N.HUM_F32, channels=C, rows=ROWS, x_row=80, x=Q, weight=K)
+    d.update(kw)
+    return N.HumNormArgs(**d)
+
+
+# (rows of x are 64 of 80 elements wide: 4 x 16 elements lie between one row and the next)
+@pytest.mark.parametrize("at,row", [(Q + 4, 80), (Q - 4, 80), (Q + 320, 80), (Q + 3 * 320, 80), (Q + 4 * 65, 96), (Q, 96), (Q, 64),
+                                    (Q + 4 * 320 + 252, 64), (K, 80), (K + 252, 80), (V, 80)])
+def test_norm_rows_that_overlap_are_refused(at, row):
+    """Rows at another place inside x's: a workgroup would store over rows that others have yet to read."""
+    L = N.lib()
+    refused(L.hum_layer_norm(r(norm()), V, 1e-5, at, row, None, None, None))
+    refused(L.hum_layer_norm_backward(r(norm()), V, 64, DECAY, GRAD, at, row if at != V else 80, None, None, None, 0, None))
+    refused(L.hum_layer_norm_backward(r(norm(x=V, x_row=64)), Q, 80, DECAY, GRAD, at, row if at != V else 80, None, None, None, 0, None))
+
+
+def test_norm_statistics_and_sums_that_overlap_are_refused():
+    L, need = N.lib(), ctypes.c_uint64(0)
+    for mean, rstd in ((Q, STATE), (STATE, K), (V + 4, STATE), (STATE, STATE + 16), (OUT, STATE), (STATE, OUT + 4 * 320)):
+        refused(L.hum_layer_norm(r(norm()), V, 1e-5, OUT, 80, mean, rstd, None))
+    assert L.hum_layer_norm_workspace(r(norm()), r(need)) == 0 and need.value
+    back = lambda dw, db, space, dx=OUT: L.hum_layer_norm_backward(r(norm()), V, 64, DECAY, GRAD, dx, 80, dw, db, space, need.value, None)
+    for dw, db, space in ((STATE, STATE + 252, SPACE), (OUT, STATE, SPACE), (STATE, SPACE + 64, SPACE), (STATE, NEXT, OUT), (STATE, NEXT, Q),
+                          (STATE, NEXT, V + 16), (STATE, NEXT, K), (STATE, NEXT, DECAY), (STATE, NEXT, GRAD)):
+        refused(back(dw, db, space))
+    for dx in (DECAY, GRAD + 16, K):
+        refused(back(STATE, NEXT, SPACE, dx))
