@@ -54,6 +54,7 @@ class _Entry:
         self.norm_workspace = bind("hum_layer_norm_workspace", b, need)
         self.norm_backward = bind("hum_layer_norm_backward", b, vp, i64, vp, vp, vp, i64, vp, vp, vp, u64, vp)
         self.raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        self.forward_ad = torch.autograd.forward_ad
         self.written = torch.autograd.graph.increment_version   # for tensors of the caller's that a kernel wrote into
 
     def stream(self, index):
@@ -67,6 +68,14 @@ def _e():
     if _entry is None:
         _entry = _Entry()
     return _entry
+
+
+def _no_tangents(e, *xs):
+    """Forward-mode derivatives are refused: past the autograd functions they would be dropped without a word."""
+    if getattr(e.forward_ad, "_current_level", 0) < 0:   # outside dual_level no tensor has one
+        return
+    if any(x is not None and e.forward_ad.unpack_dual(x).tangent is not None for x in xs):
+        raise NotImplementedError("the policy memory's operators have no forward-mode derivative")
 
 
 def _type(e, x, what):
@@ -265,8 +274,10 @@ def decay_attention(q, k, v, log_decay, state=None, reset=None, lengths=None, sc
     the first step (None = zeros), contiguous float32.  reset [lanes, steps] uint8 or bool: nonzero where an episode starts,
     whatever came before is not seen from there on, also where it is not finite.  lengths [lanes] int32: steps behind a
     lane's length are not read and give zeros; the final state is the one after the last step held.  scale: default
-    dk ** -0.5.  Differentiable in q, k, v and state."""
-    t = _e().t
+    dk ** -0.5.  Differentiable in q, k, v and state, once and backwards."""
+    e = _e()
+    t = e.t
+    _no_tangents(e, q, k, v, log_decay, state)
     if t.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
                                 or (state is not None and state.requires_grad)):
         if log_decay.requires_grad:
@@ -286,6 +297,7 @@ def decay_attention_step(q, k, v, log_decay, state, reset=None, active=None, sca
     t = e.t
     if t.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (state is not None and state.requires_grad)):
         raise ValueError("decay_attention_step is not differentiable: use decay_attention, or torch.no_grad()")
+    _no_tangents(e, q, k, v, log_decay, state)
     if state is None:
         raise ValueError("state is required (PolicyMemory.begin, or zeros)")
     q, k, v, log_decay, _, sizes = _check(e, q, k, v, log_decay, state, reset, None, 3)
@@ -403,9 +415,11 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, needs=(True, True, True)
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """Layer norm over the last dimension of x (any leading shape, 1 to 16384 channels): (x - mean) / sqrt(var + eps) *
     weight + bias, sums in float32.  weight, bias: float32 or x's type, None = ones / zeros.  Differentiable in x, weight
-    and bias; the parameter gradients have the same bits every time."""
-    if _e().t.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
-                                     or (bias is not None and bias.requires_grad)):
+    and bias, once and backwards; the parameter gradients have the same bits every time."""
+    e = _e()
+    _no_tangents(e, x, weight, bias)
+    if e.t.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
+                                  or (bias is not None and bias.requires_grad)):
         return _autograd()[1].apply(x, weight, bias, eps)
     return layer_norm_forward(x, weight, bias, eps, stats=False)[0]
 

@@ -132,3 +132,26 @@ def test_norm_statistics_and_sums_that_overlap_are_refused():
         refused(back(dw, db, space))
     for dx in (DECAY, GRAD + 16, K):
         refused(back(STATE, NEXT, SPACE, dx))
+
+
+# ---------------------------------------------------------------------------------------------- forward-mode derivatives
+@pytest.mark.parametrize("grad", [False, True])
+def test_tangents_are_refused_not_dropped(grad):
+    """No operator has a forward-mode derivative: a dual tensor raises, also where gradients are not recorded."""
+    import torch.autograd.forward_ad as fwd
+    x, ld = torch.randn(2, 3, 4, 8), torch.zeros(4)
+    s, w = torch.randn(2, 4, 8, 8), torch.ones(8)
+    with fwd.dual_level(), torch.set_grad_enabled(grad):
+        dual = lambda a: fwd.make_dual(a, torch.ones_like(a))
+        for ops in ((dual(x), x, x, None), (x, dual(x), x, None), (x, x, dual(x), None), (x, x, x, dual(s))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                M.decay_attention(*ops[:3], ld, state=ops[3])
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                M.decay_attention_step(*(a[:, 0] for a in ops[:3]), ld, s if ops[3] is None else ops[3])
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            M.decay_attention(x, x, x, dual(ld))
+        for ops in ((dual(x), w, w), (x, dual(w), w), (x, w, dual(w))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                M.layer_norm(*ops)
+        with pytest.raises(ValueError, match="no CPU path"):
+            M.layer_norm(x, w, w)   # (no tangent: refused for its device)
