@@ -35,8 +35,9 @@
 // bits).  An output is rounded once.
 //
 // Non-finite values.  A row of Z multiplies zeros of P for the steps that must not see it (earlier steps, other
-// episodes), and 0 x inf is NaN: such values of z enter the products as zeros and make NaN of the channels of exactly the
-// steps that see them, so an episode that diverged leaves the next one, and its own earlier steps, untouched.
+// episodes, those past which lambda^d is 0), and 0 x inf is NaN: such values of z enter the products as zeros and make NaN of
+// the channels of exactly the steps that see them, so an episode that diverged leaves the next one, its own earlier steps
+// and what a head without memory does later untouched.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -411,6 +412,13 @@ __global__ void __launch_bounds__(64 * W * HEADS, walk_waves(ST, K, W, MODE)) wa
         pow_pair[l] = l < CH - 1 ? 0.f : R.s_pair * power(l - (CH - 1));
         pow_add[l] = l < CH - 1 ? 0.f : R.s_add * power(l - (CH - 1));
     }
+    // a step is seen for `reach` steps, itself among them; then its weight lambda^d is 0 in float32 (33: as far as a chunk and
+    // the state behind it ask).  A weight of 0 is a mask, also for what is not finite: see `leaving`.  fades: of any head of
+    // the workgroup's, since barriers hang on it
+    const int reach = __popcll(__ballot(l <= CH && power(l) != 0.f));
+    bool fades = HEADS == 1 && reach <= CH;
+    if constexpr (HEADS > 1)
+        for (int i = 0; i < HEADS; i++) fades |= __builtin_amdgcn_exp2f(a.log_decay[h0 + i] * 1.44269504088896340736f * (float)CH) == 0.f;
     const int seg0 = seg * a.seg_steps, seg1 = seg + 1 < a.segs ? seg0 + a.seg_steps : steps;
     const int end = len < seg1 ? len : seg1;
     auto row_of = [&](int tile) { return 8 * (r >> 2) + 4 * tile + (r & 3); };
@@ -587,7 +595,8 @@ __global__ void __launch_bounds__(64 * W * HEADS, walk_waves(ST, K, W, MODE)) wa
         // if there is none
         auto cuts_to = [&](int n) { return cut & ((2ull << n) - 1); };
         auto last_cut = [&](unsigned long long m) { return m ? 63 - __builtin_clzll(m) : 0; };
-        const int leaving = last_cut(cut);   // what leaves the chunk is of the steps from here on
+        const int kept = last_cut(cut), faded = L + rev - reach;
+        const int leaving = kept > faded ? kept : faded;   // what leaves the chunk is of the steps from here on
 
         lds_barrier<B>();   // the chunk before has been read
         if constexpr (OUTS) lay(tx[in_row / PER], PITCH, PLANE, ROWS, row, in_row * UNIT, dy, L, in_row % PER * UNIT, rx);
@@ -649,7 +658,7 @@ __global__ void __launch_bounds__(64 * W * HEADS, walk_waves(ST, K, W, MODE)) wa
             }
             lds_barrier<B>();
         }
-        if (leaving > 0) {   // z's weights will be zeros for these steps, which a y row that is not finite would not heed
+        if (kept > 0 || fades) {   // z's weights will be zeros for these steps, which a y row that is not finite would not heed
             for (int e = tid % (64 * W); e < leaving * IN * (D / 8); e += 64 * W) {
                 const int row = e / (IN * (D / 8)), at = e % (IN * (D / 8));
                 *(u32x4*)(ly + at / (D / 8) * PLANE + row * PITCH + at % (D / 8) * 8) = u32x4{0, 0, 0, 0};
@@ -719,7 +728,8 @@ __global__ void __launch_bounds__(64 * W * HEADS, walk_waves(ST, K, W, MODE)) wa
                         mma(o[c][j], T[j], P);
                     }
                     if (slow) {
-                        const unsigned sees = ((2u << n) - 1) & ~((1u << last_cut(cuts_to(n))) - 1);
+                        const int from = last_cut(cuts_to(n)), near = n + 1 - reach;
+                        const unsigned sees = ((2u << n) - 1) & ~((1u << (from > near ? from : near)) - 1);
 #pragma unroll
                         for (int j = 0; j < J; j++)
 #pragma unroll
@@ -967,6 +977,7 @@ __global__ void __launch_bounds__(256) step_kernel(StepArgs a) {
     const bool on = !a.active || a.active[b];
     const bool fresh = a.reset && a.reset[(long)b * a.reset_lane];
     const float lambda = __builtin_amdgcn_exp2f(a.log_decay[h] * 1.44269504088896340736f);
+    const bool forget = fresh || lambda == 0.f;   // (0 times what is not finite)
     const bool keep = !on && a.state_in == a.state_out;   // an idle lane's state in place stays as it is
     float o[U];
 #pragma unroll
@@ -976,7 +987,7 @@ __global__ void __launch_bounds__(256) step_kernel(StepArgs a) {
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const bool in = LPR > 1 ? c0 + j >= own : j < a.dk;
-                s[u][j] = (fresh ? 0.f : s[u][j] * lambda) + v[u] * k[j];
+                s[u][j] = (forget ? 0.f : s[u][j] * lambda) + v[u] * k[j];
                 o[u] += in ? s[u][j] * q[j] : 0.f;
             }
             o[u] = row_sum<LPR>(o[u]) * a.scale;

@@ -471,7 +471,8 @@ typedef struct {
  * query head h reads key / value head h / (heads / kv_heads).  Rows may have any alignment to their elements and any
  * strides (rows of whole 16-byte units are the fast ones).  All sums and the state are float32; an output is rounded once.
  * A value that is not finite makes NaN or an infinity of what the formula lets it reach, and of nothing else: not of
- * earlier steps, other lanes or other episodes.  Steps behind a lane's length are not read; their outputs and gradients
+ * earlier steps, other lanes or other episodes.  A weight of 0 is a mask: with log_decay -inf (or one whose exp is 0 in
+ * float32) nothing reaches later steps.  Steps behind a lane's length are not read; their outputs and gradients
  * are zeros.  log_decay is a constant schedule (<= 0; -inf: no memory), not a trained parameter: it has no gradient. */
 typedef struct {
     int32_t device, type;
