@@ -31,6 +31,13 @@ def _normc(rng, shape, std):
     return (w * std / np.sqrt(np.square(w).sum(axis=0, keepdims=True))).astype(np.float32)
 
 
+def _written(tr, out):
+    """Kernels wrote into the caller's trajectory tensors: a gradient that has saved one of them raises."""
+    if out:
+        from torch.autograd.graph import increment_version
+        increment_version([x for f, x in tr.items() if out.get(f) is x])
+
+
 class DevicePolicy:
     """The policy network on one GPU (weights fp32, TF kernel layout [in][out]); n_in -> n_out = 70 -> 17 (the
     low-level policy) or 44 -> 2 (the high-level one)."""
@@ -260,6 +267,7 @@ class DevicePolicy:
             fn = N.lib().hum_rollout_fused if fused else N.lib().hum_rollout
             N.check(fn(*args, venv._stream()), "hum_rollout_fused" if fused else "hum_rollout")
         venv._advanced()
+        _written(tr, out)
         return tr
 
 
@@ -297,6 +305,7 @@ class DevicePolicy:
             if tr:
                 tr["rewards"][i].copy_(venv.reward)
                 tr["dones"][i].copy_(venv.done)
+        _written(tr, out)
         return tr
 
 
@@ -364,6 +373,7 @@ def hier_rollout(venv, high, low, k, explore=True, step0=0, trajectories=True, f
         fn = "hum_hier_rollout_fused" if fused else "hum_hier_rollout"
         N.check(getattr(N.lib(), fn)(*args, venv._stream()), fn)
     venv._advanced()
+    _written(tr, out)
     return tr
 
 

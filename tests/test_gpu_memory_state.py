@@ -153,3 +153,21 @@ def test_a_replayed_step_ends_the_start_of_an_episode():
         torch.cuda.synchronize()
         assert not env.begun.any()
     env.close()
+
+
+@pytest.mark.parametrize("how", ["plain", "memory", "fused"])
+@pytest.mark.parametrize("field", ["obs", "actions"])
+def test_gradient_notices_that_a_trajectory_was_recorded_over(how, field):
+    """rollout(out=) writes into the trajectory a learner's pass has saved: backward() raises."""
+    n = 256
+    pol, mem, env = DevicePolicy.random_init(seed=1), M.PolicyMemory(heads=2, channels=16), HumanoidVecEnv(n, seed=2)
+    env.reset()
+    kw = dict(memory=mem, state=mem.begin(n)) if how == "memory" else dict(fused=how == "fused")
+    tr = pol.rollout(env, 2, **kw)
+    w = torch.ones(tr[field].shape[-1], device="cuda", requires_grad=True)
+    loss = (M.layer_norm(tr[field], w) if field == "obs" else tr[field] * w).sum()
+    pol.rollout(env, 2, out=tr, **kw)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    env.close()
+    pol.close()
