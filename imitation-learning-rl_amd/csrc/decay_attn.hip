@@ -23,7 +23,8 @@
 // goes to the other waves, without a change of layout.  Contractions over the steps read Y and Z back transposed.
 //
 // What bounds it (bf16, time-major rows).  Many lanes: HBM.  Forward of 4096 lanes x 32 steps, 4 heads x 64 x 64: 0.80 GB
-// in 152 us, 5.3 TB/s where a large copy reaches 5.1; gradient 1.28 GB in 297 us.  Few lanes: the latency of a chunk (LDS
+// in 153 us, 5.3 TB/s where a large copy reaches 5.1; gradient 1.28 GB in 298 to 353 us, by which of several equal sets of
+// tensors it works on.  Few lanes: the latency of a chunk (LDS
 // round trips and dependent matrix instructions), 2 to 4 us of it, since a walk is serial: so walks are cut into segments
 // (cut_of), whose states cost traffic of their own.  Forward of 1 x 8192 steps, 8 heads x 128 x 128: segments' states 19,
 // scan 13, outputs 30 us.
@@ -32,7 +33,9 @@
 // float32 as three, exactly but for 2^-27; products of parts are exact in the float32 accumulators.  Computed operands are
 // split likewise: P and the state read by O into two parts (2^-18 of the value, under the output's own 2^-9 or 2^-12; three
 // for float32), the weighted Z that enters the state into three (2^-27, below float32's 2^-24: the state is held in 32
-// bits).  An output is rounded once.
+// bits).  An output is rounded once.  These bounds hold from about 2^-109 on: the matrix cores take parts below 2^-126 as
+// zeros (float32 operands of 1e-36 are good to 1e-4), and a float32 from 2^128 - 2^119 on has an infinite first part and
+// counts as infinite.
 //
 // Non-finite values.  A row of Z multiplies zeros of P for the steps that must not see it (earlier steps, other
 // episodes, those past which lambda^d is 0), and 0 x inf is NaN: such values of z enter the products as zeros and make NaN of
@@ -194,7 +197,7 @@ template <> struct Num<HUM_F32> { typedef float T; static constexpr int IN = 3, 
 // How a walk's rows are accessed.  BUFFER: rows of whole aligned units of 16 bytes, through buffers.  WIDE: 16 bytes at any
 // alignment.  ANY: the same with 64-bit addresses and a branch for heads of fewer channels than 16 bytes hold; also steps
 // 2^25 bytes apart and more, or backwards in memory.  Gradient of 4096 x 32 steps, 4 heads, bf16: 64 channels in BUFFER
-// 301 us, 63 in WIDE 442 (60: 381), element by element 916 (900); WIDE saves 3 % against ANY
+// 300 us, 63 in WIDE 439 (60: 380; the first version, element by element, 916 and 900); WIDE saves 3 % against ANY
 enum Mode { BUFFER, WIDE, ANY };
 
 // 16 loaded bytes into the planes of an LDS tile
@@ -355,7 +358,8 @@ __device__ __forceinline__ f32x4 quad_transpose(f32x4 v) {
 }
 
 // waves per SIMD that the registers are limited for (the state takes 16 K of them): the most that fit without scratch memory,
-// a few bytes of which cost more than a wave gives (forward of 4096 x 32 steps: 162 us, 180 with 12 bytes, 186 with two waves)
+// a few bytes of which cost more than a wave gives (4096 x 32 steps, 4 heads x 64 x 64, bf16: 156 us and gradient 300 with
+// three waves, 175 and 379 with two, 228 and 509 with four and their scratch)
 constexpr int walk_waves(int st, int k, int w, Mode mode) {   // (a single wave has all of a chunk's rows in flight)
     const bool alone = k > 1 && w == 1;
     if (mode != BUFFER) return st == HUM_BF16 ? (k > 1 ? 2 : 3) : k > 2 ? 1 : 2;
@@ -365,7 +369,7 @@ constexpr int walk_waves(int st, int k, int w, Mode mode) {   // (a single wave 
 // One workgroup per HEADS neighbouring heads of a lane, role and segment; W waves per head, each with 32 of z's channels and
 // its slice of the state.  A head's waves share the chunk's x and y rows (K operands of 32 channels) and P; the heads of a
 // workgroup only share the loading, so that a load meets long pieces of few rows (with one head, 4096 lanes' time-major
-// steps lie 2 MB apart and each load meets 8 pages for 1 KB: forward 177 us, 168 us with the heads together).  OUTS: rows
+// steps lie 2 MB apart and each load meets 8 pages for 1 KB: forward 168 us, 156 us with the heads together).  OUTS: rows
 // come out (else the states of the segments are wanted only).
 template <int ST, int K, int W, int J, int HEADS, Mode MODE, bool OUTS>
 __global__ void __launch_bounds__(64 * W * HEADS, walk_waves(ST, K, W, MODE)) walk_kernel(WalkArgs a) {
@@ -390,8 +394,9 @@ __global__ void __launch_bounds__(64 * W * HEADS, walk_waves(ST, K, W, MODE)) wa
     float *const pow_pair = pows_pair[sub], *const pow_add = pows_add[sub];
     unsigned* const lodd = odds[sub][wave];
     // the roles of one segment read the same rows, and NEAR segments in a row are neighbours in memory (the heads of a lane,
-    // lanes of a time-major step): they go to one XCD, one after the other.  Gradient of 4096 lanes x 32 steps: 380 us,
-    // 407 with NEAR = 1, 377 with 32 (which leaves XCDs idle at few lanes)
+    // lanes of a time-major step): they go to one XCD, one after the other.  Gradient of 4096 lanes x 32 steps, bf16,
+    // 3 heads x 64 x 64: 212 us, 231 with NEAR = 1, 211 with 32 (which leaves XCDs idle at few lanes); 4 heads, which share a
+    // workgroup, 300 with any
     const int block = blockIdx.x, ri = block / XCDS % a.nroles, turn = block / (XCDS * a.nroles);
     const int item = (turn / NEAR * XCDS + block % XCDS) * NEAR + turn % NEAR;
     if (item >= a.lanes * a.heads / HEADS * a.segs) return;
@@ -1083,11 +1088,15 @@ void launch_walk_j(const WalkArgs& a, hipStream_t s) {
 }
 // W waves of 32 of z's channels, or 2 W of 16: half of a wave's part of a chunk, while a head's rows are read from LDS twice
 // as often.  Thin slices are faster while a wave of 32 channels has a SIMD of its own (thin: bf16, 4 heads x 64 x 64, 200 steps,
-// 64 lanes: 21.4 us with wide slices, 18.5; 128 lanes 25.7 and 22.8, 512 lanes 62 and 64), and always for types of several
-// parts (float32, 512 lanes: 146 and 125 us) and where the registers of wide slices leave a SIMD two waves or one (float16,
-// 1024 lanes x 100 steps x 127 channels: 609 and 428 us; bf16 63 channels 121 and 116, gradient 272 and 257).
+// 64 lanes: 21.2 us with wide slices, 18.3; 128 lanes 26.4 and 21.6), wide ones from there on but for some forwards (512 lanes
+// 65.5 and 62.4, gradient 136 and 149; 128 channels 163 and 195; 4096 time-major lanes x 32 steps 153 and 192, gradient 300
+// and 392).  Thin ones always for types of several parts (but float16 of more than 64 channels: gradient of 512 lanes x 100
+// steps x 128 333 and 447) and for unaligned rows of up to 64 channels or of two parts: as measured when wide slices were
+// built for them too, float32 4 x 64 x 64, 512 lanes x 200 steps 146 and 125 us, float16 1024 lanes x 100 steps x 127 609
+// and 428, bf16 63 channels 121 and 116, gradient 272 and 257.
 // Rows of more than 64 channels are work for four waves to load and to form P of, also where z has fewer channels than they
-// could hold (float32, 128 x 32 channels, 64 lanes x 100 steps: 28.9 us with two waves, 24.8 with four).
+// could hold (float32, 128 x 32 channels, 64 lanes x 100 steps: 28.9 us with two waves, 24.8 with four); with wide slices,
+// for many walks, z of up to 32 channels still has one wave, with the registers of a SIMD to itself.
 template <int ST, int K, int W, bool OUTS>
 void launch_walk_o(const WalkArgs& a, Mode mode, bool together, bool thin, hipStream_t s) {
     constexpr int THIN = K > 2 && W == 1 ? 4 : 2 * W;
@@ -1122,7 +1131,7 @@ void launch_walk_k(const WalkArgs& a, int w, Mode mode, bool together, bool thin
 template <int ST>
 void launch_walk_t(const WalkArgs& a, hipStream_t s) {
     // together: four heads of a step are neighbours and the steps so far apart that a chunk's 32 rows lie in as many pages
-    // (gradient of 4096 x 32 steps, time-major 2 MB apart: 337 us with single heads, 309 us; lane-major 263 and 284 us)
+    // (gradient of 4096 x 32 steps, time-major 2 MB apart: 333 us with single heads, 300 us; lane-major 259 and 272 us)
     bool buffers = !a.reset || (a.reset_step >= 0 && a.reset_step < (1l << 25)), wide = true, together = true;
     auto near = [](const Rows& m, int d) { return m.near && d * Num<ST>::SIZE >= 16; };
     auto within = [](const Rows& m, int d) { return m.head >= 0 && 3 * m.head + d <= m.step && m.step * Num<ST>::SIZE >= 1 << 16; };
@@ -1144,8 +1153,9 @@ void launch_walk_t(const WalkArgs& a, hipStream_t s) {
 // Few lanes and many steps: the walks are cut into segments that run side by side, each from the state that a first pass
 // over the segments before it and a scan have left for it (segments without outputs: half the work of a walk).  Longer
 // walks have longer segments (each has a state in memory and a turn in the scan) and more of them side by side; walks
-// that would be cut into few, or are short, do not gain what the first pass and two launches cost.  Averages over types,
-// widths of 32 to 128 and both directions, against the best cut of each case:
+// that would be cut into few, or are short, do not gain what the first pass and two launches cost.  The numbers are fitted to
+// measurements, there is no model behind them, and they count a.steps, not the lanes' lengths.  Averages over types, widths
+// of 32 to 128 and both directions, against the best cut of each case:
 //     12 to 24 chunks,  8 waves: uncut 2.34, segments of 1 chunk 1.00, of 4 1.67;  256 waves: uncut 1.02, up to 2048 waves 1.29
 //     32 chunks, 256 waves: uncut 1.09, 2048 waves 1.11;  63 chunks, 256 waves: uncut 1.25, 2048 1.09, 4096 1.06
 //     125 chunks, 512 waves: uncut 1.06, 4096 1.02;  250 chunks, 16 waves: segments of 1 chunk 1.13, 2 1.10, 3 1.00, 4 1.09

@@ -11,8 +11,9 @@
 // row pair per workgroup; a second launch adds those in float64 in a fixed order (no atomics: the same bits each run).
 // All sums are float32 or wider; y, dx are rounded once to the rows' type, dw, db once to the weights'.
 //
-// 131072 x 256 bf16: forward 0.13 GB in 24 us, 5.5 TB/s (a large copy: 5.1); backward 0.20 GB in 41 us and 4 us of the
-// second launch.  4099 x 1111 float32 at a pitch of 1148: backward 14 and 4 us for 55 MB.  One row: 8 us, the host's.
+// 131072 x 256 bf16: forward 0.13 GB in 24 us, 5.5 TB/s (a large copy: 5.1); backward 0.20 GB in 44 us a call: 35 (part of
+// the rows come from the last cache) and 4 of the second launch, and what lies between launches.  4099 x 1111 float32 at a
+// pitch of 1148: backward 15 and 4 us for 55 MB.  One row: 8 us, the host's.
 #include <hip/hip_runtime.h>
 
 #include <cmath>

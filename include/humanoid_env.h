@@ -470,6 +470,8 @@ typedef struct {
  * q [lanes, steps, heads, dk], k [lanes, steps, kv_heads, dk], v [lanes, steps, kv_heads, dv] of element type `type`;
  * query head h reads key / value head h / (heads / kv_heads).  Rows may have any alignment to their elements and any
  * strides (rows of whole 16-byte units are the fast ones).  All sums and the state are float32; an output is rounded once.
+ * Fragments of float32 are exact to float32's rounding for magnitudes from 2^-109 on (parts of operands below 2^-126 count
+ * as zeros); from 2^128 - 2^119 on they count as infinite.
  * A value that is not finite makes NaN or an infinity of what the formula lets it reach, and of nothing else: not of
  * earlier steps, other lanes or other episodes.  A weight of 0 is a mask: with log_decay -inf (or one whose exp is 0 in
  * float32) nothing reaches later steps.  Steps behind a lane's length are not read; their outputs and gradients
