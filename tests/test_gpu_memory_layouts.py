@@ -88,3 +88,31 @@ def test_norm_into_its_input_or_beside_it():
     assert torch.equal(y, want[:rows // 2])
     M.layer_norm_forward(half[0], out=half[0])
     assert torch.equal(half[0], half[1])
+
+
+def test_calls_of_two_threads_on_their_own_streams():
+    """Nothing is shared between calls: every thread gets what it gets alone, refusals of one do not reach the other."""
+    import threading
+    cases = [Case(3, 431, 2, 1, 40, 72, kind="bf16", resets=0.01), Case(40, 45, 4, 2, 32, 32, kind="fp32", order="time", resets=0.05)]
+    alone = [c.forward() + c.backward() for c in cases]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(c, want):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got = c.forward() + c.backward()
+                    x = torch.ones(5, 64, device="cuda")
+                    with pytest.raises(N.NativeError, match="hum_layer_norm: .*overlap"):
+                        M.layer_norm_forward(x, x[2], out=x)
+                    torch.cuda.current_stream().synchronize()
+                    assert all(torch.equal(a, b) for a, b in zip(got, want))
+        except BaseException as e:   # (else the thread would end without the test knowing)
+            wrong.append(e)
+    threads = [threading.Thread(target=work, args=a) for a in zip(cases, alone)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong
