@@ -483,8 +483,14 @@ class PolicyMemory:
 
     def forward(self, obs, state=None, reset=None, lengths=None):
         """(features [steps, lanes, n_in], final state) for a fragment's observations obs [steps, lanes, n_in] from the
-        state before its first step; reset [steps, lanes] as in step; lengths [lanes]: steps held (RLlib's seq_lens)."""
-        q, k, v = (x.transpose(0, 1) for x in self._project(obs))
+        state before its first step; reset [steps, lanes] as in step; lengths [lanes]: steps held (RLlib's seq_lens), the
+        observations behind them may be anything."""
+        t, seen = _e().t, obs
+        if lengths is not None:   # what pads a lane passes the norm and the product, whose gradients would meet it with zeros
+            _on(lengths, obs.device, "lengths", tuple(obs.shape[1:2]), (t.int32,))
+            held = t.arange(obs.shape[0], device=obs.device)[:, None] < lengths
+            seen = t.where(held[..., None], obs, t.zeros((), dtype=obs.dtype, device=obs.device))
+        q, k, v = (x.transpose(0, 1) for x in self._project(seen))
         out, state = decay_attention(q, k, v, self.log_decay, state=state,
                                      reset=reset.transpose(0, 1) if reset is not None else None, lengths=lengths)
         return self._join(obs, out.transpose(0, 1)), state

@@ -171,3 +171,34 @@ def test_gradient_notices_that_a_trajectory_was_recorded_over(how, field):
         loss.backward()
     env.close()
     pol.close()
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_padding_that_is_not_finite_stays_out_of_the_gradients(bad):
+    """Observations behind a lane's length are whatever the batch holds there: the held steps' features and every parameter's
+    gradient are what they are with zeros in their place."""
+    k, n = 40, 6
+    mem = M.PolicyMemory(heads=2, channels=16, seed=3)
+    with torch.no_grad():
+        mem.w_out += 0.1 * rows(32, 70, seed=8)
+    obs, weight = rows(k, n, 70), rows(k, n, 70, seed=1)
+    lengths = torch.tensor([40, 0, 1, 33, 17, 39], dtype=torch.int32, device="cuda")
+    held = (torch.arange(k, device="cuda")[:, None] < lengths)[..., None]
+    runs = []
+    for pad in (0.0, bad):
+        x = torch.where(held, obs, torch.full_like(obs, pad)).requires_grad_(True)
+        f, state = mem.forward(x, state=rows(n, 2, 16, 16, seed=2), lengths=lengths)
+        loss = torch.where(held, f * weight, torch.zeros_like(f)).sum() + state.sum()
+        runs.append((torch.where(held, f, torch.zeros_like(f)), state) + torch.autograd.grad(loss, mem.parameters() + [x]))
+    for a, b in zip(*runs):
+        assert torch.equal(a, b)
+    assert all(g.isfinite().all() for g in runs[1])
+
+
+def test_lengths_of_the_core_are_checked():
+    mem, obs = M.PolicyMemory(heads=2, channels=16), rows(4, 3, 70)
+    ok = torch.tensor([4, 2, 0], dtype=torch.int32, device="cuda")
+    assert mem.forward(obs, lengths=ok)[0].shape == (4, 3, 70)
+    for bad in (ok.long(), ok[:2], ok.cpu(), ok[:, None]):
+        with pytest.raises(ValueError, match="lengths"):
+            mem.forward(obs, lengths=bad)
